@@ -52,6 +52,12 @@ typedef enum tf_rope_style {
   TF_ROPE_ROTATE_HALF = 1  /* pairs (k, k + D/2) */
 } tf_rope_style;
 
+typedef enum tf_act {
+  TF_ACT_SILU = 0,      /* g / (1 + exp(-g)): the reference's SwiGLU (swiglu.rs:56-95) */
+  TF_ACT_GELU = 1,      /* g * Phi(g), the error-function form */
+  TF_ACT_GELU_TANH = 2  /* g / 2 * (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+} tf_act;
+
 /* ---------------- library ---------------- */
 
 TF_API int tf_b200_version(void);
@@ -270,6 +276,79 @@ TF_API int tf_b200_gemm_qkv_rope_bf16(const void* x, const void* w_qkv, void* q,
  * (m / world) % 128 == 0; world <= 8. */
 TF_API int tf_b200_gemm_push_bf16(const void* a, const void* b, void* const* peer_recv, int m,
                                   int n, int k, int a_seq, int rank, int world, void* stream);
+
+/* ---------------- gated feed-forward block, forward and backward (tcgen05) ----------------
+ * The whole feed-forward of a block (src/layers/ffn.rs:47-56 around swiglu.rs:56-95):
+ *   [g | u] = x [Wg; Wu]^T,  a = act(g) * u,  y = a Wd^T (+ residual)
+ *   x, residual, y [m, d_model]; w_gate_up [2 * d_ff, d_model] = [gate rows; up rows], the
+ *   layer's own layout; w_down [d_model, d_ff]; all bf16 row-major.
+ *   a [m, d_ff] bf16: scratch, written (the activations).
+ *   z [m, 2 * d_ff] fp32 or NULL: [g | u] as accumulated, written for the backward pass.
+ *   residual: NULL, or added to the fp32 product before y's one rounding; y may be residual.
+ * act: tf_act.  d_model % 8 == 0, d_ff % 8 == 0, 16-byte aligned pointers; m == 0 is a no-op.
+ * Any m from one token on: few tokens take a kernel that streams the weights once. */
+TF_API int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, const void* w_down,
+                                      const void* residual, void* a, float* z, void* y, int m,
+                                      int d_model, int d_ff, int act, void* stream);
+/* Its backward pass (the gradient chain of ffn.rs:47-56 with swiglu.rs:98-136):
+ *   da = dy Wd, [dg | du] = [da u act'(g) | da act(g)]
+ *   dx = [dg | du] [Wg; Wu], dw_gate_up = [dg | du]^T x, dw_down = dy^T a   (bf16, rounded once;
+ *   fully written, repeatable bit for bit).
+ * z: the forward's; a is computed again from it.  dx NULL skips it; dw_gate_up and dw_down are
+ * given or NULL each.  workspace: tf_b200_gated_ffn_bwd_workspace_size(m, d_ff) bytes, 16-byte
+ * aligned.  m == 0: the weights' gradients are zero. */
+TF_API size_t tf_b200_gated_ffn_bwd_workspace_size(int m, int d_ff);
+TF_API int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, const void* w_down,
+                                      const float* z, const void* dy, void* dx, void* dw_gate_up,
+                                      void* dw_down, void* workspace, int m, int d_model, int d_ff,
+                                      int act, void* stream);
+
+/* ---------------- the norms around a block, with its gate, scales and dropout ----------------
+ *   n = RMSNorm(f) * w_post        (w_post NULL: n = f)
+ *   y = residual_scale * x + branch_scale * dropout(gate * n)      (f NULL: y = x, not written)
+ *   h = RMSNorm(y) * w_pre         (w_pre NULL: no h)
+ * x (residual stream), f (the block's output), y, h [rows, cols] bf16; w_post, w_pre [cols] bf16;
+ * gate [gate_rows, cols] bf16 or NULL, one row for each rows / gate_rows consecutive rows
+ * (gate_rows 1: one gate; the number of sequences; rows: one a token); RMSNorm as in
+ * tf_b200_rmsnorm_bf16 (fused_add_rmsnorm.rs:53-110).  y may be x.
+ * Dropout: drop_p is the probability of dropping, 0 for none; rng is a device pointer to two
+ * 64-bit words (seed, offset), 8-byte aligned (NULL only when drop_p == 0); `site` tells the
+ * dropouts of one step apart.  See tf_b200_dropout_bf16.
+ * cols % 8 == 0, <= 8192. */
+TF_API int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const void* w_post,
+                                       const void* gate, const void* w_pre, void* y, void* h,
+                                       const void* rng, int rows, int cols, int gate_rows,
+                                       float eps, float residual_scale, float branch_scale,
+                                       float drop_p, unsigned site, void* stream);
+/* Its backward pass: from dy (the gradient of y; NULL: zero) and dh (of h; with w_pre) to dx, df,
+ * dw_post, dgate, dw_pre (bf16, each required where its tensor was given; fully written,
+ * repeatable bit for bit).  f and y are the forward's (f may be NULL when neither w_post nor gate
+ * is given, y when w_pre is not); df NULL: the forward had no f.  rng, drop_p and site as in the
+ * forward: the mask is drawn again.  dx may be dy.
+ * workspace: tf_b200_block_norm_bwd_workspace_size(rows, cols) bytes, 16-byte aligned. */
+TF_API size_t tf_b200_block_norm_bwd_workspace_size(int rows, int cols);
+TF_API int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const void* dy,
+                                       const void* dh, const void* w_post, const void* gate,
+                                       const void* w_pre, void* dx, void* df, void* dw_post,
+                                       void* dgate, void* dw_pre, const void* rng, void* workspace,
+                                       int rows, int cols, int gate_rows, float eps,
+                                       float residual_scale, float branch_scale, float drop_p,
+                                       unsigned site, void* stream);
+
+/* ---------------- dropout, its mask never stored ----------------
+ * y[i] = (kept(i) ? x[i] * 65536 / t : 0) (+ residual[i]), t = floor((1 - p) * 65536 + 1/2):
+ * element i is kept iff its 16 bits are below t.  The bits are those of Philox4x32-10 (Salmon,
+ * Moraes, Dror, Shaw, 2011) with key `seed` and counter (i / 8, site, offset low, offset high);
+ * element i has half i % 8 of the 128 bits, low halves first.  The probability is so rounded to a
+ * multiple of 2^-16, and the scale belongs to the rounded one.
+ * The backward pass is the same call on the gradient.  rng: device pointer to (seed, offset), two
+ * 64-bit words, read when the kernel runs, so a captured graph draws new masks when they change.
+ * n <= 2^35; x, residual (or NULL) and y are 16-byte aligned and may be the same buffer.
+ * p in [0, 1]; p == 0 needs no rng. */
+TF_API int tf_b200_dropout_bf16(const void* x, const void* residual, void* y, const void* rng,
+                                size_t n, float p, unsigned site, void* stream);
+TF_API int tf_b200_dropout_f32(const float* x, const float* residual, float* y, const void* rng,
+                               size_t n, float p, unsigned site, void* stream);
 
 #ifdef __cplusplus
 }

@@ -91,6 +91,31 @@ pub mod ffi {
         pub fn tf_b200_gemm_push_bf16(a: *const c_void, b: *const c_void,
             peer_recv: *const *mut c_void, m: c_int, n: c_int, k: c_int, a_seq: c_int, rank: c_int,
             world: c_int, stream: *mut c_void) -> c_int;
+        pub fn tf_b200_gated_ffn_fwd_bf16(x: *const c_void, w_gate_up: *const c_void,
+            w_down: *const c_void, residual: *const c_void, a: *mut c_void, z: *mut f32,
+            y: *mut c_void, m: c_int, d_model: c_int, d_ff: c_int, act: c_int,
+            stream: *mut c_void) -> c_int;
+        pub fn tf_b200_gated_ffn_bwd_workspace_size(m: c_int, d_ff: c_int) -> usize;
+        pub fn tf_b200_gated_ffn_bwd_bf16(x: *const c_void, w_gate_up: *const c_void,
+            w_down: *const c_void, z: *const f32, dy: *const c_void, dx: *mut c_void,
+            dw_gate_up: *mut c_void, dw_down: *mut c_void, workspace: *mut c_void, m: c_int,
+            d_model: c_int, d_ff: c_int, act: c_int, stream: *mut c_void) -> c_int;
+        pub fn tf_b200_block_norm_fwd_bf16(x: *const c_void, f: *const c_void,
+            w_post: *const c_void, gate: *const c_void, w_pre: *const c_void, y: *mut c_void,
+            h: *mut c_void, rng: *const c_void, rows: c_int, cols: c_int, gate_rows: c_int,
+            eps: f32, residual_scale: f32, branch_scale: f32, drop_p: f32, site: u32,
+            stream: *mut c_void) -> c_int;
+        pub fn tf_b200_block_norm_bwd_workspace_size(rows: c_int, cols: c_int) -> usize;
+        pub fn tf_b200_block_norm_bwd_bf16(f: *const c_void, y: *const c_void, dy: *const c_void,
+            dh: *const c_void, w_post: *const c_void, gate: *const c_void, w_pre: *const c_void,
+            dx: *mut c_void, df: *mut c_void, dw_post: *mut c_void, dgate: *mut c_void,
+            dw_pre: *mut c_void, rng: *const c_void, workspace: *mut c_void, rows: c_int,
+            cols: c_int, gate_rows: c_int, eps: f32, residual_scale: f32, branch_scale: f32,
+            drop_p: f32, site: u32, stream: *mut c_void) -> c_int;
+        pub fn tf_b200_dropout_bf16(x: *const c_void, residual: *const c_void, y: *mut c_void,
+            rng: *const c_void, n: usize, p: f32, site: u32, stream: *mut c_void) -> c_int;
+        pub fn tf_b200_dropout_f32(x: *const f32, residual: *const f32, y: *mut f32,
+            rng: *const c_void, n: usize, p: f32, site: u32, stream: *mut c_void) -> c_int;
     }
 }
 
@@ -111,6 +136,11 @@ pub enum Status {
 /// reference's RoPE (src/kernels/rope.rs); rotate-half pairs (k, k + D/2).
 pub const ROPE_INTERLEAVED: c_int = 0;
 pub const ROPE_ROTATE_HALF: c_int = 1;
+
+/// `tf_act` of the header: SiLU is the reference's SwiGLU (src/kernels/swiglu.rs).
+pub const ACT_SILU: c_int = 0;
+pub const ACT_GELU: c_int = 1;
+pub const ACT_GELU_TANH: c_int = 2;
 
 /// Turns a status code into `anyhow::Result`, with the library's message.
 pub fn check(rc: c_int) -> anyhow::Result<()> {

@@ -22,10 +22,15 @@ TF_ERR_DEVICE_TIMEOUT = -6
 TF_ROPE_INTERLEAVED = 0
 TF_ROPE_ROTATE_HALF = 1
 
+TF_ACT_SILU = 0
+TF_ACT_GELU = 1
+TF_ACT_GELU_TANH = 2
+
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
 SZ = ctypes.c_size_t
+U = ctypes.c_uint
 
 # name -> (restype, argtypes), in header order
 SIGNATURES = {
@@ -53,6 +58,14 @@ SIGNATURES = {
     "tf_b200_rope_table_f32": (I, [P, I, I, F, P]),
     "tf_b200_gemm_qkv_rope_bf16": (I, [P] * 6 + [I] * 6 + [P]),
     "tf_b200_gemm_push_bf16": (I, [P, P, ctypes.POINTER(ctypes.c_void_p)] + [I] * 6 + [P]),
+    "tf_b200_gated_ffn_fwd_bf16": (I, [P] * 7 + [I] * 4 + [P]),
+    "tf_b200_gated_ffn_bwd_workspace_size": (SZ, [I, I]),
+    "tf_b200_gated_ffn_bwd_bf16": (I, [P] * 9 + [I] * 4 + [P]),
+    "tf_b200_block_norm_fwd_bf16": (I, [P] * 8 + [I] * 3 + [F] * 4 + [U, P]),
+    "tf_b200_block_norm_bwd_workspace_size": (SZ, [I, I]),
+    "tf_b200_block_norm_bwd_bf16": (I, [P] * 14 + [I] * 3 + [F] * 4 + [U, P]),
+    "tf_b200_dropout_bf16": (I, [P] * 4 + [SZ, F, U, P]),
+    "tf_b200_dropout_f32": (I, [P] * 4 + [SZ, F, U, P]),
 }
 
 

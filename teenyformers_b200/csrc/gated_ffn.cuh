@@ -1,0 +1,733 @@
+// gated_ffn.cuh -- the gated feed-forward block and its backward pass on the
+// 5th-generation tensor cores (bf16 operands, fp32 accumulation in TMEM).
+//
+//   z = x W^T, W = [Wg; Wu] [2F, d], z = [g | u]       a = act(g) * u
+//   y = a Wd^T (+ residual)
+//   da = dy Wd     dg = da u act'(g)    du = da act(g)    dz = [dg | du]
+//   dx = dz W      dW = dz^T x          dWd = dy^T a
+// (teenyformers' FFN: src/layers/ffn.rs:47-56 around src/kernels/swiglu.rs:56-136.)
+//
+// Rounding: z leaves the accumulators in fp32 when it is saved for the
+// backward pass, which recomputes a from it bit for bit (so a need not be
+// kept); a, dz and every result are rounded once to bf16, as operands of the
+// next product or as outputs.  With z in bf16 the gradients' error against
+// the formulas in 64 bits grows from 1.4 to 1.8 output roundings.
+//
+// Two kernels:
+//   ffn_pair_kernel    persistent CTA pairs (cta_group::2), 256 x 256 tiles;
+//                      the structure of gemm_sm100.cuh's kernel with operands
+//                      of either major and several products in one launch
+//   ffn_token_kernel   few tokens: the weight rows are the MMA's M, the tokens
+//                      its N; K is split over a cluster and joined through
+//                      distributed shared memory
+#pragma once
+
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "gemm_sm100.cuh"
+#include "norm_act.cuh"
+#include "sm100.cuh"
+
+namespace tfb {
+
+enum FfnAct : int { FFN_ACT_SILU = 0, FFN_ACT_GELU = 1, FFN_ACT_GELU_TANH = 2 };
+
+// act(g)
+template <int ACT>
+__device__ __forceinline__ float ffn_act(float g) {
+  if constexpr (ACT == FFN_ACT_SILU) {
+    return g / (1.0f + __expf(-g));
+  } else if constexpr (ACT == FFN_ACT_GELU) {
+    return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+  } else {
+    // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), v = sqrt(2/pi) (g + 0.044715 g^3)
+    const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
+    return g / (1.0f + __expf(-2.0f * v));
+  }
+}
+
+// act(g) and act'(g)
+template <int ACT>
+__device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope) {
+  if constexpr (ACT == FFN_ACT_SILU) {
+    const float s = 1.0f / (1.0f + __expf(-g));
+    value = ffn_act<ACT>(g);
+    slope = s * (1.0f + g * (1.0f - s));
+  } else if constexpr (ACT == FFN_ACT_GELU) {
+    value = ffn_act<ACT>(g);
+    slope = 0.5f * (1.0f + erff(g * 0.70710678118654752f)) +
+            g * 0.39894228040143268f * __expf(-0.5f * g * g);
+  } else {
+    const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
+    const float s = 1.0f / (1.0f + __expf(-2.0f * v));
+    value = ffn_act<ACT>(g);
+    slope = s + g * s * (1.0f - s) * 2.0f * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
+  }
+}
+
+__device__ __forceinline__ float ffn_act_rt(int act, float g) {
+  if (act == FFN_ACT_SILU) return ffn_act<FFN_ACT_SILU>(g);
+  if (act == FFN_ACT_GELU) return ffn_act<FFN_ACT_GELU>(g);
+  return ffn_act<FFN_ACT_GELU_TANH>(g);
+}
+
+// ===================================================================== CTA pairs
+enum FfnMode : int {
+  FFN_GLU = 0,    // A = x, B = W (gate rows to the even CTA, up rows to the odd one): a (, z)
+  FFN_DGLU = 1,   // A = dy, B = Wd read MN-major: dz and a from z and the product da
+  FFN_STORE = 2,  // up to three products, each rounded to bf16 (+ residual)
+};
+
+constexpr int kFfnMaxProblems = 3;
+
+// One product D[M, N] = A[M, K] B[N, K]^T.  Either operand may be stored with
+// its M / N index innermost (a_mn / b_mn: rows of the stored matrix are K).
+struct FfnProblem {
+  int M, N, n_mblk, n_nblk, n_kblk, n_tiles, group_m;
+  int a_mn, b_mn;
+  __nv_bfloat16* out;             // FFN_STORE: [M, N]
+  const __nv_bfloat16* residual;  // FFN_STORE: [M, N] or null
+};
+
+struct FfnPairParams {
+  FfnProblem prob[kFfnMaxProblems];
+  int n_prob;
+  // static schedule (ffn_next): T0 tiles of the longer K, then `light` tiles
+  int heavy, light, bal_rounds;
+  // FFN_GLU / FFN_DGLU
+  int F;
+  __nv_bfloat16* a;   // [M, F]
+  float* z;           // [M, 2F]; null in FFN_GLU: not saved
+  __nv_bfloat16* dz;  // [M, 2F]
+};
+
+struct FfnMaps {
+  CUtensorMap a[kFfnMaxProblems], b[kFfnMaxProblems];
+};
+
+// The i-th tile of a pair, in the concatenated list of all products' tiles
+// (those with the longer K first); -1 at the end.  Heavy tiles go round robin;
+// the pairs that get one fewer of them (those from heavy % n_pairs on) then
+// take bal_rounds light tiles each, about one heavy tile's work, before the
+// round robin over all pairs goes on.
+__device__ __forceinline__ int ffn_next(const FfnPairParams& p, int pair, int n_pairs, int i) {
+  const int mine = pair < p.heavy ? (p.heavy - 1 - pair) / n_pairs + 1 : 0;
+  if (i < mine) return pair + i * n_pairs;
+  int j = i - mine;
+  const int r = p.heavy % n_pairs, q = n_pairs - r;
+  int first = 0;
+  if (p.bal_rounds > 0) {
+    first = p.bal_rounds * q;
+    if (pair >= r) {
+      if (j < p.bal_rounds) return p.heavy + j * q + (pair - r);
+      j -= p.bal_rounds;
+    }
+  }
+  const long long l = (long long)first + pair + (long long)j * n_pairs;
+  return l < p.light ? p.heavy + (int)l : -1;
+}
+
+// Tile of the list -> product, row block and column block (grouped order).
+__device__ __forceinline__ int ffn_tile(const FfnPairParams& p, int t, int& mb, int& nb) {
+  int k = 0;
+  while (k + 1 < p.n_prob && t >= p.prob[k].n_tiles) {
+    t -= p.prob[k].n_tiles;
+    ++k;
+  }
+  const FfnProblem& q = p.prob[k];
+  const int per_group = q.group_m * q.n_nblk;
+  const int g = t / per_group;
+  const int m_first = g * q.group_m;
+  const int gm = min(q.group_m, q.n_mblk - m_first);
+  const int local = t - g * per_group;
+  mb = m_first + local % gm;
+  nb = local / gm;
+  return k;
+}
+
+// Stages a warp's 32 rows x 32 columns of fp32 (row = lane) as 128-byte rows of
+// 16-byte chunks XOR-swizzled by row.
+__device__ __forceinline__ void ffn_stage32(uint32_t stg, const uint32_t (&r)[32], int lane) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    gemm_sts128(stg + lane * 128 + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2],
+                r[4 * j + 3]);
+}
+// ... and reads them back 4 columns a lane: iteration `it` gives row it * 4 +
+// lane / 8, columns 4 (lane % 8)..
+__device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) {
+  const int rr = it * 4 + (lane >> 3);
+  const uint4 v = gemm_lds128(stg + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
+                     __uint_as_float(v.w));
+}
+
+// Epilogue of one accumulator tile for one warp: TMEM columns acc.. (this
+// warp's lane quarter), output rows row0..row0+31, column block nb.
+template <int MODE, int ACT, class Release>
+__device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
+                                                  uint32_t acc, int row0, int nb, int lane,
+                                                  uint32_t stg, Release&& release_acc) {
+  if (row0 >= q.M) {
+    release_acc();
+    return;
+  }
+  const int rows_valid = q.M - row0;
+  if constexpr (MODE == FFN_GLU) {
+    // columns 0..127 of the accumulator are gate, 128..255 up of outputs 128 nb..
+    const uint32_t stg_z = stg + 4096;
+    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
+    __nv_bfloat16* a_row0 = p.a + (long long)row0 * p.F;
+    for (int c = 0; c < 2; ++c) {
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t gr[32], ur[32];
+        tmem_ld32(acc + c * 64 + hh * 32, gr);
+        tmem_ld32(acc + 128 + c * 64 + hh * 32, ur);
+        tmem_wait_ld();
+        if (c == 1 && hh == 1) release_acc();
+#pragma unroll
+        for (int jc = 0; jc < 4; ++jc) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 8 * jc + 2 * e;
+            w[e] = pack_bf16x2(
+                ffn_act<ACT>(__uint_as_float(gr[k])) * __uint_as_float(ur[k]),
+                ffn_act<ACT>(__uint_as_float(gr[k + 1])) * __uint_as_float(ur[k + 1]));
+          }
+          gemm_sts128(stg + lane * 128 + (((hh * 4 + jc) ^ (lane & 7)) << 4), w[0], w[1], w[2],
+                      w[3]);
+        }
+        if (p.z) {
+          const int col = nb * 128 + c * 64 + hh * 32 + c4;
+          for (int half = 0; half < 2; ++half) {
+            if (half == 0)
+              ffn_stage32(stg_z, gr, lane);
+            else
+              ffn_stage32(stg_z, ur, lane);
+            __syncwarp();
+            float* z_row0 = p.z + (long long)row0 * 2 * p.F + (half ? p.F : 0);
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+              const float4 v = ffn_unstage32(stg_z, it, lane);
+              const int rr = it * 4 + r4;
+              if (rr < rows_valid && col < p.F)
+                *reinterpret_cast<float4*>(z_row0 + (long long)rr * 2 * p.F + col) = v;
+            }
+            __syncwarp();
+          }
+        }
+      }
+      __syncwarp();
+      const int col0 = nb * 128 + c * 64;
+      gemm_store_rows64(stg, a_row0 + col0, nullptr, p.F, lane, rows_valid, p.F - col0);
+      __syncwarp();
+    }
+  } else if constexpr (MODE == FFN_DGLU) {
+    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
+    for (int c = 0; c < kGemmBN / 32; ++c) {
+      const int col = nb * kGemmBN + c * 32 + c4;
+      float4 g[8], u[8];
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < p.F) {
+          const float* zr = p.z + (long long)(row0 + rr) * 2 * p.F + col;
+          g[it] = *reinterpret_cast<const float4*>(zr);
+          u[it] = *reinterpret_cast<const float4*>(zr + p.F);
+        }
+      }
+      uint32_t r[32];
+      tmem_ld32(acc + c * 32, r);
+      tmem_wait_ld();
+      if (c == kGemmBN / 32 - 1) release_acc();
+      const uint32_t sb = stg + (c & 1) * 4096;
+      ffn_stage32(sb, r, lane);
+      __syncwarp();
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const float4 d4 = ffn_unstage32(sb, it, lane);
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < p.F) {
+          const float d[4] = {d4.x, d4.y, d4.z, d4.w};
+          const float gv[4] = {g[it].x, g[it].y, g[it].z, g[it].w};
+          const float uv[4] = {u[it].x, u[it].y, u[it].z, u[it].w};
+          float dg[4], du[4], av[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float value, slope;
+            ffn_act_grad<ACT>(gv[e], value, slope);
+            av[e] = value * uv[e];
+            du[e] = d[e] * value;
+            dg[e] = d[e] * uv[e] * slope;
+          }
+          const long long row = row0 + rr;
+          *reinterpret_cast<uint2*>(p.dz + row * 2 * p.F + col) =
+              make_uint2(pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3]));
+          *reinterpret_cast<uint2*>(p.dz + row * 2 * p.F + p.F + col) =
+              make_uint2(pack_bf16x2(du[0], du[1]), pack_bf16x2(du[2], du[3]));
+          *reinterpret_cast<uint2*>(p.a + row * p.F + col) =
+              make_uint2(pack_bf16x2(av[0], av[1]), pack_bf16x2(av[2], av[3]));
+        }
+      }
+    }
+  } else if (q.residual) {
+    // the residual is added to the fp32 product: one rounding
+    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
+    for (int c = 0; c < kGemmBN / 32; ++c) {
+      uint32_t r[32];
+      tmem_ld32(acc + c * 32, r);
+      tmem_wait_ld();
+      if (c == kGemmBN / 32 - 1) release_acc();
+      const uint32_t sb = stg + (c & 1) * 4096;
+      ffn_stage32(sb, r, lane);
+      __syncwarp();
+      const int col = nb * kGemmBN + c * 32 + c4;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const float4 v = ffn_unstage32(sb, it, lane);
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < q.N) {
+          const long long at = (long long)(row0 + rr) * q.N + col;
+          const uint2 w = *reinterpret_cast<const uint2*>(q.residual + at);
+          *reinterpret_cast<uint2*>(q.out + at) = make_uint2(
+              pack_bf16x2(v.x + __uint_as_float(w.x << 16),
+                          v.y + __uint_as_float(w.x & 0xFFFF0000u)),
+              pack_bf16x2(v.z + __uint_as_float(w.y << 16),
+                          v.w + __uint_as_float(w.y & 0xFFFF0000u)));
+        }
+      }
+    }
+  } else {
+    for (int c = 0; c < kGemmBN / 64; ++c) {
+      uint32_t r0[32], r1[32];
+      tmem_ld32(acc + c * 64, r0);
+      tmem_ld32(acc + c * 64 + 32, r1);
+      tmem_wait_ld();
+      if (c == kGemmBN / 64 - 1) release_acc();
+      const uint32_t sb = stg + (c & 1) * 4096;
+#pragma unroll
+      for (int jc = 0; jc < 8; ++jc) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 8 * jc + 2 * e;
+          w[e] = pack_bf16x2(__uint_as_float(k < 32 ? r0[k] : r1[k - 32]),
+                             __uint_as_float(k + 1 < 32 ? r0[k + 1] : r1[k + 1 - 32]));
+        }
+        gemm_sts128(sb + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+      const int col0 = nb * kGemmBN + c * 64;
+      gemm_store_rows64(sb, q.out + (long long)row0 * q.N + col0, nullptr, q.N, lane, rows_valid,
+                        q.N - col0);
+      __syncwarp();
+    }
+  }
+}
+
+// Roles, barriers, ring and TMEM as in gemm_bf16_sm100_pair_kernel.  A k-block
+// of an operand with its M / N index innermost arrives as two 64 (K) x 64
+// (M / N) boxes: 128-byte rows of K, swizzled, which the MMA reads MN-major
+// (8 KB between the 64-column halves, 1 KB between groups of 8 K rows, 2 KB a
+// K step of 16).
+template <int MODE, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+    ffn_pair_kernel(const __grid_constant__ FfnMaps maps,
+                    const __grid_constant__ FfnPairParams p) {
+  using C = GemmPairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;  // same offset in both CTAs
+  uint8_t* sptr = smem_raw + (sbase - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sptr + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PB_COUNT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const bool leader = crank == 0;
+  const int pair = (int)cluster_id_x(), n_pairs = (int)cluster_count_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(bar(PB_FULL + s), 1);
+      mbar_init(bar(PB_EMPTY + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(PB_AFULL + b), 1);
+      mbar_init(bar(PB_AEMPTY + b), 8);  // 4 epilogue warps x 2 CTAs
+    }
+    mbar_init(bar(PB_DRAIN), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), C::TM_COLS);
+    tmem_relinquish_pair();
+  }
+  if (warp == 0 && lane < p.n_prob) {
+    tma_prefetch_desc(&maps.a[lane]);
+    tma_prefetch_desc(&maps.b[lane]);
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers initialised before any remote signal
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ===================== TMA producer (both CTAs) =====================
+    const uint32_t full0 = mapa_cta(bar(PB_FULL), 0);  // the even CTA's FULL[0]
+    int g = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const int t = ffn_next(p, pair, n_pairs, i);
+      if (t < 0) break;
+      int mb, nb;
+      const int k = ffn_tile(p, t, mb, nb);
+      const FfnProblem& q = p.prob[k];
+      const CUtensorMap* tm_a = &maps.a[k];
+      const CUtensorMap* tm_b = &maps.b[k];
+      const int m0 = mb * 256 + (int)crank * 128;  // this CTA's rows of A
+      const int n0 = MODE == FFN_GLU ? nb * 128 + (int)crank * p.F  // gate rows | up rows
+                                     : nb * 256 + (int)crank * 128;
+      const bool a_mn = q.a_mn, b_mn = q.b_mn;
+      for (int kb = 0; kb < q.n_kblk; ++kb, ++g) {
+        const int s = g % kPairStages, u = g / kPairStages;
+        if (u > 0) ok = mbar_wait_warp(bar(PB_EMPTY + s), (u - 1) & 1, abort_flag, 921);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t sa = sbase + s * C::STAGE_BYTES;
+          const uint32_t fb = full0 + s * 8;
+          if (leader) mbar_arrive_expect_tx(bar(PB_FULL + s), 2 * C::STAGE_BYTES);
+          if (a_mn) {
+            tma_load_2d_pair(sa, tm_a, fb, m0, kb * kGemmBK);
+            tma_load_2d_pair(sa + 8192, tm_a, fb, m0 + 64, kb * kGemmBK);
+          } else {
+            tma_load_2d_pair(sa, tm_a, fb, kb * kGemmBK, m0);
+          }
+          if (b_mn) {
+            tma_load_2d_pair(sa + C::A_BYTES, tm_b, fb, n0, kb * kGemmBK);
+            tma_load_2d_pair(sa + C::A_BYTES + 8192, tm_b, fb, n0 + 64, kb * kGemmBK);
+          } else {
+            tma_load_2d_pair(sa + C::A_BYTES, tm_b, fb, kb * kGemmBK, n0);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (leader) {
+        // the last copies counted on each stage (both CTAs') land first
+        for (int s = 0; s < kPairStages; ++s) {
+          const int n_s = g > s ? (g - s - 1) / kPairStages + 1 : 0;
+          if (n_s) (void)mbar_wait(bar(PB_FULL + s), (n_s - 1) & 1, nullptr, 922);
+        }
+      } else {
+        // the odd CTA cannot see the even CTA's barrier: give copies in flight
+        // into its own shared memory time to land
+        __nanosleep(200000);
+      }
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer (even CTA only) ===================
+    if (leader) {
+      int g = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const int t = ffn_next(p, pair, n_pairs, i);
+        if (t < 0) break;
+        int mb, nb;
+        const FfnProblem& q = p.prob[ffn_tile(p, t, mb, nb)];
+        const int a_mn = q.a_mn, b_mn = q.b_mn, n_kblk = q.n_kblk;
+        const uint32_t idesc = make_idesc_bf16(256, kGemmBN, a_mn, b_mn);
+        const uint64_t da0 = make_sdesc_sw128(sbase, a_mn ? 8192 : 16, 1024);
+        const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
+        const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+        const int b = i & 1, use = i >> 1;
+        if (use > 0) ok = mbar_wait_warp(bar(PB_AEMPTY + b), (use - 1) & 1, abort_flag, 923);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + b * kGemmBN;
+        for (int kb = 0; kb < n_kblk; ++kb, ++g) {
+          const int s = g % kPairStages;
+          ok = mbar_wait_warp(bar(PB_FULL + s), (g / kPairStages) & 1, abort_flag, 924);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t off = s * C::STAGE_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < kGemmBK / 16; ++kk)
+              mma_ss_pair(acc, desc_adv(da0, off + kk * a_step), desc_adv(db0, off + kk * b_step),
+                          idesc, (kb | kk) != 0 ? 1u : 0u);
+            tc_commit_pair_mc(bar(PB_EMPTY + s), 0x3);  // the stage is free in both CTAs
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (elect_one()) tc_commit_pair_mc(bar(PB_AFULL + b), 0x3);
+        __syncwarp();
+      }
+      // every pair MMA has completed before either CTA frees TMEM or exits
+      if (elect_one()) tc_commit_pair(bar(PB_DRAIN));
+      __syncwarp();
+      (void)mbar_wait(bar(PB_DRAIN), 0, nullptr, 925);
+    }
+  } else {
+    // ===================== epilogue (both CTAs) =========================
+    const int quarter = warp & 3;
+    const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * C::EPI_WARP_BYTES;
+    const uint32_t aempty0 = mapa_cta(bar(PB_AEMPTY), 0);
+    for (int i = 0;; ++i) {
+      const int t = ffn_next(p, pair, n_pairs, i);
+      if (t < 0) break;
+      int mb, nb;
+      const FfnProblem& q = p.prob[ffn_tile(p, t, mb, nb)];
+      const int b = i & 1, use = i >> 1;
+      if (!mbar_wait_warp(bar(PB_AFULL + b), use & 1, abort_flag, 926)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * kGemmBN;
+      const int row0 = mb * 256 + (int)crank * 128 + quarter * 32;
+      auto release_acc = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
+      };
+      ffn_epilogue_warp<MODE, ACT>(p, q, acc, row0, nb, lane, stg, release_acc);
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // no CTA frees TMEM or leaves while the pair still uses it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, C::TM_COLS);
+  }
+}
+
+// ===================================================================== few tokens
+// out[t, j] over a 128-row tile of weights (GLU: 64 gate rows and the 64 up
+// rows of the same outputs) and NT tokens: D[128, NT] = Wtile[128, K] X[NT, K]^T.
+// The block is bound by reading the weights once: a cluster of S CTAs takes
+// one tile, each a contiguous run of k-blocks through its own TMA ring, and
+// the S partial tiles are summed through distributed shared memory, always in
+// rank order, so results repeat bit for bit.
+//   warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 move the accumulator
+//   from TMEM to shared memory; all warps join the partials.
+constexpr int kTokThreads = 192;
+
+template <int NT>
+struct TokCfg {
+  static constexpr int W_BYTES = 128 * 64 * 2;
+  static constexpr int X_BYTES = NT * 64 * 2;
+  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
+  static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 3;
+  static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_ALLOC = OFF_BAR + 256 + 1024;
+  static constexpr int TM_COLS = NT < 32 ? 32 : NT;
+  static_assert(NT * 128 * 4 <= OFF_BAR, "the partial tile exceeds the ring");
+};
+
+struct TokParams {
+  int m;        // tokens
+  int n_out;    // outputs of a token: d_ff (GLU) or d_model
+  int n_kblk;   // k-blocks of 64
+  int act;      // GLU
+  int pdl;      // launched with programmatic stream serialization
+  __nv_bfloat16* out;             // [m, n_out]
+  float* z;                       // GLU: [m, 2 n_out] or null
+  const __nv_bfloat16* residual;  // [m, n_out] or null
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
+                                            int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+// Programmatic dependent launch: blocks until the kernels this one depends on
+// have completed and their writes are visible (returns at once without PDL).
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <int NT, bool GLU>
+__global__ void __launch_bounds__(kTokThreads)
+    ffn_token_kernel(const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_x, const TokParams p) {
+  using C = TokCfg<NT>;
+  constexpr int ROWS = GLU ? 64 : 128;  // outputs of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;  // same offset in every CTA of the cluster
+  uint8_t* sptr = smem_raw + (sbase - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sptr + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto full = [&](int s) { return smem_u32(bars + s); };
+  auto empty = [&](int s) { return smem_u32(bars + C::STAGES + s); };
+  const uint32_t done = smem_u32(bars + 2 * C::STAGES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = (int)gridDim.z;  // the cluster: CTAs of the same (x, y)
+  const int rank = (int)cluster_ctarank();
+  const int j0 = (int)blockIdx.x * ROWS, t0 = (int)blockIdx.y * NT;
+  const int kb0 = (int)((long long)p.n_kblk * rank / S);
+  const int kb1 = (int)((long long)p.n_kblk * (rank + 1) / S);
+  const int n_kb = kb1 - kb0;  // at least 1: S <= n_kblk
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (GLU) pdl_launch_dependents();
+
+  if (warp == 0) {
+    auto load_w = [&](int kb, int s) {
+      const uint32_t sw = sbase + s * C::STAGE_BYTES;
+      if constexpr (GLU) {
+        tma_load_2d(sw, &tm_w, full(s), (kb0 + kb) * 64, j0);
+        tma_load_2d(sw + 8192, &tm_w, full(s), (kb0 + kb) * 64, p.n_out + j0);
+      } else {
+        tma_load_2d(sw, &tm_w, full(s), (kb0 + kb) * 64, j0);
+      }
+    };
+    // the weights do not depend on the kernel before this one: the ring's
+    // first stages are requested before its result is waited for
+    const int early = min(n_kb, C::STAGES);
+    if (elect_one())
+      for (int kb = 0; kb < early; ++kb) {
+        mbar_arrive_expect_tx(full(kb), C::STAGE_BYTES);
+        load_w(kb, kb);
+      }
+    __syncwarp();
+    if (p.pdl) pdl_wait();
+    int issued = 0;
+    bool ok = true;
+    for (int kb = 0; kb < n_kb; ++kb) {
+      const int s = kb % C::STAGES, u = kb / C::STAGES;
+      if (u > 0) ok = mbar_wait_warp(empty(s), (u - 1) & 1, abort_flag, 931);
+      if (!ok) break;
+      if (elect_one()) {
+        if (u > 0) {
+          mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
+          load_w(kb, s);
+        }
+        tma_load_2d(sbase + s * C::STAGE_BYTES + C::W_BYTES, &tm_x, full(s), (kb0 + kb) * 64, t0);
+      }
+      __syncwarp();
+      issued = kb + 1;
+    }
+    if (!ok)  // copies in flight land before the shared memory goes away
+      for (int s = 0; s < C::STAGES; ++s) {
+        const int n_s = issued > s ? (issued - s - 1) / C::STAGES + 1 : 0;
+        if (n_s) (void)mbar_wait(full(s), (n_s - 1) & 1, nullptr, 932);
+      }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc_bf16(128, NT, 0, 0);
+    const uint64_t dw0 = make_sdesc_sw128(sbase, 16, 1024);
+    const uint64_t dx0 = make_sdesc_sw128(sbase + C::W_BYTES, 16, 1024);
+    bool ok = true;
+    for (int kb = 0; kb < n_kb; ++kb) {
+      const int s = kb % C::STAGES;
+      ok = mbar_wait_warp(full(s), (kb / C::STAGES) & 1, abort_flag, 933);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t off = s * C::STAGE_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ss(tmem, desc_adv(dw0, off + kk * 32), desc_adv(dx0, off + kk * 32), idesc,
+                 (kb | kk) != 0 ? 1u : 0u);
+        tc_commit(empty(s));
+      }
+      __syncwarp();
+    }
+    // completes when every MMA issued above has, whether or not all were
+    if (elect_one()) tc_commit(done);
+    __syncwarp();
+  }
+  // Every thread: the accumulator is complete (or the CTA gave up).
+  (void)mbar_wait(done, 0, nullptr, 934);
+  tc_fence_after();
+  __syncthreads();  // the ring's shared memory is free: it now holds the partial tile
+  float* part = reinterpret_cast<float*>(sptr);  // [NT][128]
+  if (warp >= 2) {
+    const int quarter = warp & 3;
+    const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+    for (int c = 0; c < NT; c += 16) {
+      if (t0 + c >= p.m) break;
+      uint32_t r[16];
+      tmem_ld16(acc + c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        part[(c + e) * 128 + quarter * 32 + lane] = __uint_as_float(r[e]);
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TM_COLS);
+  }
+  if (p.pdl) pdl_wait();  // the residual and the output belong to the stream's order too
+  if (!*abort_flag) {
+    // this CTA joins ROWS / S outputs of every token
+    const int rows = ROWS / S, r0 = rank * rows;
+    const int tokens = min(NT, p.m - t0);
+    const uint32_t part_addr = sbase;
+    for (int e = threadIdx.x; e < rows * tokens; e += kTokThreads) {
+      const int t = e / rows, j = r0 + e % rows;
+      const int col = j0 + j;
+      if (col >= p.n_out) continue;
+      float g = 0.0f, u = 0.0f;
+      for (int s = 0; s < S; ++s) {
+        const uint32_t at = mapa_cta(part_addr + (uint32_t)(t * 128 + j) * 4, s);
+        g += ld_cluster_f32(at);
+        if constexpr (GLU) u += ld_cluster_f32(at + 64 * 4);
+      }
+      const long long row = t0 + t;
+      if constexpr (GLU) {
+        if (p.z) {
+          p.z[row * 2 * p.n_out + col] = g;
+          p.z[row * 2 * p.n_out + p.n_out + col] = u;
+        }
+        g = ffn_act_rt(p.act, g) * u;
+      } else if (p.residual) {
+        g += __bfloat162float(p.residual[row * p.n_out + col]);
+      }
+      p.out[row * p.n_out + col] = __float2bfloat16_rn(g);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another reads its partial tile
+}
+
+}  // namespace tfb

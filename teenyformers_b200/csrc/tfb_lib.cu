@@ -27,6 +27,9 @@
 #include "norm_act.cuh"
 #include "comm_norm.cuh"
 #include "gemm_sm100.cuh"
+#include "gated_ffn.cuh"
+#include "block_norm.cuh"
+#include "dropout.cuh"
 
 using namespace tfb;
 
@@ -141,6 +144,21 @@ int ensure_device_setup() {
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_SWIGLU>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_QKV_ROPE>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_PUSH>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<16, true>, TokCfg<16>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<32, true>, TokCfg<32>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<64, true>, TokCfg<64>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<128, true>, TokCfg<128>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<16, false>, TokCfg<16>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<32, false>, TokCfg<32>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<64, false>, TokCfg<64>::SMEM_ALLOC);
+    set((const void*)ffn_token_kernel<128, false>, TokCfg<128>::SMEM_ALLOC);
     // CTA pairs that fit at once (SMs pair up within a GPC; one CTA per SM)
     g_pair_clusters[dev] = g_num_sms[dev] / 2;
     if (e == cudaSuccess) {
@@ -968,4 +986,403 @@ extern "C" int tf_b200_flash_attn2_bwd_bf16_noalloc(const void* q, const void* k
   // the deterministic two-kernel path: its scratch is only the per-row statistics
   return bwd_bf16_impl(q, k, v, o, d_o, lse, dq, dk, dv, ws, batch, n_heads_q, n_heads_kv,
                        n_ctx_q, n_ctx_k, head_dim, softmax_scale, causal, stream, false);
+}
+
+// ===================================================================== gated feed-forward
+namespace {
+
+void ffn_problem(FfnProblem& q, int M, int N, int K, int a_mn, int b_mn, void* out,
+                 const void* residual) {
+  q.M = M, q.N = N;
+  q.n_mblk = (M + 255) / 256;
+  q.n_nblk = (N + kGemmBN - 1) / kGemmBN;
+  q.n_kblk = (K + kGemmBK - 1) / kGemmBK;
+  q.n_tiles = q.n_mblk * q.n_nblk;
+  q.group_m = std::min(q.n_mblk, 8);
+  q.a_mn = a_mn, q.b_mn = b_mn;
+  q.out = static_cast<__nv_bfloat16*>(out);
+  q.residual = static_cast<const __nv_bfloat16*>(residual);
+}
+
+// An operand's k-blocks: rows [mn, k] with k innermost, or (mn_major) rows
+// [k, mn] read in 64 x 64 boxes.
+bool ffn_operand(CUtensorMap* map, const void* base, int mn, int k, int mn_major) {
+  return mn_major ? make_bf16_2d_map(map, base, mn, k, 64)
+                  : make_bf16_2d_map(map, base, k, mn, 128);
+}
+
+template <int MODE, int ACT>
+int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
+  // products come longest K first; those of the first one's K are the heavy tiles
+  long long heavy = 0, light = 0;
+  for (int i = 0; i < prm.n_prob; ++i)
+    (prm.prob[i].n_kblk == prm.prob[0].n_kblk ? heavy : light) += prm.prob[i].n_tiles;
+  if (!fits_i32(heavy + light)) return TF_ERR_TOO_LARGE;
+  const long long clusters = std::min<long long>(heavy + light, g_pair_clusters[current_device()]);
+  prm.heavy = (int)heavy, prm.light = (int)light, prm.bal_rounds = 0;
+  const long long r = heavy % clusters, q = clusters - r;
+  if (light > 0 && r > 0)
+    prm.bal_rounds = (int)std::min<long long>(
+        prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
+  ffn_pair_kernel<MODE, ACT>
+      <<<(unsigned)(2 * clusters), kGemmThreads, GemmPairCfg::SMEM_ALLOC, st>>>(maps, prm);
+  return launch_status();
+}
+
+template <int MODE>
+int ffn_pair_launch_act(int act, const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
+  switch (act) {
+    case TF_ACT_SILU: return ffn_pair_launch<MODE, FFN_ACT_SILU>(maps, prm, st);
+    case TF_ACT_GELU: return ffn_pair_launch<MODE, FFN_ACT_GELU>(maps, prm, st);
+    default: return ffn_pair_launch<MODE, FFN_ACT_GELU_TANH>(maps, prm, st);
+  }
+}
+
+// One product of the few-token kernel: `rows` weight rows a tile.
+template <int NT, bool GLU>
+int ffn_token_launch(const void* w, int w_rows, const void* x, int k, TokParams& prm,
+                     cudaStream_t st) {
+  constexpr int ROWS = GLU ? 64 : 128;
+  CUtensorMap tw, tx;
+  if (!make_bf16_2d_map(&tw, w, k, w_rows, ROWS) || !make_bf16_2d_map(&tx, x, k, prm.m, NT))
+    return TF_ERR_CUDA;
+  prm.n_kblk = (k + 63) / 64;
+  const long long gx = (prm.n_out + ROWS - 1) / ROWS, gy = (prm.m + NT - 1) / NT;
+  if (gy > 65535) return TF_ERR_TOO_LARGE;
+  int S = 1;
+  while (S < 8 && gx * gy * S < 148 && prm.n_kblk >= 4 * S) S *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)gx, (unsigned)gy, (unsigned)S);
+  cfg.blockDim = dim3(kTokThreads, 1, 1);
+  cfg.dynamicSmemBytes = TokCfg<NT>::SMEM_ALLOC;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)S;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = prm.pdl ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, ffn_token_kernel<NT, GLU>, tw, tx, prm) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return TF_ERR_CUDA;
+  }
+  return launch_status();
+}
+
+template <bool GLU>
+int ffn_token_launch_nt(const void* w, int w_rows, const void* x, int k, TokParams& prm,
+                        cudaStream_t st) {
+  if (prm.m <= 16) return ffn_token_launch<16, GLU>(w, w_rows, x, k, prm, st);
+  if (prm.m <= 32) return ffn_token_launch<32, GLU>(w, w_rows, x, k, prm, st);
+  if (prm.m <= 64) return ffn_token_launch<64, GLU>(w, w_rows, x, k, prm, st);
+  return ffn_token_launch<128, GLU>(w, w_rows, x, k, prm, st);
+}
+
+// Tokens up to which a call takes the few-token kernel.
+constexpr int kFfnTokenMax = 128;
+
+int ffn_check(int m, int d_model, int d_ff, int act) {
+  if (m < 0 || d_model < 0 || d_ff < 0) return TF_ERR_INVALID_ARG;
+  if (act < TF_ACT_SILU || act > TF_ACT_GELU_TANH) return TF_ERR_INVALID_ARG;
+  if (d_model % 8 != 0 || d_ff % 8 != 0) return TF_ERR_UNSUPPORTED;
+  if (!fits_i32(2LL * d_ff)) return TF_ERR_TOO_LARGE;
+  return TF_OK;
+}
+
+}  // namespace
+
+extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, const void* w_down,
+                                          const void* residual, void* a, float* z, void* y, int m,
+                                          int d_model, int d_ff, int act, void* stream) {
+  if (int st = ffn_check(m, d_model, d_ff, act)) return st;
+  if (m == 0 || d_model == 0) return TF_OK;
+  if (d_ff == 0) return TF_ERR_UNSUPPORTED;
+  if (!x || !w_gate_up || !w_down || !a || !y) return TF_ERR_INVALID_ARG;
+  if (!is_aligned(x, 16) || !is_aligned(w_gate_up, 16) || !is_aligned(w_down, 16) ||
+      !is_aligned(residual, 16) || !is_aligned(a, 16) || !is_aligned(z, 16) || !is_aligned(y, 16))
+    return TF_ERR_MISALIGNED;
+  if (int st = ensure_device_setup()) return st;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (m <= kFfnTokenMax) {
+    TokParams g{};
+    g.m = m, g.n_out = d_ff, g.act = act;
+    g.out = static_cast<__nv_bfloat16*>(a);
+    g.z = z;
+    if (int e = ffn_token_launch_nt<true>(w_gate_up, 2 * d_ff, x, d_model, g, st)) return e;
+    TokParams d{};
+    d.m = m, d.n_out = d_model, d.pdl = 1;
+    d.out = static_cast<__nv_bfloat16*>(y);
+    d.residual = static_cast<const __nv_bfloat16*>(residual);
+    return ffn_token_launch_nt<false>(w_down, d_model, a, d_ff, d, st);
+  }
+  FfnMaps maps;
+  FfnPairParams prm{};
+  prm.n_prob = 1;
+  prm.F = d_ff;
+  prm.a = static_cast<__nv_bfloat16*>(a);
+  prm.z = z;
+  ffn_problem(prm.prob[0], m, 2 * d_ff, d_model, 0, 0, nullptr, nullptr);
+  prm.prob[0].n_nblk = (d_ff + 127) / 128;  // 128 gate and 128 up rows a tile
+  prm.prob[0].n_tiles = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
+  if (!ffn_operand(&maps.a[0], x, m, d_model, 0) ||
+      !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0))
+    return TF_ERR_CUDA;
+  if (int e = ffn_pair_launch_act<FFN_GLU>(act, maps, prm, st)) return e;
+  FfnPairParams down{};
+  down.n_prob = 1;
+  ffn_problem(down.prob[0], m, d_model, d_ff, 0, 0, y, residual);
+  if (!ffn_operand(&maps.a[0], a, m, d_ff, 0) || !ffn_operand(&maps.b[0], w_down, d_model, d_ff, 0))
+    return TF_ERR_CUDA;
+  return ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, down, st);
+}
+
+extern "C" size_t tf_b200_gated_ffn_bwd_workspace_size(int m, int d_ff) {
+  if (m <= 0 || d_ff <= 0 || d_ff % 8 != 0) return 0;
+  return (size_t)m * d_ff * 3 * 2;  // dz [m, 2 d_ff] and a [m, d_ff]
+}
+
+extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, const void* w_down,
+                                          const float* z, const void* dy, void* dx,
+                                          void* dw_gate_up, void* dw_down, void* workspace, int m,
+                                          int d_model, int d_ff, int act, void* stream) {
+  if (int st = ffn_check(m, d_model, d_ff, act)) return st;
+  if (d_model == 0) return TF_OK;
+  if (d_ff == 0) return TF_ERR_UNSUPPORTED;
+  if (!is_aligned(x, 16) || !is_aligned(w_gate_up, 16) || !is_aligned(w_down, 16) ||
+      !is_aligned(z, 16) || !is_aligned(dy, 16) || !is_aligned(dx, 16) ||
+      !is_aligned(dw_gate_up, 16) || !is_aligned(dw_down, 16) || !is_aligned(workspace, 16))
+    return TF_ERR_MISALIGNED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (m == 0) {  // sums over no tokens
+    const size_t w = (size_t)d_ff * d_model * 2;
+    if (dw_gate_up && cudaMemsetAsync(dw_gate_up, 0, 2 * w, st) != cudaSuccess) return TF_ERR_CUDA;
+    if (dw_down && cudaMemsetAsync(dw_down, 0, w, st) != cudaSuccess) return TF_ERR_CUDA;
+    return TF_OK;
+  }
+  if (!x || !w_gate_up || !w_down || !z || !dy || !workspace) return TF_ERR_INVALID_ARG;
+  if (!dx && !dw_gate_up && !dw_down) return TF_OK;
+  if (int e = ensure_device_setup()) return e;
+  __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(workspace);
+  __nv_bfloat16* a = dz + (size_t)m * 2 * d_ff;
+  FfnMaps maps;
+  FfnPairParams prm{};
+  prm.n_prob = 1;
+  prm.F = d_ff;
+  prm.a = a;
+  prm.z = const_cast<float*>(z);
+  prm.dz = dz;
+  ffn_problem(prm.prob[0], m, d_ff, d_model, 0, 1, nullptr, nullptr);
+  if (!ffn_operand(&maps.a[0], dy, m, d_model, 0) ||
+      !ffn_operand(&maps.b[0], w_down, d_ff, d_model, 1))
+    return TF_ERR_CUDA;
+  if (int e = ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st)) return e;
+
+  // the three products that follow in one launch, those with the longer K first
+  FfnPairParams g{};
+  bool ok = true;
+  auto add_dx = [&] {
+    if (!dx) return;
+    const int i = g.n_prob++;
+    ffn_problem(g.prob[i], m, d_model, 2 * d_ff, 0, 1, dx, nullptr);
+    ok = ok && ffn_operand(&maps.a[i], dz, m, 2 * d_ff, 0) &&
+         ffn_operand(&maps.b[i], w_gate_up, d_model, 2 * d_ff, 1);
+  };
+  if (2 * d_ff >= m) add_dx();
+  if (dw_gate_up) {
+    const int i = g.n_prob++;
+    ffn_problem(g.prob[i], 2 * d_ff, d_model, m, 1, 1, dw_gate_up, nullptr);
+    ok = ok && ffn_operand(&maps.a[i], dz, 2 * d_ff, m, 1) &&
+         ffn_operand(&maps.b[i], x, d_model, m, 1);
+  }
+  if (dw_down) {
+    const int i = g.n_prob++;
+    ffn_problem(g.prob[i], d_model, d_ff, m, 1, 1, dw_down, nullptr);
+    ok = ok && ffn_operand(&maps.a[i], dy, d_model, m, 1) && ffn_operand(&maps.b[i], a, d_ff, m, 1);
+  }
+  if (2 * d_ff < m) add_dx();
+  if (!ok) return TF_ERR_CUDA;
+  return ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, g, st);
+}
+
+// ===================================================================== block norm, dropout
+namespace {
+
+// p in [0, 1] (NaN refused); the generator's words are read on the device.
+int dropout_params(DropoutParams& d, const void* rng, float p, unsigned site, size_t n) {
+  if (!(p >= 0.0f && p <= 1.0f)) return TF_ERR_INVALID_ARG;
+  d = DropoutParams{};
+  if (p == 0.0f) return TF_OK;
+  if (!rng) return TF_ERR_INVALID_ARG;
+  if (!is_aligned(rng, 8)) return TF_ERR_MISALIGNED;
+  if (n > (size_t)1 << 35) return TF_ERR_TOO_LARGE;  // a group's index is 32 bits of the counter
+  d.rng = static_cast<const unsigned long long*>(rng);
+  d.site = site;
+  d.threshold = (unsigned)std::floor((1.0 - (double)p) * 65536.0 + 0.5);
+  d.scale = d.threshold ? (float)(65536.0 / d.threshold) : 0.0f;
+  return TF_OK;
+}
+
+int block_norm_check(int rows, int cols, bool gate, int gate_rows, float eps, float residual_scale,
+                     float branch_scale) {
+  if (rows < 0 || cols < 0) return TF_ERR_INVALID_ARG;
+  if (cols % 8 != 0 || cols > kBnMaxCols) return TF_ERR_UNSUPPORTED;
+  if (gate && (gate_rows < 1 || rows % gate_rows != 0)) return TF_ERR_INVALID_ARG;
+  if (!(eps >= 0.0f) || !std::isfinite(eps) || !std::isfinite(residual_scale) ||
+      !std::isfinite(branch_scale))
+    return TF_ERR_INVALID_ARG;
+  return TF_OK;
+}
+
+// One launch of a kernel<WPR, VPT> by the shape's team size.
+#define TFB_BN_DISPATCH(T, LAUNCH)                                        \
+  do {                                                                    \
+    if ((T).wpr == 1 && (T).vpt == 1) LAUNCH(1, 1);                       \
+    else if ((T).wpr == 1) LAUNCH(1, 2);                                  \
+    else if ((T).wpr == 2) LAUNCH(2, 2);                                  \
+    else if ((T).wpr == 4) LAUNCH(4, 2);                                  \
+    else if ((T).vpt == 2) LAUNCH(8, 2);                                  \
+    else LAUNCH(8, 4);                                                    \
+  } while (0)
+
+}  // namespace
+
+extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const void* w_post,
+                                           const void* gate, const void* w_pre, void* y, void* h,
+                                           const void* rng, int rows, int cols, int gate_rows,
+                                           float eps, float residual_scale, float branch_scale,
+                                           float drop_p, unsigned site, void* stream) {
+  if (int e = block_norm_check(rows, cols, gate != nullptr, gate_rows, eps, residual_scale,
+                               branch_scale))
+    return e;
+  BlockNormParams p{};
+  if (int e = dropout_params(p.drop, rng, drop_p, site, (size_t)rows * (size_t)cols)) return e;
+  if (rows == 0 || cols == 0) return TF_OK;
+  if (!x || (f && !y) || (w_pre && !h)) return TF_ERR_INVALID_ARG;
+  if (!f && (!w_pre || w_post || gate || p.drop.rng)) return TF_ERR_INVALID_ARG;
+  for (const void* t : {x, f, w_post, gate, w_pre, (const void*)y, (const void*)h})
+    if (!is_aligned(t, 16)) return TF_ERR_MISALIGNED;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.f = static_cast<const __nv_bfloat16*>(f);
+  p.w_post = static_cast<const __nv_bfloat16*>(w_post);
+  p.gate = static_cast<const __nv_bfloat16*>(gate);
+  p.w_pre = static_cast<const __nv_bfloat16*>(w_pre);
+  p.y = static_cast<__nv_bfloat16*>(y);
+  p.h = static_cast<__nv_bfloat16*>(h);
+  p.rows = rows, p.cols = cols, p.rows_per_gate = gate ? rows / gate_rows : 1;
+  p.eps = eps, p.residual_scale = residual_scale, p.branch_scale = branch_scale;
+  const BlockNormTeams t = block_norm_teams(rows, cols);
+  const unsigned grid = (unsigned)(((long long)rows * t.wpr + kBnWarps - 1) / kBnWarps);
+#define TFB_BN_FWD(W, V) \
+  block_norm_fwd_kernel<W, V><<<grid, kBnThreads, 0, static_cast<cudaStream_t>(stream)>>>(p)
+  TFB_BN_DISPATCH(t, TFB_BN_FWD);
+#undef TFB_BN_FWD
+  return launch_status();
+}
+
+extern "C" size_t tf_b200_block_norm_bwd_workspace_size(int rows, int cols) {
+  if (rows <= 0 || cols <= 0 || cols % 8 != 0 || cols > kBnMaxCols) return 0;
+  // two weights' and two gate segments' fp32 sums a team
+  return (size_t)block_norm_teams(rows, cols).n_teams * cols * 4 * 4;
+}
+
+extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const void* dy,
+                                           const void* dh, const void* w_post, const void* gate,
+                                           const void* w_pre, void* dx, void* df, void* dw_post,
+                                           void* dgate, void* dw_pre, const void* rng,
+                                           void* workspace, int rows, int cols, int gate_rows,
+                                           float eps, float residual_scale, float branch_scale,
+                                           float drop_p, unsigned site, void* stream) {
+  if (int e = block_norm_check(rows, cols, gate != nullptr, gate_rows, eps, residual_scale,
+                               branch_scale))
+    return e;
+  BlockNormBwdParams p{};
+  if (int e = dropout_params(p.drop, rng, drop_p, site, (size_t)rows * (size_t)cols)) return e;
+  if (cols == 0) return TF_OK;
+  if ((w_post && !dw_post) || (gate && !dgate) || (w_pre && !dw_pre)) return TF_ERR_INVALID_ARG;
+  for (const void* t : {f, y, dy, dh, w_post, gate, w_pre, (const void*)dx, (const void*)df,
+                        (const void*)dw_post, (const void*)dgate, (const void*)dw_pre,
+                        (const void*)workspace})
+    if (!is_aligned(t, 16)) return TF_ERR_MISALIGNED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // sums over no rows
+    const size_t b = (size_t)cols * 2;
+    if (w_post && cudaMemsetAsync(dw_post, 0, b, st) != cudaSuccess) return TF_ERR_CUDA;
+    if (w_pre && cudaMemsetAsync(dw_pre, 0, b, st) != cudaSuccess) return TF_ERR_CUDA;
+    if (gate && cudaMemsetAsync(dgate, 0, b * gate_rows, st) != cudaSuccess) return TF_ERR_CUDA;
+    return TF_OK;
+  }
+  if (!dx || !workspace || (!dy && !dh)) return TF_ERR_INVALID_ARG;
+  if ((w_pre != nullptr) != (dh != nullptr) || (w_pre && !y)) return TF_ERR_INVALID_ARG;
+  if (!df && (!w_pre || f || w_post || gate || p.drop.rng)) return TF_ERR_INVALID_ARG;
+  if ((w_post || gate) && !f) return TF_ERR_INVALID_ARG;
+  p.f = static_cast<const __nv_bfloat16*>(f);
+  p.w_post = static_cast<const __nv_bfloat16*>(w_post);
+  p.gate = static_cast<const __nv_bfloat16*>(gate);
+  p.y = static_cast<const __nv_bfloat16*>(y);
+  p.w_pre = static_cast<const __nv_bfloat16*>(w_pre);
+  p.dy = static_cast<const __nv_bfloat16*>(dy);
+  p.dh = static_cast<const __nv_bfloat16*>(dh);
+  p.dx = static_cast<__nv_bfloat16*>(dx);
+  p.df = static_cast<__nv_bfloat16*>(df);
+  p.dgate = static_cast<__nv_bfloat16*>(dgate);
+  p.rows = rows, p.cols = cols, p.rows_per_gate = gate ? rows / gate_rows : 1;
+  p.eps = eps, p.residual_scale = residual_scale, p.branch_scale = branch_scale;
+  const BlockNormTeams t = block_norm_teams(rows, cols);
+  p.rows_per_team = t.rows_per_team, p.n_teams = t.n_teams;
+  p.part_post = static_cast<float*>(workspace);
+  p.part_pre = p.part_post + (size_t)t.n_teams * cols;
+  p.part_gate = p.part_pre + (size_t)t.n_teams * cols;
+  const unsigned grid = (unsigned)((t.n_teams * t.wpr + kBnWarps - 1) / kBnWarps);
+#define TFB_BN_BWD(W, V) block_norm_bwd_kernel<W, V><<<grid, kBnThreads, 0, st>>>(p)
+  TFB_BN_DISPATCH(t, TFB_BN_BWD);
+#undef TFB_BN_BWD
+  if (int e = launch_status()) return e;
+  if (!w_post && !w_pre && !gate) return TF_OK;
+  BlockNormSumParams s{};
+  s.part_post = p.part_post, s.part_pre = p.part_pre, s.part_gate = p.part_gate;
+  s.dw_post = w_post ? static_cast<__nv_bfloat16*>(dw_post) : nullptr;
+  s.dw_pre = w_pre ? static_cast<__nv_bfloat16*>(dw_pre) : nullptr;
+  s.dgate = gate && p.rows_per_gate > 1 ? p.dgate : nullptr;  // one row a gate: written already
+  s.cols = cols, s.n_teams = t.n_teams, s.rows_per_team = t.rows_per_team;
+  s.rows_per_gate = p.rows_per_gate, s.gate_rows = gate ? gate_rows : 0;
+  const int outs = 2 + (s.dgate ? gate_rows : 0);
+  const dim3 sgrid((unsigned)((cols + 31) / 32), (unsigned)std::min(outs, 1024));
+  block_norm_sum_kernel<<<sgrid, 256, 0, st>>>(s);
+  return launch_status();
+}
+
+namespace {
+
+template <typename T>
+int dropout_launch(const T* x, const T* residual, T* y, const void* rng, size_t n, float p,
+                   unsigned site, void* stream) {
+  DropoutParams d;
+  if (int e = dropout_params(d, rng, p, site, n)) return e;
+  if (n == 0) return TF_OK;
+  if (!x || !y) return TF_ERR_INVALID_ARG;
+  if (!is_aligned(x, 16) || !is_aligned(residual, 16) || !is_aligned(y, 16))
+    return TF_ERR_MISALIGNED;
+  if (n > (size_t)1 << 40) return TF_ERR_TOO_LARGE;
+  const size_t blocks = (n / 8 + 255) / 256;
+  const unsigned grid = (unsigned)std::max<size_t>(1, std::min<size_t>(blocks, 148 * 8));
+  dropout_kernel<T><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(x, residual, y,
+                                                                         (long long)n, d);
+  return launch_status();
+}
+
+}  // namespace
+
+extern "C" int tf_b200_dropout_bf16(const void* x, const void* residual, void* y, const void* rng,
+                                    size_t n, float p, unsigned site, void* stream) {
+  return dropout_launch(static_cast<const __nv_bfloat16*>(x),
+                        static_cast<const __nv_bfloat16*>(residual),
+                        static_cast<__nv_bfloat16*>(y), rng, n, p, site, stream);
+}
+
+extern "C" int tf_b200_dropout_f32(const float* x, const float* residual, float* y, const void* rng,
+                                   size_t n, float p, unsigned site, void* stream) {
+  return dropout_launch(x, residual, y, rng, n, p, site, stream);
 }

@@ -12,6 +12,9 @@ device-memory / stream plumbing only):
   RopeOp              src/kernels/rope.rs:246-281
   TransposeHeadsOp    src/kernels/transpose_heads.rs:168-203
   MergeHeadsOp        src/kernels/transpose_heads.rs:276-312
+  GatedFfnOp          src/layers/ffn.rs:47-56 with src/kernels/swiglu.rs:56-261
+  BlockNormOp         src/kernels/fused_add_rmsnorm.rs:53-340, gated and scaled
+  DropoutOp           (no counterpart)
 
 Errors: the reference asserts on bad shapes (src/layers/attention.rs:68);
 here a bad call raises ValueError (shape) or TfError (status from the C ABI).
@@ -24,15 +27,18 @@ import math
 import torch
 
 from . import _capi
-from ._capi import TF_ROPE_INTERLEAVED, TF_ROPE_ROTATE_HALF, TfError, call
+from ._capi import (TF_ACT_GELU, TF_ACT_GELU_TANH, TF_ACT_SILU, TF_ROPE_INTERLEAVED,
+                    TF_ROPE_ROTATE_HALF, TfError, call)
 
 __all__ = [
     "FlashAttn2Op", "CausalFlashAttn2Op", "RopeOp", "TransposeHeadsOp", "MergeHeadsOp",
     "flash_attn2_fwd", "flash_attn2_bwd", "rope", "rope_transpose", "transpose_heads",
     "merge_heads", "bwd_workspace", "rmsnorm", "swiglu", "flash_attn2_decode",
     "decode_workspace", "linear", "linear_swiglu", "swiglu_weight_blocks", "rope_table",
-    "linear_qkv_rope", "linear_push", "TF_ROPE_INTERLEAVED",
-    "TF_ROPE_ROTATE_HALF", "TfError",
+    "linear_qkv_rope", "linear_push", "gated_ffn", "gated_ffn_bwd", "block_norm",
+    "block_norm_bwd", "dropout", "dropout_rng", "GatedFfnOp", "BlockNormOp", "DropoutOp",
+    "TF_ROPE_INTERLEAVED", "TF_ROPE_ROTATE_HALF", "TF_ACT_SILU", "TF_ACT_GELU",
+    "TF_ACT_GELU_TANH", "TfError",
 ]
 
 
@@ -342,6 +348,206 @@ def linear_push(x: torch.Tensor, weight: torch.Tensor, peer_recv_ptrs, rank: int
          world, _stream(x))
 
 
+# ----------------------------------------------------------------- feed-forward side of a block
+def _launch(device: torch.device, name: str, *args) -> None:
+    """call(name, *args, stream) on `device`'s current stream, with that device
+    current (the library launches on the current device)."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream)
+
+
+def _addr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _dense(device: torch.device, dtype: torch.dtype, what: str, *ts) -> None:
+    for t in ts:
+        if t is not None:
+            _need(t.dtype == dtype and t.device == device and t.is_contiguous(),
+                  f"{what} tensors must be contiguous {dtype} tensors on {device}")
+
+
+def _buffer(t: torch.Tensor | None, shape, dtype: torch.dtype, device: torch.device,
+            name: str) -> torch.Tensor:
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _need(tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.device == device
+          and t.is_contiguous(), f"{name} must be a contiguous {dtype} {tuple(shape)} tensor")
+    return t
+
+
+def _ffn_shapes(x, w_gate_up, w_down):
+    _need(x.is_cuda and x.dim() >= 1 and w_gate_up.dim() == 2 and w_down.dim() == 2,
+          "x must be a [..., d] CUDA tensor, w_gate_up and w_down matrices")
+    d_ff, d = w_down.shape[1], w_down.shape[0]
+    _need(x.shape[-1] == d and tuple(w_gate_up.shape) == (2 * d_ff, d),
+          "expected x [..., d], w_gate_up [2 * d_ff, d], w_down [d, d_ff]")
+    return x.numel() // max(d, 1), d, d_ff
+
+
+def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
+              act: int = TF_ACT_SILU, residual: torch.Tensor | None = None, save: bool = False,
+              out: torch.Tensor | None = None, act_out: torch.Tensor | None = None,
+              z_out: torch.Tensor | None = None):
+    """(act(x Wg^T) * (x Wu^T)) Wd^T (+ residual), the gated feed-forward of a block
+    (ffn.rs:47-56 around swiglu.rs:56-95), for any number of tokens.
+
+    x [..., d] bf16; w_gate_up [2 * d_ff, d] = [Wg; Wu] (the layer's layout); w_down
+    [d, d_ff]; act TF_ACT_SILU / GELU / GELU_TANH.  ``save`` also returns z
+    [..., 2 * d_ff] fp32 = x [Wg; Wu]^T for gated_ffn_bwd.  ``out``, ``act_out``
+    ([..., d_ff] scratch) and ``z_out`` are buffers to use instead of new ones."""
+    m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
+    dev, lead = x.device, tuple(x.shape[:-1])
+    _dense(dev, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, residual)
+    _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
+    y = _buffer(out, lead + (d,), torch.bfloat16, dev, "out")
+    a = _buffer(act_out, lead + (d_ff,), torch.bfloat16, dev, "act_out")
+    z = _buffer(z_out, lead + (2 * d_ff,), torch.float32, dev, "z_out") if save else None
+    _launch(dev, "tf_b200_gated_ffn_fwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
+            w_down.data_ptr(), _addr(residual), a.data_ptr(), _addr(z), y.data_ptr(), m, d, d_ff,
+            int(act))
+    return (y, z) if save else y
+
+
+def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, z: torch.Tensor,
+                  dy: torch.Tensor, act: int = TF_ACT_SILU, grads=None, need=(True, True, True),
+                  workspace: torch.Tensor | None = None):
+    """(dx, dw_gate_up, dw_down) of gated_ffn from z (gated_ffn(..., save=True)) and dy;
+    a False in ``need`` skips that gradient (None in its place).  The residual's
+    gradient is dy itself.  ``grads``: three tensors to write instead of new ones."""
+    m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
+    dev = x.device
+    _dense(dev, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, dy)
+    _dense(dev, torch.float32, "z", z)
+    _need(dy.shape == x.shape, "dy must have x's shape")
+    _need(tuple(z.shape) == tuple(x.shape[:-1]) + (2 * d_ff,), "z must be [..., 2 * d_ff]")
+    given = (None, None, None) if grads is None else grads
+    g = [_buffer(t, like.shape, torch.bfloat16, dev, "a gradient") if on else None
+         for t, like, on in zip(given, (x, w_gate_up, w_down), need)]
+    n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d_ff)
+    ws = torch.empty(int(n), dtype=torch.uint8, device=dev) if workspace is None else workspace
+    _need(ws.device == dev and ws.is_contiguous() and ws.numel() * ws.element_size() >= n,
+          "workspace too small")
+    _launch(dev, "tf_b200_gated_ffn_bwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
+            w_down.data_ptr(), z.data_ptr(), dy.data_ptr(), _addr(g[0]), _addr(g[1]), _addr(g[2]),
+            ws.data_ptr(), m, d, d_ff, int(act))
+    return tuple(g)
+
+
+def dropout_rng(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
+    """The generator words of the dropouts: an int64 [2] tensor (seed, offset).  Give
+    every step another offset (in place, if a graph replays the step) and every
+    dropout of a step another ``site``; a backward pass needs its forward's."""
+    wrap = lambda v: (int(v) + (1 << 63)) % (1 << 64) - (1 << 63)
+    return torch.tensor([wrap(seed), wrap(offset)], dtype=torch.int64, device=device)
+
+
+def _rng_addr(p: float, rng: torch.Tensor | None, site: int, device: torch.device):
+    _need(0 <= site < 1 << 32, "site must be a 32-bit number")
+    if not p:
+        return None
+    _need(rng is not None and rng.dtype == torch.int64 and rng.numel() == 2
+          and rng.is_contiguous() and rng.device == device,
+          f"p > 0 needs rng, an int64 [2] tensor (seed, offset) on {device}")
+    return rng.data_ptr()
+
+
+def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
+            residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """dropout(x) (+ residual), bf16 or fp32, the mask drawn from (rng, site) by a
+    counter-based generator and never stored.  The backward pass is
+    ``dropout(dy, p, rng, site)``.  ``out`` may be x or residual."""
+    fn = {torch.float32: "tf_b200_dropout_f32", torch.bfloat16: "tf_b200_dropout_bf16"}.get(x.dtype)
+    _need(fn is not None, f"unsupported dtype {x.dtype}")
+    _need(x.is_cuda, "x must be a CUDA tensor")
+    dev = x.device
+    _dense(dev, x.dtype, "dropout", x, residual)
+    _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
+    y = _buffer(out, x.shape, x.dtype, dev, "out")
+    _launch(dev, fn, x.data_ptr(), _addr(residual), y.data_ptr(), _rng_addr(p, rng, site, dev),
+            x.numel(), float(p), int(site))
+    return y
+
+
+def _norm_shapes(x, w_post, gate, w_pre):
+    _need(x.is_cuda and x.dim() >= 1, "block_norm tensors must be [..., cols] CUDA tensors")
+    cols = x.shape[-1]
+    rows = x.numel() // max(cols, 1)
+    for w in (w_post, w_pre):
+        _need(w is None or w.numel() == cols, "a norm's weight must have the last dim's size")
+    gate_rows = 1
+    if gate is not None:
+        _need(gate.shape[-1] == cols, "gate must be [gate_rows, cols] or [cols]")
+        gate_rows = gate.numel() // max(cols, 1)
+        _need(gate_rows >= 1 and rows % gate_rows == 0, "the gate's rows must divide x's")
+    return rows, cols, gate_rows
+
+
+def block_norm(x: torch.Tensor, f: torch.Tensor | None, w_post: torch.Tensor | None = None,
+               gate: torch.Tensor | None = None, w_pre: torch.Tensor | None = None,
+               eps: float = 1e-5, residual_scale: float = 1.0, branch_scale: float = 1.0,
+               p: float = 0.0, rng: torch.Tensor | None = None, site: int = 0,
+               out: torch.Tensor | None = None, norm_out: torch.Tensor | None = None):
+    """The norms on either side of a block's residual sum, in one pass:
+
+        y = residual_scale * x + branch_scale * dropout(gate * RMSNorm(f) * w_post)
+        h = RMSNorm(y) * w_pre
+
+    x (residual stream) and f (the block's output) [..., cols] bf16; w_post, w_pre
+    [cols] or None (no norm there); gate [gate_rows, cols] or None, one row for
+    every rows / gate_rows consecutive rows.  f None: only the norm before a block
+    (y is x).  Returns (y, h), h None without w_pre.  ``out`` may be x."""
+    rows, cols, gate_rows = _norm_shapes(x, w_post, gate, w_pre)
+    dev = x.device
+    _dense(dev, torch.bfloat16, "block_norm", x, f, w_post, gate, w_pre)
+    _need(f is None or f.shape == x.shape, "f must have x's shape")
+    y = x if f is None else _buffer(out, x.shape, x.dtype, dev, "out")
+    h = None if w_pre is None else _buffer(norm_out, x.shape, x.dtype, dev, "norm_out")
+    _launch(dev, "tf_b200_block_norm_fwd_bf16", x.data_ptr(), _addr(f), _addr(w_post), _addr(gate),
+            _addr(w_pre), y.data_ptr(), _addr(h), _rng_addr(p, rng, site, dev), rows, cols, gate_rows,
+            float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
+    return y, h
+
+
+def block_norm_bwd(f: torch.Tensor | None, y: torch.Tensor | None, dy: torch.Tensor | None,
+                   dh: torch.Tensor | None, w_post: torch.Tensor | None = None,
+                   gate: torch.Tensor | None = None, w_pre: torch.Tensor | None = None,
+                   eps: float = 1e-5, residual_scale: float = 1.0, branch_scale: float = 1.0,
+                   p: float = 0.0, rng: torch.Tensor | None = None, site: int = 0,
+                   branch: bool = True, workspace: torch.Tensor | None = None):
+    """(dx, df, dw_post, dgate, dw_pre) of block_norm from dy (None: zero) and dh (with
+    w_pre), the forward's f and y, and its rng, p and site; None in the place of what
+    was not there.  ``branch=False``: the forward had f None."""
+    like = dy if dy is not None else dh
+    _need(like is not None, "dy or dh is needed")
+    rows, cols, gate_rows = _norm_shapes(like, w_post, gate, w_pre)
+    dev = like.device
+    _dense(dev, torch.bfloat16, "block_norm", f, y, dy, dh, w_post, gate, w_pre)
+    for t in (f, y, dy, dh):
+        _need(t is None or t.shape == like.shape, "f, y, dy and dh must have one shape")
+    _need((w_pre is None) == (dh is None), "dh belongs to w_pre")
+    _need(w_pre is None or y is not None, "w_pre needs the forward's y")
+    _need(branch or (f is None and w_post is None and gate is None and not p),
+          "branch=False takes no f, w_post, gate or dropout")
+    _need(f is not None or (w_post is None and gate is None), "w_post and gate need f")
+    new = lambda t: None if t is None else torch.empty_like(t)
+    dx, df = torch.empty_like(like), torch.empty_like(like) if branch else None
+    dw_post, dgate, dw_pre = new(w_post), new(gate), new(w_pre)
+    n = _capi.raw("tf_b200_block_norm_bwd_workspace_size", rows, cols)
+    ws = torch.empty(int(n), dtype=torch.uint8, device=dev) if workspace is None else workspace
+    _need(ws.device == dev and ws.is_contiguous() and ws.numel() * ws.element_size() >= n,
+          "workspace too small")
+    _launch(dev, "tf_b200_block_norm_bwd_bf16", _addr(f), _addr(y), _addr(dy), _addr(dh),
+            _addr(w_post), _addr(gate), _addr(w_pre), dx.data_ptr(), _addr(df), _addr(dw_post),
+            _addr(dgate), _addr(dw_pre), _rng_addr(p, rng, site, dev), ws.data_ptr(), rows, cols,
+            gate_rows, float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
+    return dx, df, dw_post, dgate, dw_pre
+
+
 # ----------------------------------------------------------------- op classes
 class FlashAttn2Op:
     """Bidirectional flash attention (reference FlashAttn2Op).
@@ -479,3 +685,101 @@ class MergeHeadsOp:
 
     def backward(self, grad_output):
         return transpose_heads(grad_output, self.n_heads)
+
+
+class GatedFfnOp:
+    """The gated feed-forward of a block (the reference builds it from Linear ->
+    SwigluOp -> Linear, src/layers/ffn.rs:47-56): primary input x [..., d]; others
+    w_gate_up [2 * d_ff, d], w_down [d, d_ff].  Param cache z [..., 2 * d_ff] fp32
+    (written when ``forward`` is asked to save it for the backward)."""
+
+    name = "gated_ffn"
+
+    def __init__(self, d_ff: int, act: int = TF_ACT_SILU):
+        self.d_ff = int(d_ff)
+        self.act = int(act)
+
+    def infer_output_shape(self, input_shapes):
+        return tuple(input_shapes[0])
+
+    def n_activation_inputs(self) -> int:
+        return 3
+
+    def param_shapes(self, input_shapes, output_shape=None):
+        return [list(input_shapes[0][:-1]) + [2 * self.d_ff]]
+
+    def has_backward(self) -> bool:
+        return True
+
+    def forward(self, x, w_gate_up, w_down, residual=None, save=False):
+        _need(w_down.shape[-1] == self.d_ff, "d_ff mismatch")
+        return gated_ffn(x, w_gate_up, w_down, self.act, residual=residual, save=save)
+
+    def backward(self, x, w_gate_up, w_down, z, grad_output, workspace=None):
+        return gated_ffn_bwd(x, w_gate_up, w_down, z, grad_output, self.act, workspace=workspace)
+
+
+class BlockNormOp:
+    """The norms around a block's residual sum (the reference's FusedAddRmsNormOp,
+    src/kernels/fused_add_rmsnorm.rs:53-110, with the norm after the block, its
+    gate, scales and dropout).  Primary input x, other f; outputs (y, h)."""
+
+    name = "block_norm"
+
+    def __init__(self, eps: float = 1e-5, residual_scale: float = 1.0, branch_scale: float = 1.0,
+                 p: float = 0.0, site: int = 0):
+        self.eps = float(eps)
+        self.residual_scale = float(residual_scale)
+        self.branch_scale = float(branch_scale)
+        self.p = float(p)
+        self.site = int(site)
+
+    def infer_output_shape(self, input_shapes):
+        return tuple(input_shapes[0])
+
+    def n_activation_inputs(self) -> int:
+        return 2
+
+    def param_shapes(self, input_shapes, output_shape=None):
+        return []
+
+    def has_backward(self) -> bool:
+        return True
+
+    def _kw(self, rng):
+        return dict(eps=self.eps, residual_scale=self.residual_scale,
+                    branch_scale=self.branch_scale, p=self.p, rng=rng, site=self.site)
+
+    def forward(self, x, f, w_post=None, gate=None, w_pre=None, rng=None):
+        return block_norm(x, f, w_post, gate, w_pre, **self._kw(rng))
+
+    def backward(self, f, y, grad_y, grad_h, w_post=None, gate=None, w_pre=None, rng=None):
+        return block_norm_bwd(f, y, grad_y, grad_h, w_post, gate, w_pre, **self._kw(rng))
+
+
+class DropoutOp:
+    """Dropout by a counter-based generator; forward and backward draw the same mask."""
+
+    name = "dropout"
+
+    def __init__(self, p: float, site: int = 0):
+        self.p = float(p)
+        self.site = int(site)
+
+    def infer_output_shape(self, input_shapes):
+        return tuple(input_shapes[0])
+
+    def n_activation_inputs(self) -> int:
+        return 1
+
+    def param_shapes(self, input_shapes, output_shape=None):
+        return []
+
+    def has_backward(self) -> bool:
+        return True
+
+    def forward(self, x, rng, residual=None):
+        return dropout(x, self.p, rng, self.site, residual=residual)
+
+    def backward(self, grad_output, rng):
+        return dropout(grad_output, self.p, rng, self.site)
