@@ -33,17 +33,19 @@ namespace tfb {
 
 enum FfnAct : int { FFN_ACT_SILU = 0, FFN_ACT_GELU = 1, FFN_ACT_GELU_TANH = 2 };
 
-// act(g)
+// act(g).  The quotients use __fdividef (2 ulp; 0 for a divisor above 2^126,
+// where the result is below 1e-36): a full fp32 division is a dozen
+// instructions, and the epilogue of a short product is bound by its own.
 template <int ACT>
 __device__ __forceinline__ float ffn_act(float g) {
   if constexpr (ACT == FFN_ACT_SILU) {
-    return g / (1.0f + __expf(-g));
+    return __fdividef(g, 1.0f + __expf(-g));
   } else if constexpr (ACT == FFN_ACT_GELU) {
     return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
   } else {
     // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), v = sqrt(2/pi) (g + 0.044715 g^3)
     const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    return g / (1.0f + __expf(-2.0f * v));
+    return __fdividef(g, 1.0f + __expf(-2.0f * v));
   }
 }
 
@@ -51,7 +53,7 @@ __device__ __forceinline__ float ffn_act(float g) {
 template <int ACT>
 __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope) {
   if constexpr (ACT == FFN_ACT_SILU) {
-    const float s = 1.0f / (1.0f + __expf(-g));
+    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
     value = ffn_act<ACT>(g);
     slope = s * (1.0f + g * (1.0f - s));
   } else if constexpr (ACT == FFN_ACT_GELU) {
@@ -60,7 +62,7 @@ __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope
             g * 0.39894228040143268f * __expf(-0.5f * g * g);
   } else {
     const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    const float s = 1.0f / (1.0f + __expf(-2.0f * v));
+    const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * v));
     value = ffn_act<ACT>(g);
     slope = s + g * s * (1.0f - s) * 2.0f * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
   }
@@ -163,72 +165,84 @@ __device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) 
                      __uint_as_float(v.w));
 }
 
-// Epilogue of one accumulator tile for one warp: TMEM columns acc.. (this
-// warp's lane quarter), output rows row0..row0+31, column block nb.
-template <int MODE, int ACT, class Release>
-__device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
-                                                  uint32_t acc, int row0, int nb, int lane,
-                                                  uint32_t stg, Release&& release_acc) {
+constexpr int kFfnEpiWarps = 8;
+constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
+constexpr int kFfnEpiBytes = GemmPairCfg::EPI_WARP_BYTES * 4 / kFfnEpiWarps;  // a warp's staging
+
+// Epilogue of one accumulator tile for one warp: TMEM columns acc.. of this
+// warp's lane quarter, output rows row0..row0+31, column block nb, the half
+// `hf` of the tile's columns (two warps share a lane quarter: the epilogue of
+// a tile with a short K, bound by its instructions, then takes half the time).
+// Values pass through the warp's 4 KB of shared memory, so that global loads
+// and stores are whole 64- or 128-byte row segments.  wait_acc() blocks until
+// the accumulator is complete; what does not depend on it is loaded first.
+template <int MODE, int ACT, class Wait, class Release>
+__device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
+                                                  uint32_t acc, int row0, int nb, int hf, int lane,
+                                                  uint32_t stg, Wait&& wait_acc,
+                                                  Release&& release_acc) {
   if (row0 >= q.M) {
+    if (!wait_acc()) return false;
     release_acc();
-    return;
+    return true;
   }
   const int rows_valid = q.M - row0;
+  const int r4 = lane >> 3, c4 = (lane & 7) * 4;  // ffn_unstage32: row in a group of 4, column
   if constexpr (MODE == FFN_GLU) {
     // columns 0..127 of the accumulator are gate, 128..255 up of outputs 128 nb..
-    const uint32_t stg_z = stg + 4096;
-    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
-    __nv_bfloat16* a_row0 = p.a + (long long)row0 * p.F;
-    for (int c = 0; c < 2; ++c) {
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t gr[32], ur[32];
-        tmem_ld32(acc + c * 64 + hh * 32, gr);
-        tmem_ld32(acc + 128 + c * 64 + hh * 32, ur);
-        tmem_wait_ld();
-        if (c == 1 && hh == 1) release_acc();
+    if (!wait_acc()) return false;
+    for (int hh = 0; hh < 2; ++hh) {
+      const int c0 = hf * 64 + hh * 32;
+      const int col0 = nb * 128 + c0;
+      uint32_t gr[32], ur[32];
+      tmem_ld32(acc + c0, gr);
+      tmem_ld32(acc + 128 + c0, ur);
+      tmem_wait_ld();
+      if (hh == 1) release_acc();
+      // a: 64-byte rows of 16-byte chunks, XOR-swizzled by pairs of rows
 #pragma unroll
-        for (int jc = 0; jc < 4; ++jc) {
-          uint32_t w[4];
+      for (int jc = 0; jc < 4; ++jc) {
+        uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = 8 * jc + 2 * e;
-            w[e] = pack_bf16x2(
-                ffn_act<ACT>(__uint_as_float(gr[k])) * __uint_as_float(ur[k]),
-                ffn_act<ACT>(__uint_as_float(gr[k + 1])) * __uint_as_float(ur[k + 1]));
-          }
-          gemm_sts128(stg + lane * 128 + (((hh * 4 + jc) ^ (lane & 7)) << 4), w[0], w[1], w[2],
-                      w[3]);
+        for (int e = 0; e < 4; ++e) {
+          const int k = 8 * jc + 2 * e;
+          w[e] = pack_bf16x2(ffn_act<ACT>(__uint_as_float(gr[k])) * __uint_as_float(ur[k]),
+                             ffn_act<ACT>(__uint_as_float(gr[k + 1])) * __uint_as_float(ur[k + 1]));
         }
-        if (p.z) {
-          const int col = nb * 128 + c * 64 + hh * 32 + c4;
-          for (int half = 0; half < 2; ++half) {
-            if (half == 0)
-              ffn_stage32(stg_z, gr, lane);
-            else
-              ffn_stage32(stg_z, ur, lane);
-            __syncwarp();
-            float* z_row0 = p.z + (long long)row0 * 2 * p.F + (half ? p.F : 0);
-#pragma unroll
-            for (int it = 0; it < 8; ++it) {
-              const float4 v = ffn_unstage32(stg_z, it, lane);
-              const int rr = it * 4 + r4;
-              if (rr < rows_valid && col < p.F)
-                *reinterpret_cast<float4*>(z_row0 + (long long)rr * 2 * p.F + col) = v;
-            }
-            __syncwarp();
-          }
-        }
+        gemm_sts128(stg + lane * 64 + ((jc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
       }
       __syncwarp();
-      const int col0 = nb * 128 + c * 64;
-      gemm_store_rows64(stg, a_row0 + col0, nullptr, p.F, lane, rows_valid, p.F - col0);
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int rr = it * 8 + (lane >> 2), jc = lane & 3;
+        const uint4 v = gemm_lds128(stg + rr * 64 + ((jc ^ ((rr >> 1) & 3)) << 4));
+        if (rr < rows_valid && col0 + jc * 8 < p.F)
+          *reinterpret_cast<uint4*>(p.a + (long long)(row0 + rr) * p.F + col0 + jc * 8) = v;
+      }
       __syncwarp();
+      if (p.z) {
+        for (int half = 0; half < 2; ++half) {
+          if (half == 0)
+            ffn_stage32(stg, gr, lane);
+          else
+            ffn_stage32(stg, ur, lane);
+          __syncwarp();
+          float* z_row0 = p.z + (long long)row0 * 2 * p.F + (half ? p.F : 0) + col0 + c4;
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const float4 v = ffn_unstage32(stg, it, lane);
+            const int rr = it * 4 + r4;
+            if (rr < rows_valid && col0 + c4 < p.F)
+              *reinterpret_cast<float4*>(z_row0 + (long long)rr * 2 * p.F) = v;
+          }
+          __syncwarp();
+        }
+      }
     }
   } else if constexpr (MODE == FFN_DGLU) {
-    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
-    for (int c = 0; c < kGemmBN / 32; ++c) {
-      const int col = nb * kGemmBN + c * 32 + c4;
-      float4 g[8], u[8];
+    float4 g[8], u[8];
+    auto load_z = [&](int c) {
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
 #pragma unroll
       for (int it = 0; it < 8; ++it) {
         const int rr = it * 4 + r4;
@@ -238,16 +252,20 @@ __device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const 
           u[it] = *reinterpret_cast<const float4*>(zr + p.F);
         }
       }
+    };
+    load_z(0);
+    if (!wait_acc()) return false;
+    for (int c = 0; c < 4; ++c) {
       uint32_t r[32];
-      tmem_ld32(acc + c * 32, r);
+      tmem_ld32(acc + hf * 128 + c * 32, r);
       tmem_wait_ld();
-      if (c == kGemmBN / 32 - 1) release_acc();
-      const uint32_t sb = stg + (c & 1) * 4096;
-      ffn_stage32(sb, r, lane);
+      if (c == 3) release_acc();
+      ffn_stage32(stg, r, lane);
       __syncwarp();
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
 #pragma unroll
       for (int it = 0; it < 8; ++it) {
-        const float4 d4 = ffn_unstage32(sb, it, lane);
+        const float4 d4 = ffn_unstage32(stg, it, lane);
         const int rr = it * 4 + r4;
         if (rr < rows_valid && col < p.F) {
           const float d[4] = {d4.x, d4.y, d4.z, d4.w};
@@ -271,42 +289,56 @@ __device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const 
               make_uint2(pack_bf16x2(av[0], av[1]), pack_bf16x2(av[2], av[3]));
         }
       }
+      if (c < 3) load_z(c + 1);
+      __syncwarp();
     }
   } else if (q.residual) {
     // the residual is added to the fp32 product: one rounding
-    const int r4 = lane >> 3, c4 = (lane & 7) * 4;
-    for (int c = 0; c < kGemmBN / 32; ++c) {
-      uint32_t r[32];
-      tmem_ld32(acc + c * 32, r);
-      tmem_wait_ld();
-      if (c == kGemmBN / 32 - 1) release_acc();
-      const uint32_t sb = stg + (c & 1) * 4096;
-      ffn_stage32(sb, r, lane);
-      __syncwarp();
-      const int col = nb * kGemmBN + c * 32 + c4;
+    uint2 res[8];
+    auto load_res = [&](int c) {
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
 #pragma unroll
       for (int it = 0; it < 8; ++it) {
-        const float4 v = ffn_unstage32(sb, it, lane);
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < q.N)
+          res[it] = *reinterpret_cast<const uint2*>(q.residual + (long long)(row0 + rr) * q.N + col);
+      }
+    };
+    load_res(0);
+    if (!wait_acc()) return false;
+    for (int c = 0; c < 4; ++c) {
+      uint32_t r[32];
+      tmem_ld32(acc + hf * 128 + c * 32, r);
+      tmem_wait_ld();
+      if (c == 3) release_acc();
+      ffn_stage32(stg, r, lane);
+      __syncwarp();
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const float4 v = ffn_unstage32(stg, it, lane);
         const int rr = it * 4 + r4;
         if (rr < rows_valid && col < q.N) {
-          const long long at = (long long)(row0 + rr) * q.N + col;
-          const uint2 w = *reinterpret_cast<const uint2*>(q.residual + at);
-          *reinterpret_cast<uint2*>(q.out + at) = make_uint2(
+          const uint2 w = res[it];
+          *reinterpret_cast<uint2*>(q.out + (long long)(row0 + rr) * q.N + col) = make_uint2(
               pack_bf16x2(v.x + __uint_as_float(w.x << 16),
                           v.y + __uint_as_float(w.x & 0xFFFF0000u)),
               pack_bf16x2(v.z + __uint_as_float(w.y << 16),
                           v.w + __uint_as_float(w.y & 0xFFFF0000u)));
         }
       }
+      if (c < 3) load_res(c + 1);
+      __syncwarp();
     }
   } else {
-    for (int c = 0; c < kGemmBN / 64; ++c) {
+    if (!wait_acc()) return false;
+    for (int c = 0; c < 2; ++c) {
+      const int col0 = nb * kGemmBN + hf * 128 + c * 64;
       uint32_t r0[32], r1[32];
-      tmem_ld32(acc + c * 64, r0);
-      tmem_ld32(acc + c * 64 + 32, r1);
+      tmem_ld32(acc + hf * 128 + c * 64, r0);
+      tmem_ld32(acc + hf * 128 + c * 64 + 32, r1);
       tmem_wait_ld();
-      if (c == kGemmBN / 64 - 1) release_acc();
-      const uint32_t sb = stg + (c & 1) * 4096;
+      if (c == 1) release_acc();
 #pragma unroll
       for (int jc = 0; jc < 8; ++jc) {
         uint32_t w[4];
@@ -316,15 +348,15 @@ __device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const 
           w[e] = pack_bf16x2(__uint_as_float(k < 32 ? r0[k] : r1[k - 32]),
                              __uint_as_float(k + 1 < 32 ? r0[k + 1] : r1[k + 1 - 32]));
         }
-        gemm_sts128(sb + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+        gemm_sts128(stg + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
       }
       __syncwarp();
-      const int col0 = nb * kGemmBN + c * 64;
-      gemm_store_rows64(sb, q.out + (long long)row0 * q.N + col0, nullptr, q.N, lane, rows_valid,
+      gemm_store_rows64(stg, q.out + (long long)row0 * q.N + col0, nullptr, q.N, lane, rows_valid,
                         q.N - col0);
       __syncwarp();
     }
   }
+  return true;
 }
 
 // Roles, barriers, ring and TMEM as in gemm_bf16_sm100_pair_kernel.  A k-block
@@ -333,7 +365,7 @@ __device__ __forceinline__ void ffn_epilogue_warp(const FfnPairParams& p, const 
 // (8 KB between the 64-column halves, 1 KB between groups of 8 K rows, 2 KB a
 // K step of 16).
 template <int MODE, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     ffn_pair_kernel(const __grid_constant__ FfnMaps maps,
                     const __grid_constant__ FfnPairParams p) {
   using C = GemmPairCfg;
@@ -357,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(PB_AFULL + b), 1);
-      mbar_init(bar(PB_AEMPTY + b), 8);  // 4 epilogue warps x 2 CTAs
+      mbar_init(bar(PB_AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
     }
     mbar_init(bar(PB_DRAIN), 1);
     *abort_flag = 0;
@@ -476,8 +508,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
   } else {
     // ===================== epilogue (both CTAs) =========================
-    const int quarter = warp & 3;
-    const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * C::EPI_WARP_BYTES;
+    const int quarter = warp & 3, hf = (warp - 2) >> 2;
+    const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * kFfnEpiBytes;
     const uint32_t aempty0 = mapa_cta(bar(PB_AEMPTY), 0);
     for (int i = 0;; ++i) {
       const int t = ffn_next(p, pair, n_pairs, i);
@@ -485,16 +517,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       int mb, nb;
       const FfnProblem& q = p.prob[ffn_tile(p, t, mb, nb)];
       const int b = i & 1, use = i >> 1;
-      if (!mbar_wait_warp(bar(PB_AFULL + b), use & 1, abort_flag, 926)) break;
-      tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * kGemmBN;
       const int row0 = mb * 256 + (int)crank * 128 + quarter * 32;
+      auto wait_acc = [&]() {
+        const bool ok = mbar_wait_warp(bar(PB_AFULL + b), use & 1, abort_flag, 926);
+        tc_fence_after();
+        return ok;
+      };
       auto release_acc = [&]() {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
       };
-      ffn_epilogue_warp<MODE, ACT>(p, q, acc, row0, nb, lane, stg, release_acc);
+      if (!ffn_epilogue_warp<MODE, ACT>(p, q, acc, row0, nb, hf, lane, stg, wait_acc, release_acc))
+        break;
     }
   }
 

@@ -1025,7 +1025,7 @@ int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
     prm.bal_rounds = (int)std::min<long long>(
         prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
   ffn_pair_kernel<MODE, ACT>
-      <<<(unsigned)(2 * clusters), kGemmThreads, GemmPairCfg::SMEM_ALLOC, st>>>(maps, prm);
+      <<<(unsigned)(2 * clusters), kFfnThreads, GemmPairCfg::SMEM_ALLOC, st>>>(maps, prm);
   return launch_status();
 }
 

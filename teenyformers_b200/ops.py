@@ -349,14 +349,18 @@ def linear_push(x: torch.Tensor, weight: torch.Tensor, peer_recv_ptrs, rank: int
 
 
 # ----------------------------------------------------------------- feed-forward side of a block
-def _launch(device: torch.device, name: str, *args) -> None:
-    """call(name, *args, stream) on `device`'s current stream, with that device
-    current (the library launches on the current device)."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
+# These wrappers sit on the decode path, where a kernel takes a few microseconds:
+# messages are formatted only when they are raised, and the stream and device
+# are read without torch's Python objects around them.
+def _launch(x: torch.Tensor, name: str, *args) -> None:
+    """call(name, *args, stream) on the current stream of x's device, with that
+    device current (the library launches on the current device)."""
+    index = x.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
         call(name, *args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             call(name, *args, stream)
 
 
@@ -364,19 +368,21 @@ def _addr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _dense(device: torch.device, dtype: torch.dtype, what: str, *ts) -> None:
+def _dense(x: torch.Tensor, dtype: torch.dtype, what: str, *ts) -> None:
+    index = x.get_device()
     for t in ts:
-        if t is not None:
-            _need(t.dtype == dtype and t.device == device and t.is_contiguous(),
-                  f"{what} tensors must be contiguous {dtype} tensors on {device}")
+        if t is not None and (t.dtype != dtype or t.get_device() != index
+                              or not t.is_contiguous()):
+            raise ValueError(f"{what} tensors must be contiguous {dtype} tensors on {x.device}")
 
 
-def _buffer(t: torch.Tensor | None, shape, dtype: torch.dtype, device: torch.device,
+def _buffer(t: torch.Tensor | None, shape, dtype: torch.dtype, x: torch.Tensor,
             name: str) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _need(tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.device == device
-          and t.is_contiguous(), f"{name} must be a contiguous {dtype} {tuple(shape)} tensor")
+        return torch.empty(shape, dtype=dtype, device=x.device)
+    if (t.shape != shape or t.dtype != dtype or t.get_device() != x.get_device()
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {x.device}")
     return t
 
 
@@ -401,13 +407,13 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
     [..., 2 * d_ff] fp32 = x [Wg; Wu]^T for gated_ffn_bwd.  ``out``, ``act_out``
     ([..., d_ff] scratch) and ``z_out`` are buffers to use instead of new ones."""
     m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
-    dev, lead = x.device, tuple(x.shape[:-1])
-    _dense(dev, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, residual)
+    lead = x.shape[:-1]
+    _dense(x, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, residual)
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
-    y = _buffer(out, lead + (d,), torch.bfloat16, dev, "out")
-    a = _buffer(act_out, lead + (d_ff,), torch.bfloat16, dev, "act_out")
-    z = _buffer(z_out, lead + (2 * d_ff,), torch.float32, dev, "z_out") if save else None
-    _launch(dev, "tf_b200_gated_ffn_fwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
+    y = _buffer(out, x.shape, torch.bfloat16, x, "out")
+    a = _buffer(act_out, lead + (d_ff,), torch.bfloat16, x, "act_out")
+    z = _buffer(z_out, lead + (2 * d_ff,), torch.float32, x, "z_out") if save else None
+    _launch(x, "tf_b200_gated_ffn_fwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
             w_down.data_ptr(), _addr(residual), a.data_ptr(), _addr(z), y.data_ptr(), m, d, d_ff,
             int(act))
     return (y, z) if save else y
@@ -420,19 +426,16 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor
     a False in ``need`` skips that gradient (None in its place).  The residual's
     gradient is dy itself.  ``grads``: three tensors to write instead of new ones."""
     m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
-    dev = x.device
-    _dense(dev, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, dy)
-    _dense(dev, torch.float32, "z", z)
+    _dense(x, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, dy)
+    _dense(x, torch.float32, "z", z)
     _need(dy.shape == x.shape, "dy must have x's shape")
-    _need(tuple(z.shape) == tuple(x.shape[:-1]) + (2 * d_ff,), "z must be [..., 2 * d_ff]")
+    _need(z.shape == x.shape[:-1] + (2 * d_ff,), "z must be [..., 2 * d_ff]")
     given = (None, None, None) if grads is None else grads
-    g = [_buffer(t, like.shape, torch.bfloat16, dev, "a gradient") if on else None
+    g = [_buffer(t, like.shape, torch.bfloat16, x, "a gradient") if on else None
          for t, like, on in zip(given, (x, w_gate_up, w_down), need)]
     n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d_ff)
-    ws = torch.empty(int(n), dtype=torch.uint8, device=dev) if workspace is None else workspace
-    _need(ws.device == dev and ws.is_contiguous() and ws.numel() * ws.element_size() >= n,
-          "workspace too small")
-    _launch(dev, "tf_b200_gated_ffn_bwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
+    ws = _workspace(n, workspace, x)
+    _launch(x, "tf_b200_gated_ffn_bwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
             w_down.data_ptr(), z.data_ptr(), dy.data_ptr(), _addr(g[0]), _addr(g[1]), _addr(g[2]),
             ws.data_ptr(), m, d, d_ff, int(act))
     return tuple(g)
@@ -446,14 +449,23 @@ def dropout_rng(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
     return torch.tensor([wrap(seed), wrap(offset)], dtype=torch.int64, device=device)
 
 
-def _rng_addr(p: float, rng: torch.Tensor | None, site: int, device: torch.device):
+def _rng_addr(p: float, rng: torch.Tensor | None, site: int, x: torch.Tensor):
     _need(0 <= site < 1 << 32, "site must be a 32-bit number")
     if not p:
         return None
-    _need(rng is not None and rng.dtype == torch.int64 and rng.numel() == 2
-          and rng.is_contiguous() and rng.device == device,
-          f"p > 0 needs rng, an int64 [2] tensor (seed, offset) on {device}")
+    if (rng is None or rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous()
+            or rng.get_device() != x.get_device()):
+        raise ValueError(f"p > 0 needs rng, an int64 [2] tensor (seed, offset) on {x.device}")
     return rng.data_ptr()
+
+
+def _workspace(n: int, ws: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
+    if ws is None:
+        return torch.empty(int(n), dtype=torch.uint8, device=x.device)
+    if ws.get_device() != x.get_device() or not ws.is_contiguous() or \
+            ws.numel() * ws.element_size() < n:
+        raise ValueError(f"workspace must be contiguous and have {n} bytes on {x.device}")
+    return ws
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
@@ -462,13 +474,13 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
     counter-based generator and never stored.  The backward pass is
     ``dropout(dy, p, rng, site)``.  ``out`` may be x or residual."""
     fn = {torch.float32: "tf_b200_dropout_f32", torch.bfloat16: "tf_b200_dropout_bf16"}.get(x.dtype)
-    _need(fn is not None, f"unsupported dtype {x.dtype}")
+    if fn is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
     _need(x.is_cuda, "x must be a CUDA tensor")
-    dev = x.device
-    _dense(dev, x.dtype, "dropout", x, residual)
+    _dense(x, x.dtype, "dropout", x, residual)
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
-    y = _buffer(out, x.shape, x.dtype, dev, "out")
-    _launch(dev, fn, x.data_ptr(), _addr(residual), y.data_ptr(), _rng_addr(p, rng, site, dev),
+    y = _buffer(out, x.shape, x.dtype, x, "out")
+    _launch(x, fn, x.data_ptr(), _addr(residual), y.data_ptr(), _rng_addr(p, rng, site, x),
             x.numel(), float(p), int(site))
     return y
 
@@ -502,13 +514,12 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None, w_post: torch.Tensor | N
     every rows / gate_rows consecutive rows.  f None: only the norm before a block
     (y is x).  Returns (y, h), h None without w_pre.  ``out`` may be x."""
     rows, cols, gate_rows = _norm_shapes(x, w_post, gate, w_pre)
-    dev = x.device
-    _dense(dev, torch.bfloat16, "block_norm", x, f, w_post, gate, w_pre)
+    _dense(x, torch.bfloat16, "block_norm", x, f, w_post, gate, w_pre)
     _need(f is None or f.shape == x.shape, "f must have x's shape")
-    y = x if f is None else _buffer(out, x.shape, x.dtype, dev, "out")
-    h = None if w_pre is None else _buffer(norm_out, x.shape, x.dtype, dev, "norm_out")
-    _launch(dev, "tf_b200_block_norm_fwd_bf16", x.data_ptr(), _addr(f), _addr(w_post), _addr(gate),
-            _addr(w_pre), y.data_ptr(), _addr(h), _rng_addr(p, rng, site, dev), rows, cols, gate_rows,
+    y = x if f is None else _buffer(out, x.shape, x.dtype, x, "out")
+    h = None if w_pre is None else _buffer(norm_out, x.shape, x.dtype, x, "norm_out")
+    _launch(x, "tf_b200_block_norm_fwd_bf16", x.data_ptr(), _addr(f), _addr(w_post), _addr(gate),
+            _addr(w_pre), y.data_ptr(), _addr(h), _rng_addr(p, rng, site, x), rows, cols, gate_rows,
             float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
     return y, h
 
@@ -525,8 +536,7 @@ def block_norm_bwd(f: torch.Tensor | None, y: torch.Tensor | None, dy: torch.Ten
     like = dy if dy is not None else dh
     _need(like is not None, "dy or dh is needed")
     rows, cols, gate_rows = _norm_shapes(like, w_post, gate, w_pre)
-    dev = like.device
-    _dense(dev, torch.bfloat16, "block_norm", f, y, dy, dh, w_post, gate, w_pre)
+    _dense(like, torch.bfloat16, "block_norm", f, y, dy, dh, w_post, gate, w_pre)
     for t in (f, y, dy, dh):
         _need(t is None or t.shape == like.shape, "f, y, dy and dh must have one shape")
     _need((w_pre is None) == (dh is None), "dh belongs to w_pre")
@@ -538,12 +548,10 @@ def block_norm_bwd(f: torch.Tensor | None, y: torch.Tensor | None, dy: torch.Ten
     dx, df = torch.empty_like(like), torch.empty_like(like) if branch else None
     dw_post, dgate, dw_pre = new(w_post), new(gate), new(w_pre)
     n = _capi.raw("tf_b200_block_norm_bwd_workspace_size", rows, cols)
-    ws = torch.empty(int(n), dtype=torch.uint8, device=dev) if workspace is None else workspace
-    _need(ws.device == dev and ws.is_contiguous() and ws.numel() * ws.element_size() >= n,
-          "workspace too small")
-    _launch(dev, "tf_b200_block_norm_bwd_bf16", _addr(f), _addr(y), _addr(dy), _addr(dh),
+    ws = _workspace(n, workspace, like)
+    _launch(like, "tf_b200_block_norm_bwd_bf16", _addr(f), _addr(y), _addr(dy), _addr(dh),
             _addr(w_post), _addr(gate), _addr(w_pre), dx.data_ptr(), _addr(df), _addr(dw_post),
-            _addr(dgate), _addr(dw_pre), _rng_addr(p, rng, site, dev), ws.data_ptr(), rows, cols,
+            _addr(dgate), _addr(dw_pre), _rng_addr(p, rng, site, like), ws.data_ptr(), rows, cols,
             gate_rows, float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
     return dx, df, dw_post, dgate, dw_pre
 
