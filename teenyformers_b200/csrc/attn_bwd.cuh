@@ -122,15 +122,6 @@ struct BwdParams {
   int n_items;        // fused path: BHkv * n_kt
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_dst),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
 __device__ __forceinline__ void mbar_wait_noabort(uint32_t bar, uint32_t parity, int site) {
   (void)mbar_wait(bar, parity, nullptr, site);
 }

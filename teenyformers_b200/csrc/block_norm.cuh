@@ -50,115 +50,302 @@ struct BlockNormParams {
   DropoutParams drop;
 };
 
-// Sums NV values over a team's threads.  `buf` alternates between calls: a
-// thread can only write buffer b again after the team's barrier of the call
+// ---------------------------------------------------------------- teams and rings
+// A row is worked on by a team of WPR warps (the smallest of 1, 2, 4, 8 that
+// holds it at VPT 16-byte vectors a thread); a 256-thread CTA has 8 / WPR
+// teams, each with a contiguous run of rows.  The rows' tensors arrive through
+// a ring of shared-memory stages, filled by bulk copies of one or several
+// whole rows (rows are contiguous), so the loads of the next rows run under
+// the arithmetic and the two reductions of this one: with plain loads the
+// forward pass of 16384 x 4096 took 100 us and the backward pass 370 us, bound
+// by load latency (4.7 and more stalled cycles an instruction).
+constexpr int kBnStages = 3;
+constexpr int kBnCtas = 296;  // two CTAs on each of 148 SMs
+constexpr int kBnRingBytes = 98304;  // a CTA's stages, where a row is not longer
+
+struct BlockNormTeams {
+  int wpr, vpt, rows_per_team, n_teams, n_ctas;
+  int rows_per_stage, smem;
+};
+// A pure function of the shape, so that the workspace query and the launch
+// agree.  `tensors`: the most that a row's stage holds.
+inline BlockNormTeams block_norm_teams(int rows, int cols, int tensors) {
+  BlockNormTeams t;
+  const int nvec = cols / 8;
+  t.vpt = nvec <= 32 ? 1 : nvec <= 512 ? 2 : 4;
+  t.wpr = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
+  const int teams = kBnWarps / t.wpr;
+  const int want = kBnCtas * teams;
+  t.rows_per_team = rows > 0 ? (int)(((long long)rows + want - 1) / want) : 1;
+  t.n_teams = (int)(((long long)rows + t.rows_per_team - 1) / t.rows_per_team);
+  t.n_ctas = (t.n_teams + teams - 1) / teams;
+  const int row_stage = teams * kBnStages * tensors * cols * 2;
+  int r = kBnRingBytes / row_stage;
+  r = r < 1 ? 1 : r > 8 ? 8 : r;
+  t.rows_per_stage = r < t.rows_per_team ? r : t.rows_per_team;
+  t.smem = t.rows_per_stage * row_stage;
+  return t;
+}
+
+__device__ __forceinline__ uint4 bn_lds(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Eight bf16 as four packed fp32 pairs, and back.
+__device__ __forceinline__ void bn_unpack(const uint4& v, uint64_t (&f)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    f[i] = f2_make(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint4 bn_pack(const uint64_t (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    f2_split(f[i], lo, hi);
+    w[i] = pack_bf16x2(lo, hi);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float bn_hsum(uint64_t v) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return lo + hi;
+}
+// Dropout of eight elements held as pairs.
+__device__ __forceinline__ void bn_dropout(const DropoutParams& d, const PhiloxState& s,
+                                           uint32_t group, uint64_t (&f)[4]) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_split(f[i], v[2 * i], v[2 * i + 1]);
+  dropout8(d, s, group, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = f2_make(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ void bn_store_f32(float* dst, int v, const uint64_t (&f)[4]) {
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_split(f[i], a[2 * i], a[2 * i + 1]);
+  reinterpret_cast<float4*>(dst)[2 * v] = make_float4(a[0], a[1], a[2], a[3]);
+  reinterpret_cast<float4*>(dst)[2 * v + 1] = make_float4(a[4], a[5], a[6], a[7]);
+}
+
+// One team's ring of row stages.  Chunk k is the rows from row0 + k * step on,
+// rows_per_stage of them or as many as there are before row1.
+template <int TENSORS>
+struct BnRing {
+  const __nv_bfloat16* src[TENSORS];  // null: absent
+  uint32_t bar, data;                 // kBnStages mbarriers; the team's stages
+  uint32_t slot, stage;               // bytes of one tensor's rows, and of a stage
+  int rows_per_stage, row0, row1, cols, present;
+  long long step;
+
+  // (the team's first thread)
+  __device__ __forceinline__ void issue(int k) const {
+    const long long r = row0 + k * step;
+    if (r >= row1) return;
+    const uint32_t bytes = (uint32_t)min((long long)rows_per_stage, row1 - r) * cols * 2;
+    const int s = k % kBnStages;
+    mbar_arrive_expect_tx(bar + s * 8, bytes * present);
+#pragma unroll
+    for (int i = 0; i < TENSORS; ++i)
+      if (src[i])
+        bulk_load(data + s * stage + i * slot, src[i] + r * cols, bytes, bar + s * 8);
+  }
+  // Every thread of the team.  A wait that runs out (a fault) is recorded and
+  // makes the later ones return at once; the outputs are then invalid.
+  __device__ __forceinline__ void wait(int k, volatile int* abort_flag, int site) const {
+    (void)mbar_wait(bar + (k % kBnStages) * 8, (k / kBnStages) & 1, abort_flag, site);
+  }
+  __device__ __forceinline__ uint32_t at(int k, int i, int row_in_stage) const {
+    return data + (k % kBnStages) * stage + i * slot + (uint32_t)row_in_stage * cols * 2;
+  }
+};
+
+template <int WPR>
+__device__ __forceinline__ void team_sync(int team) {
+  if constexpr (WPR == 1)
+    __syncwarp();
+  else
+    named_bar_sync(1 + team, WPR * 32);
+}
+
+// Sums NV <= 4 values over a team's threads.  `buf` alternates between calls:
+// a thread can only write buffer b again after the team's barrier of the call
 // in between, which every thread reaches after its reads of b.
 template <int WPR, int NV>
-__device__ __forceinline__ void team_sum(float (&v)[NV], float (*red)[2][kBnWarps][4], int& buf,
+__device__ __forceinline__ void team_sum(float (&v)[NV], float4 (*red)[kBnWarps], int& buf,
                                          int team, int warp_in_team) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
     for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   if constexpr (WPR > 1) {
-    float(*r)[4] = (*red)[buf] + team * WPR;
+    float4* r = red[buf] + team * WPR;
     buf ^= 1;
     if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int k = 0; k < NV; ++k) r[warp_in_team][k] = v[k];
+      r[warp_in_team] = make_float4(v[0], NV > 1 ? v[1 % NV] : 0.0f, NV > 2 ? v[2 % NV] : 0.0f, 0.0f);
     named_bar_sync(1 + team, WPR * 32);
+    float4 t = r[0];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      v[k] = r[0][k];
-#pragma unroll
-      for (int w = 1; w < WPR; ++w) v[k] += r[w][k];
+    for (int w = 1; w < WPR; ++w) {
+      const float4 a = r[w];
+      t.x += a.x;
+      if (NV > 1) t.y += a.y;
+      if (NV > 2) t.z += a.z;
     }
+    v[0] = t.x;
+    if constexpr (NV > 1) v[1] = t.y;
+    if constexpr (NV > 2) v[2] = t.z;
   }
 }
 
+// ---------------------------------------------------------------- forward
+// VPT vectors a thread; the weights stay in registers over the team's rows
+// (gate * w_post as their fp32 product, renewed where the gate's row changes).
 template <int WPR, int VPT>
-__global__ void __launch_bounds__(kBnThreads) block_norm_fwd_kernel(const BlockNormParams p) {
-  constexpr int TEAMS = kBnWarps / WPR, TT = WPR * 32;
-  __shared__ float red[2][kBnWarps][4];
-  const int team = (int)threadIdx.x / TT, tid = (int)threadIdx.x % TT;
-  const long long row = (long long)blockIdx.x * TEAMS + team;
-  if (row >= p.rows) return;  // whole teams leave: their barriers are their own
+__global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
+    block_norm_fwd_kernel(const BlockNormParams p, const BlockNormTeams tm) {
+  constexpr int TT = WPR * 32;
+  extern __shared__ uint4 bn_stages[];
+  __shared__ float4 red[2][kBnWarps];
+  __shared__ uint64_t bars[kBnWarps * kBnStages];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int team_in_cta = (int)threadIdx.x / TT, tid = (int)threadIdx.x % TT;
+  const int team = (int)blockIdx.x * (kBnWarps / WPR) + team_in_cta;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (team >= tm.n_teams) return;  // whole teams leave: their barriers are their own
   const int nvec = p.cols / 8;
-  const long long base = row * p.cols;
+  BnRing<2> ring;
+  ring.src[0] = p.f, ring.src[1] = p.x;
+  ring.present = p.f ? 2 : 1;
+  ring.cols = p.cols, ring.rows_per_stage = tm.rows_per_stage;
+  ring.row0 = team * tm.rows_per_stage;
+  ring.row1 = p.rows;
+  ring.step = (long long)tm.n_teams * tm.rows_per_stage;
+  ring.slot = (uint32_t)tm.rows_per_stage * p.cols * 2;
+  ring.stage = 2 * ring.slot;
+  ring.bar = smem_u32(bars + team_in_cta * kBnStages);
+  ring.data = smem_u32(bn_stages) + team_in_cta * kBnStages * ring.stage;
+  if (tid == 0)
+    for (int k = 0; k < kBnStages; ++k) ring.issue(k);
   int buf = 0;
-  uint4 xv[VPT], fv[VPT];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = tid + i * TT;
-    if (v < nvec) {
-      xv[i] = reinterpret_cast<const uint4*>(p.x + base)[v];
-      if (p.f) fv[i] = reinterpret_cast<const uint4*>(p.f + base)[v];
-    }
-  }
-  float r_f = 1.0f;
-  if (p.f && p.w_post) {
-    float ss[1] = {0.0f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (tid + i * TT < nvec) {
-        float a[8];
-        bf16x8_to_f32(fv[i], a);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss[0] = fmaf(a[e], a[e], ss[0]);
-      }
-    team_sum<WPR, 1>(ss, &red, buf, team, tid >> 5);
-    r_f = rsqrtf(ss[0] / (float)p.cols + p.eps);
-  }
   PhiloxState rng = {};
   if (p.drop.rng) rng = philox_state(p.drop);
-  const __nv_bfloat16* gate_row =
-      p.gate ? p.gate + (row / p.rows_per_gate) * (long long)p.cols : nullptr;
-  float y[VPT][8];
-  float ssy[1] = {0.0f};
+  const float inv_c = 1.0f / (float)p.cols;
+  const uint64_t rs2 = f2_make(p.residual_scale, p.residual_scale);
+
+  uint64_t wg[VPT][4];  // gate * w_post
+  uint4 wn[VPT];        // w_pre
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = tid + i * TT;
-    if (v < nvec) {
-      bf16x8_to_f32(xv[i], y[i]);
-      if (p.f) {
-        float b[8], w[8];
-        bf16x8_to_f32(fv[i], b);
-        if (p.w_post) {
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.w_post)[v], w);
+    wn[i] = p.w_pre && v < nvec ? reinterpret_cast<const uint4*>(p.w_pre)[v] : make_uint4(0, 0, 0, 0);
+  }
+  int gate_row = -1;
+  auto load_gate = [&](int g) {
+    gate_row = g;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) b[e] = b[e] * r_f * w[e];
-        }
-        if (gate_row) {
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(gate_row)[v], w);
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * TT;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) b[e] *= w[e];
-        }
-        if (p.drop.rng) dropout8(p.drop, rng, (uint32_t)(base / 8 + v), b);
+      for (int e = 0; e < 4; ++e) wg[i][e] = f2_make(1.0f, 1.0f);
+      if (v >= nvec) continue;
+      if (p.w_post) bn_unpack(reinterpret_cast<const uint4*>(p.w_post)[v], wg[i]);
+      if (p.gate) {
+        uint64_t g4[4];
+        bn_unpack(reinterpret_cast<const uint4*>(p.gate + (long long)g * p.cols)[v], g4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] = p.residual_scale * y[i][e] + p.branch_scale * b[e];
-        reinterpret_cast<uint4*>(p.y + base)[v] = f32_to_bf16x8(y[i]);
+        for (int e = 0; e < 4; ++e) wg[i][e] = f2_mul(wg[i][e], g4[e]);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ssy[0] = fmaf(y[i][e], y[i][e], ssy[0]);
     }
-  }
-  if (!p.w_pre) return;
-  team_sum<WPR, 1>(ssy, &red, buf, team, tid >> 5);
-  const float r_y = rsqrtf(ssy[0] / (float)p.cols + p.eps);
+  };
+  if (p.f) load_gate(ring.row0 / p.rows_per_gate);
+
+  int k = 0;
+  for (long long r = ring.row0; r < ring.row1; r += ring.step, ++k) {
+    ring.wait(k, abort_flag, 941);
+    const int here = (int)min((long long)tm.rows_per_stage, ring.row1 - r);
+    for (int j = 0; j < here; ++j) {
+      const int row = (int)r + j;
+      const long long base = (long long)row * p.cols;
+      const uint32_t fa = ring.at(k, 0, j), xa = ring.at(k, 1, j);
+      float r_f = 1.0f;
+      if (p.f && p.w_post) {
+        uint64_t ss = 0;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = tid + i * TT;
-    if (v < nvec) {
-      float w[8];
-      bf16x8_to_f32(reinterpret_cast<const uint4*>(p.w_pre)[v], w);
+        for (int i = 0; i < VPT; ++i)
+          if (tid + i * TT < nvec) {
+            uint64_t a[4];
+            bn_unpack(bn_lds(fa + (tid + i * TT) * 16), a);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = y[i][e] * r_y * w[e];
-      reinterpret_cast<uint4*>(p.h + base)[v] = f32_to_bf16x8(w);
+            for (int e = 0; e < 4; ++e) ss = f2_fma(a[e], a[e], ss);
+          }
+        float s1[1] = {bn_hsum(ss)};
+        team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
+        r_f = rsqrtf(s1[0] * inv_c + p.eps);
+      }
+      if (p.gate && row / p.rows_per_gate != gate_row) load_gate(row / p.rows_per_gate);
+      const float bf = p.branch_scale * r_f;
+      const uint64_t bf2 = f2_make(bf, bf);
+      uint64_t y[VPT][4], ssy = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = tid + i * TT;
+        if (v < nvec) {
+          bn_unpack(bn_lds(xa + v * 16), y[i]);
+          if (p.f) {
+            uint64_t b[4];
+            bn_unpack(bn_lds(fa + v * 16), b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = f2_mul(b[e], wg[i][e]);
+            if (p.drop.rng) bn_dropout(p.drop, rng, (uint32_t)(base / 8 + v), b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[i][e] = f2_fma(b[e], bf2, f2_mul(y[i][e], rs2));
+            reinterpret_cast<uint4*>(p.y + base)[v] = bn_pack(y[i]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ssy = f2_fma(y[i][e], y[i][e], ssy);
+        }
+      }
+      if (p.w_pre) {
+        float s1[1] = {bn_hsum(ssy)};
+        team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
+        const float r_y = rsqrtf(s1[0] * inv_c + p.eps);
+        const uint64_t ry2 = f2_make(r_y, r_y);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int v = tid + i * TT;
+          if (v < nvec) {
+            uint64_t w[4];
+            bn_unpack(wn[i], w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = f2_mul(f2_mul(y[i][e], ry2), w[e]);
+            reinterpret_cast<uint4*>(p.h + base)[v] = bn_pack(w);
+          }
+        }
+      }
     }
+    team_sync<WPR>(team_in_cta);  // every thread has read the stage
+    if (tid == 0) ring.issue(k + kBnStages);
   }
+  if (*abort_flag && tid == 0)  // copies in flight land before the shared memory goes away
+    for (int u = max(0, k - kBnStages); u < k; ++u) ring.wait(u, nullptr, 942);
 }
 
-// ------------------------------------------------------------------ backward
+// ---------------------------------------------------------------- backward
 struct BlockNormBwdParams {
   const __nv_bfloat16* f;       // read when w_post or gate is set
   const __nv_bfloat16* w_post;
@@ -170,215 +357,292 @@ struct BlockNormBwdParams {
   __nv_bfloat16* dx;
   __nv_bfloat16* df;            // null: no branch
   __nv_bfloat16* dgate;
-  float* part_post;             // [n_teams, cols]
-  float* part_pre;              // [n_teams, cols]
+  float* part_post;             // [n_ctas, cols]
+  float* part_pre;              // [n_ctas, cols]
   float* part_gate;             // [n_teams, 2, cols]
-  int rows, cols, rows_per_gate, rows_per_team, n_teams;
+  int rows, cols, rows_per_gate;
   float eps, residual_scale, branch_scale;
   DropoutParams drop;
 };
 
-// The teams of a call: two 256-thread CTAs on each of 148 SMs, contiguous
-// rows to each team.  A pure function of the shape, so that the workspace
-// query and the launch agree.
-constexpr int kBnBwdCtas = 296;
-
-struct BlockNormTeams {
-  int wpr, vpt, rows_per_team, n_teams;
-};
-inline BlockNormTeams block_norm_teams(int rows, int cols) {
-  BlockNormTeams t;
-  const int nvec = cols / 8;
-  t.vpt = nvec <= 32 ? 1 : nvec <= 512 ? 2 : 4;
-  t.wpr = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
-  const int want = kBnBwdCtas * (kBnWarps / t.wpr);
-  t.rows_per_team = rows > 0 ? (int)(((long long)rows + want - 1) / want) : 1;
-  t.n_teams = (int)(((long long)rows + t.rows_per_team - 1) / t.rows_per_team);
-  return t;
-}
-
-// Simple form: one row at a time, straight from global memory.
+// The column sums need one product a row and element: with c = sum over a
+// gate row's rows of dv f r_f, the gate's gradient is w_post c, and c times
+// the gate's row adds to dw_post.
 template <int WPR, int VPT>
-__global__ void __launch_bounds__(kBnThreads) block_norm_bwd_kernel(const BlockNormBwdParams p) {
-  constexpr int TEAMS = kBnWarps / WPR, TT = WPR * 32;
-  __shared__ float red[2][kBnWarps][4];
+__global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
+    block_norm_bwd_kernel(const BlockNormBwdParams p, const BlockNormTeams tm) {
+  constexpr int TT = WPR * 32, TEAMS = kBnWarps / WPR;
+  extern __shared__ uint4 bn_stages[];
+  __shared__ float4 red[2][kBnWarps];
+  __shared__ uint64_t bars[kBnWarps * kBnStages];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
   const int team_in_cta = (int)threadIdx.x / TT, tid = (int)threadIdx.x % TT;
   const int team = (int)blockIdx.x * TEAMS + team_in_cta;
-  if (team >= p.n_teams) return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
   const int nvec = p.cols / 8;
-  const int row0 = team * p.rows_per_team;
-  const int row1 = (int)min((long long)p.rows, (long long)row0 + p.rows_per_team);
+  const bool has_f = p.df && (p.w_post || p.gate);
+  BnRing<4> ring;
+  ring.src[0] = has_f ? p.f : nullptr;
+  ring.src[1] = p.w_pre ? p.y : nullptr;
+  ring.src[2] = p.dy;
+  ring.src[3] = p.w_pre ? p.dh : nullptr;
+  ring.present = (has_f ? 1 : 0) + (p.w_pre ? 2 : 0) + (p.dy ? 1 : 0);
+  ring.cols = p.cols, ring.rows_per_stage = tm.rows_per_stage;
+  ring.row0 = (int)min((long long)p.rows, (long long)team * tm.rows_per_team);  // past the last
+  ring.row1 = (int)min((long long)p.rows, (long long)ring.row0 + tm.rows_per_team);  // team: none
+  ring.step = tm.rows_per_stage;
+  ring.slot = (uint32_t)tm.rows_per_stage * p.cols * 2;
+  ring.stage = 4 * ring.slot;
+  ring.bar = smem_u32(bars + team_in_cta * kBnStages);
+  ring.data = smem_u32(bn_stages) + team_in_cta * kBnStages * ring.stage;
+  if (tid == 0)
+    for (int k = 0; k < kBnStages; ++k) ring.issue(k);
   int buf = 0;
   PhiloxState rng = {};
   if (p.drop.rng) rng = philox_state(p.drop);
-  const bool has_f = p.df && (p.w_post || p.gate);
-  float a_post[VPT][8], a_pre[VPT][8], a_gate[VPT][8];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a_post[i][e] = a_pre[i][e] = a_gate[i][e] = 0.0f;
+  const float inv_c = 1.0f / (float)p.cols;
+  const uint64_t rs2 = f2_make(p.residual_scale, p.residual_scale);
+  const uint64_t bs2 = f2_make(p.branch_scale, p.branch_scale);
 
-  int gate_row = row0 / p.rows_per_gate, gate_first = row0;  // this segment of the gate's rows
-  for (int row = row0; row < row1; ++row) {
-    const long long base = (long long)row * p.cols;
-    float s3[3] = {0.0f, 0.0f, 0.0f};  // y^2, dh w_pre y, f^2
+  uint64_t a_post[VPT][4], a_pre[VPT][4], a_c[VPT][4];
+  uint64_t wg[VPT][4];  // gate * w_post
+  uint4 wn[VPT];        // w_pre
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * TT;
+    wn[i] = p.w_pre && v < nvec ? reinterpret_cast<const uint4*>(p.w_pre)[v] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a_post[i][e] = a_pre[i][e] = a_c[i][e] = 0;
+  }
+  int gate_row = -1;
+  auto load_gate = [&](int g) {
+    gate_row = g;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * TT;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wg[i][e] = f2_make(1.0f, 1.0f);
+      if (v >= nvec) continue;
+      if (p.w_post) bn_unpack(reinterpret_cast<const uint4*>(p.w_post)[v], wg[i]);
+      if (p.gate) {
+        uint64_t g4[4];
+        bn_unpack(reinterpret_cast<const uint4*>(p.gate + (long long)g * p.cols)[v], g4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wg[i][e] = f2_mul(wg[i][e], g4[e]);
+      }
+    }
+  };
+  int gate_first = ring.row0;  // the first of this team's rows in the gate's row
+  if (has_f && ring.row0 < ring.row1) load_gate(ring.row0 / p.rows_per_gate);
+  // Hands over the sums of the gate row's rows up to `end` (exclusive).
+  auto flush = [&](int end) {
+    const bool whole = p.gate && gate_first == (long long)gate_row * p.rows_per_gate &&
+                       end == ((long long)gate_row + 1) * p.rows_per_gate;
+    // a segment that starts at the team's first row goes to slot 0
+    float* part = p.part_gate + ((long long)team * 2 + (gate_first == ring.row0 ? 0 : 1)) * p.cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = tid + i * TT;
       if (v < nvec) {
-        if (p.w_pre) {
-          float y8[8], d8[8], w8[8];
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.y + base)[v], y8);
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.dh + base)[v], d8);
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.w_pre)[v], w8);
+        uint64_t c4[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            s3[0] = fmaf(y8[e], y8[e], s3[0]);
-            s3[1] = fmaf(d8[e] * w8[e], y8[e], s3[1]);
-          }
-        }
-        if (has_f && p.w_post) {
-          float f8[8];
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.f + base)[v], f8);
+        for (int e = 0; e < 4; ++e) c4[e] = a_c[i][e];
+        if (p.gate) {
+          uint64_t g4[4], d4[4];
+          bn_unpack(reinterpret_cast<const uint4*>(p.gate + (long long)gate_row * p.cols)[v], g4);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s3[2] = fmaf(f8[e], f8[e], s3[2]);
-        }
-      }
-    }
-    team_sum<WPR, 3>(s3, &red, buf, team_in_cta, tid >> 5);
-    const float inv_c = 1.0f / (float)p.cols;
-    const float r_y = rsqrtf(s3[0] * inv_c + p.eps);
-    const float m_y = s3[1] * inv_c * r_y * r_y;  // mean(dh w_pre y) r_y^2
-    const float r_f = p.w_post ? rsqrtf(s3[2] * inv_c + p.eps) : 1.0f;
-    float q[VPT][8];
-    float s1[1] = {0.0f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = tid + i * TT;
-      if (v < nvec) {
-        float t[8];
-        if (p.dy) {
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.dy + base)[v], t);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) t[e] = 0.0f;
-        }
-        if (p.w_pre) {
-          float y8[8], d8[8], w8[8];
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.y + base)[v], y8);
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.dh + base)[v], d8);
-          bf16x8_to_f32(reinterpret_cast<const uint4*>(p.w_pre)[v], w8);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            a_pre[i][e] = fmaf(d8[e], y8[e] * r_y, a_pre[i][e]);
-            t[e] += r_y * (d8[e] * w8[e] - y8[e] * m_y);
-          }
-        }
-        if (p.df) {
-          float b[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) b[e] = p.branch_scale * t[e];
-          if (p.drop.rng) dropout8(p.drop, rng, (uint32_t)(base / 8 + v), b);
-          if (has_f) {
-            float n[8], w8[8], g8[8];
-            bf16x8_to_f32(reinterpret_cast<const uint4*>(p.f + base)[v], n);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              n[e] *= r_f;
-              w8[e] = g8[e] = 1.0f;
-            }
-            if (p.w_post) bf16x8_to_f32(reinterpret_cast<const uint4*>(p.w_post)[v], w8);
-            if (p.gate) {
-              bf16x8_to_f32(
-                  reinterpret_cast<const uint4*>(p.gate + (long long)gate_row * p.cols)[v], g8);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) a_gate[i][e] = fmaf(b[e], n[e] * w8[e], a_gate[i][e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              b[e] *= g8[e];
-              a_post[i][e] = fmaf(b[e], n[e], a_post[i][e]);
-              b[e] *= w8[e];
-              s1[0] = fmaf(b[e], n[e], s1[0]);
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q[i][e] = b[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] *= p.residual_scale;
-        reinterpret_cast<uint4*>(p.dx + base)[v] = f32_to_bf16x8(t);
-      }
-    }
-    if (p.df) {
-      if (p.w_post) team_sum<WPR, 1>(s1, &red, buf, team_in_cta, tid >> 5);
-      const float m_f = s1[0] * inv_c * r_f;  // mean(q w_post n) r_f
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = tid + i * TT;
-        if (v < nvec) {
+          for (int e = 0; e < 4; ++e) d4[e] = c4[e];
           if (p.w_post) {
-            float f8[8];
-            bf16x8_to_f32(reinterpret_cast<const uint4*>(p.f + base)[v], f8);
+            uint64_t w4[4];
+            bn_unpack(reinterpret_cast<const uint4*>(p.w_post)[v], w4);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[i][e] = r_f * (q[i][e] - f8[e] * m_f);
+            for (int e = 0; e < 4; ++e) d4[e] = f2_mul(d4[e], w4[e]);
           }
-          reinterpret_cast<uint4*>(p.df + base)[v] = f32_to_bf16x8(q[i]);
+          if (whole)
+            reinterpret_cast<uint4*>(p.dgate + (long long)gate_row * p.cols)[v] = bn_pack(d4);
+          else
+            bn_store_f32(part, v, d4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c4[e] = f2_mul(c4[e], g4[e]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a_post[i][e] = f2_add(a_post[i][e], c4[e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a_c[i][e] = 0;
     }
-    if (p.gate && p.df) {
-      // the last row of the gate's rows, or of this team's: hand over the sum
-      const long long gate_end = ((long long)gate_row + 1) * p.rows_per_gate;
-      if (row + 1 == gate_end || row + 1 == row1) {
-        const bool whole =
-            gate_first == (long long)gate_row * p.rows_per_gate && row + 1 == gate_end;
-        // a segment that starts at the team's first row goes to slot 0
-        float* part = p.part_gate +
-                      ((long long)team * 2 + (gate_first == row0 ? 0 : 1)) * p.cols;
+    gate_first = end;
+  };
+
+  int k = 0;
+  for (int r = ring.row0; r < ring.row1; r += tm.rows_per_stage, ++k) {
+    ring.wait(k, abort_flag, 943);
+    const int here = min(tm.rows_per_stage, ring.row1 - r);
+    for (int j = 0; j < here; ++j) {
+      const int row = r + j;
+      const long long base = (long long)row * p.cols;
+      const uint32_t fa = ring.at(k, 0, j), ya = ring.at(k, 1, j), ga = ring.at(k, 2, j),
+                     ha = ring.at(k, 3, j);
+      float s3[3] = {0.0f, 0.0f, 0.0f};  // y^2, dh w_pre y, f^2
+      {
+        uint64_t a0 = 0, a1 = 0, a2 = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const int v = tid + i * TT;
           if (v < nvec) {
-            if (whole) {
-              reinterpret_cast<uint4*>(p.dgate + (long long)gate_row * p.cols)[v] =
-                  f32_to_bf16x8(a_gate[i]);
-            } else {
-              reinterpret_cast<float4*>(part)[2 * v] =
-                  make_float4(a_gate[i][0], a_gate[i][1], a_gate[i][2], a_gate[i][3]);
-              reinterpret_cast<float4*>(part)[2 * v + 1] =
-                  make_float4(a_gate[i][4], a_gate[i][5], a_gate[i][6], a_gate[i][7]);
+            if (p.w_pre) {
+              uint64_t y4[4], d4[4], w4[4];
+              bn_unpack(bn_lds(ya + v * 16), y4);
+              bn_unpack(bn_lds(ha + v * 16), d4);
+              bn_unpack(wn[i], w4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                a0 = f2_fma(y4[e], y4[e], a0);
+                a1 = f2_fma(f2_mul(d4[e], w4[e]), y4[e], a1);
+              }
+            }
+            if (has_f && p.w_post) {
+              uint64_t f4[4];
+              bn_unpack(bn_lds(fa + v * 16), f4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a2 = f2_fma(f4[e], f4[e], a2);
             }
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a_gate[i][e] = 0.0f;
         }
-        ++gate_row;
-        gate_first = row + 1;
+        s3[0] = bn_hsum(a0), s3[1] = bn_hsum(a1), s3[2] = bn_hsum(a2);
+      }
+      if (p.w_pre || p.w_post) team_sum<WPR, 3>(s3, red, buf, team_in_cta, tid >> 5);
+      const float r_y = rsqrtf(s3[0] * inv_c + p.eps);
+      const float m_y = -(s3[1] * inv_c) * r_y * r_y * r_y;  // -r_y^3 mean(dh w_pre y)
+      const float r_f = p.w_post ? rsqrtf(s3[2] * inv_c + p.eps) : 1.0f;
+      const uint64_t ry2 = f2_make(r_y, r_y), my2 = f2_make(m_y, m_y), rf2 = f2_make(r_f, r_f);
+      uint64_t q[VPT][4], s1p = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = tid + i * TT;
+        if (v < nvec) {
+          uint64_t t[4];
+          if (p.dy) {
+            bn_unpack(bn_lds(ga + v * 16), t);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = 0;
+          }
+          if (p.w_pre) {
+            uint64_t y4[4], d4[4], w4[4];
+            bn_unpack(bn_lds(ya + v * 16), y4);
+            bn_unpack(bn_lds(ha + v * 16), d4);
+            bn_unpack(wn[i], w4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t dr = f2_mul(d4[e], ry2);
+              a_pre[i][e] = f2_fma(dr, y4[e], a_pre[i][e]);
+              t[e] = f2_fma(dr, w4[e], f2_fma(y4[e], my2, t[e]));
+            }
+          }
+          if (p.df) {
+            uint64_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = f2_mul(t[e], bs2);
+            if (p.drop.rng) bn_dropout(p.drop, rng, (uint32_t)(base / 8 + v), b);
+            if (has_f) {
+              uint64_t n[4];
+              bn_unpack(bn_lds(fa + v * 16), n);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                n[e] = f2_mul(n[e], rf2);
+                a_c[i][e] = f2_fma(b[e], n[e], a_c[i][e]);
+                b[e] = f2_mul(b[e], wg[i][e]);
+                s1p = f2_fma(b[e], n[e], s1p);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[i][e] = b[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = f2_mul(t[e], rs2);
+          reinterpret_cast<uint4*>(p.dx + base)[v] = bn_pack(t);
+        }
+      }
+      if (p.df) {
+        if (p.w_post) {
+          float s1[1] = {bn_hsum(s1p)};
+          team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
+          const float m_f = -(s1[0] * inv_c) * r_f * r_f;  // -r_f mean(q w_post n), times r_f f
+          const uint64_t mf2 = f2_make(m_f, m_f);
+#pragma unroll
+          for (int i = 0; i < VPT; ++i) {
+            const int v = tid + i * TT;
+            if (v < nvec) {
+              uint64_t f4[4];
+              bn_unpack(bn_lds(fa + v * 16), f4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[i][e] = f2_fma(q[i][e], rf2, f2_mul(f4[e], mf2));
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+          if (tid + i * TT < nvec)
+            reinterpret_cast<uint4*>(p.df + base)[tid + i * TT] = bn_pack(q[i]);
+      }
+      if (p.gate && has_f) {
+        const long long gate_end = ((long long)gate_row + 1) * p.rows_per_gate;
+        if (row + 1 == gate_end) {
+          flush(row + 1);
+          if (row + 1 < ring.row1) load_gate(gate_row + 1);
+        }
       }
     }
+    team_sync<WPR>(team_in_cta);  // every thread has read the stage
+    if (tid == 0) ring.issue(k + kBnStages);
   }
+  if (*abort_flag && tid == 0)  // copies in flight land before the shared memory goes away
+    for (int u = max(0, k - kBnStages); u < k; ++u) ring.wait(u, nullptr, 944);
+  if (has_f && gate_first < ring.row1) flush(ring.row1);
+
+  // the weights' sums: the CTA's teams joined in order through the (idle) stages
+  if constexpr (TEAMS > 1) {
+    float* sums = reinterpret_cast<float*>(bn_stages);  // [TEAMS][cols]
+    for (int which = 0; which < 2; ++which) {
+      if (which == 0 ? !(p.df && p.w_post) : !p.w_pre) continue;
+      __syncthreads();
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = tid + i * TT;
-    if (v < nvec) {
-      if (p.df && p.w_post) {
-        float4* d = reinterpret_cast<float4*>(p.part_post + (long long)team * p.cols);
-        d[2 * v] = make_float4(a_post[i][0], a_post[i][1], a_post[i][2], a_post[i][3]);
-        d[2 * v + 1] = make_float4(a_post[i][4], a_post[i][5], a_post[i][6], a_post[i][7]);
+      for (int i = 0; i < VPT; ++i) {
+        const int v = tid + i * TT;
+        if (v < nvec)
+          bn_store_f32(sums + (long long)team_in_cta * p.cols, v, which == 0 ? a_post[i] : a_pre[i]);
       }
-      if (p.w_pre) {
-        float4* d = reinterpret_cast<float4*>(p.part_pre + (long long)team * p.cols);
-        d[2 * v] = make_float4(a_pre[i][0], a_pre[i][1], a_pre[i][2], a_pre[i][3]);
-        d[2 * v + 1] = make_float4(a_pre[i][4], a_pre[i][5], a_pre[i][6], a_pre[i][7]);
+      __syncthreads();
+      float* dst = (which == 0 ? p.part_post : p.part_pre) + (long long)blockIdx.x * p.cols;
+      for (int c = threadIdx.x; c < p.cols; c += kBnThreads) {
+        float t = sums[c];
+#pragma unroll
+        for (int w = 1; w < TEAMS; ++w) t += sums[w * p.cols + c];
+        dst[c] = t;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * TT;
+      if (v < nvec) {
+        if (p.df && p.w_post) bn_store_f32(p.part_post + (long long)blockIdx.x * p.cols, v, a_post[i]);
+        if (p.w_pre) bn_store_f32(p.part_pre + (long long)blockIdx.x * p.cols, v, a_pre[i]);
       }
     }
   }
 }
 
-// Sums the teams' partials: output 0 is dw_post, 1 is dw_pre, 2 + g the gate's
-// row g where more than one team has rows of it.  32 columns a block, eight
-// strided partial sums a column, joined in a fixed order.
+// Sums the partials: output 0 is dw_post, 1 is dw_pre (a partial a CTA), 2 + g
+// the gate's row g where more than one team has rows of it (a partial a team).
+// 32 columns a block, 32 strided partial sums a column, joined in a fixed order.
 struct BlockNormSumParams {
   const float* part_post;
   const float* part_pre;
@@ -386,18 +650,18 @@ struct BlockNormSumParams {
   __nv_bfloat16* dw_post;
   __nv_bfloat16* dw_pre;
   __nv_bfloat16* dgate;  // null: no gate, or every gate row is one team's
-  int cols, n_teams, rows_per_team, rows_per_gate, gate_rows;
+  int cols, n_ctas, rows_per_team, rows_per_gate, gate_rows;
 };
 
-__global__ void __launch_bounds__(256) block_norm_sum_kernel(const BlockNormSumParams p) {
-  __shared__ float s[8][32];
+__global__ void __launch_bounds__(1024) block_norm_sum_kernel(const BlockNormSumParams p) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int col = (int)blockIdx.x * 32 + lane;
   const int outs = 2 + (p.dgate ? p.gate_rows : 0);
   for (int o = blockIdx.y; o < outs; o += gridDim.y) {
     const float* src;
     __nv_bfloat16* dst;
-    int t0 = 0, t1 = p.n_teams - 1;
+    int t0 = 0, t1 = p.n_ctas - 1;
     const int g = o - 2;
     if (o == 0) {
       src = p.part_post, dst = p.dw_post;
@@ -413,12 +677,11 @@ __global__ void __launch_bounds__(256) block_norm_sum_kernel(const BlockNormSumP
     float acc = 0.0f;
     if (col < p.cols) {
 #pragma unroll 4
-      for (int t = t0 + part; t <= t1; t += 8) {
+      for (int t = t0 + part; t <= t1; t += 32) {
         long long at = t;
         if (o >= 2) {
           // slot 0 unless the segment starts inside the team's rows
-          const bool inside =
-              (long long)g * p.rows_per_gate > (long long)t * p.rows_per_team;
+          const bool inside = (long long)g * p.rows_per_gate > (long long)t * p.rows_per_team;
           at = 2LL * t + (inside ? 1 : 0);
         }
         acc += src[at * p.cols + col];
@@ -426,11 +689,12 @@ __global__ void __launch_bounds__(256) block_norm_sum_kernel(const BlockNormSumP
     }
     s[part][lane] = acc;
     __syncthreads();
-    if (part == 0 && col < p.cols) {
+    // warp w sums column w of the block's 32
+    acc = s[lane][part];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) acc += s[k][lane];
-      dst[col] = __float2bfloat16_rn(acc);
-    }
+    for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+    const int c = (int)blockIdx.x * 32 + part;
+    if (lane == 0 && c < p.cols) dst[c] = __float2bfloat16_rn(acc);
     __syncthreads();
   }
 }

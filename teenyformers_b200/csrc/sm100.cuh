@@ -144,6 +144,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
+// Untiled bulk copy into shared memory (16-byte aligned addresses and size).
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_dst),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
 // Bulk async copies out of shared memory (TMA stores / reduce-adds) and the
 // shared-memory stores that feed them.
 // TMA tensor store of a shared-memory tile (layout as the map's swizzle) to

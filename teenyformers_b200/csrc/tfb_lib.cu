@@ -159,6 +159,21 @@ int ensure_device_setup() {
     set((const void*)ffn_token_kernel<32, false>, TokCfg<32>::SMEM_ALLOC);
     set((const void*)ffn_token_kernel<64, false>, TokCfg<64>::SMEM_ALLOC);
     set((const void*)ffn_token_kernel<128, false>, TokCfg<128>::SMEM_ALLOC);
+    set((const void*)dropout_kernel<__nv_bfloat16>, kDropSmem);
+    set((const void*)dropout_kernel<float>, kDropSmem);
+    // 8192 columns: one row a stage of three
+    const int bn_fwd = kBnStages * 2 * kBnMaxCols * 2, bn_bwd = kBnStages * 4 * kBnMaxCols * 2;
+    static_assert(kBnStages * 4 * kBnMaxCols * 2 <= 227 * 1024 - 2048, "block norm's ring");
+#define TFB_BN_SET(W, V)                                                              \
+  set((const void*)block_norm_fwd_kernel<W, V>, std::max(bn_fwd, kBnRingBytes));      \
+  set((const void*)block_norm_bwd_kernel<W, V>, std::max(bn_bwd, kBnRingBytes))
+    TFB_BN_SET(1, 1);
+    TFB_BN_SET(1, 2);
+    TFB_BN_SET(2, 2);
+    TFB_BN_SET(4, 2);
+    TFB_BN_SET(8, 2);
+    TFB_BN_SET(8, 4);
+#undef TFB_BN_SET
     // CTA pairs that fit at once (SMs pair up within a GPC; one CTA per SM)
     g_pair_clusters[dev] = g_num_sms[dev] / 2;
     if (e == cudaSuccess) {
@@ -1273,10 +1288,11 @@ extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const v
   p.h = static_cast<__nv_bfloat16*>(h);
   p.rows = rows, p.cols = cols, p.rows_per_gate = gate ? rows / gate_rows : 1;
   p.eps = eps, p.residual_scale = residual_scale, p.branch_scale = branch_scale;
-  const BlockNormTeams t = block_norm_teams(rows, cols);
-  const unsigned grid = (unsigned)(((long long)rows * t.wpr + kBnWarps - 1) / kBnWarps);
-#define TFB_BN_FWD(W, V) \
-  block_norm_fwd_kernel<W, V><<<grid, kBnThreads, 0, static_cast<cudaStream_t>(stream)>>>(p)
+  if (int e = ensure_device_setup()) return e;
+  const BlockNormTeams t = block_norm_teams(rows, cols, 2);
+#define TFB_BN_FWD(W, V)                                                   \
+  block_norm_fwd_kernel<W, V><<<(unsigned)t.n_ctas, kBnThreads, t.smem,    \
+                                static_cast<cudaStream_t>(stream)>>>(p, t)
   TFB_BN_DISPATCH(t, TFB_BN_FWD);
 #undef TFB_BN_FWD
   return launch_status();
@@ -1284,8 +1300,9 @@ extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const v
 
 extern "C" size_t tf_b200_block_norm_bwd_workspace_size(int rows, int cols) {
   if (rows <= 0 || cols <= 0 || cols % 8 != 0 || cols > kBnMaxCols) return 0;
-  // two weights' and two gate segments' fp32 sums a team
-  return (size_t)block_norm_teams(rows, cols).n_teams * cols * 4 * 4;
+  // fp32 sums: two weights' a CTA, two gate segments' a team
+  const BlockNormTeams t = block_norm_teams(rows, cols, 4);
+  return ((size_t)t.n_ctas + t.n_teams) * 2 * cols * 4;
 }
 
 extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const void* dy,
@@ -1330,13 +1347,13 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   p.dgate = static_cast<__nv_bfloat16*>(dgate);
   p.rows = rows, p.cols = cols, p.rows_per_gate = gate ? rows / gate_rows : 1;
   p.eps = eps, p.residual_scale = residual_scale, p.branch_scale = branch_scale;
-  const BlockNormTeams t = block_norm_teams(rows, cols);
-  p.rows_per_team = t.rows_per_team, p.n_teams = t.n_teams;
+  if (int e = ensure_device_setup()) return e;
+  const BlockNormTeams t = block_norm_teams(rows, cols, 4);
   p.part_post = static_cast<float*>(workspace);
-  p.part_pre = p.part_post + (size_t)t.n_teams * cols;
-  p.part_gate = p.part_pre + (size_t)t.n_teams * cols;
-  const unsigned grid = (unsigned)((t.n_teams * t.wpr + kBnWarps - 1) / kBnWarps);
-#define TFB_BN_BWD(W, V) block_norm_bwd_kernel<W, V><<<grid, kBnThreads, 0, st>>>(p)
+  p.part_pre = p.part_post + (size_t)t.n_ctas * cols;
+  p.part_gate = p.part_pre + (size_t)t.n_ctas * cols;
+#define TFB_BN_BWD(W, V) \
+  block_norm_bwd_kernel<W, V><<<(unsigned)t.n_ctas, kBnThreads, t.smem, st>>>(p, t)
   TFB_BN_DISPATCH(t, TFB_BN_BWD);
 #undef TFB_BN_BWD
   if (int e = launch_status()) return e;
@@ -1346,11 +1363,11 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   s.dw_post = w_post ? static_cast<__nv_bfloat16*>(dw_post) : nullptr;
   s.dw_pre = w_pre ? static_cast<__nv_bfloat16*>(dw_pre) : nullptr;
   s.dgate = gate && p.rows_per_gate > 1 ? p.dgate : nullptr;  // one row a gate: written already
-  s.cols = cols, s.n_teams = t.n_teams, s.rows_per_team = t.rows_per_team;
+  s.cols = cols, s.n_ctas = t.n_ctas, s.rows_per_team = t.rows_per_team;
   s.rows_per_gate = p.rows_per_gate, s.gate_rows = gate ? gate_rows : 0;
   const int outs = 2 + (s.dgate ? gate_rows : 0);
   const dim3 sgrid((unsigned)((cols + 31) / 32), (unsigned)std::min(outs, 1024));
-  block_norm_sum_kernel<<<sgrid, 256, 0, st>>>(s);
+  block_norm_sum_kernel<<<sgrid, 1024, 0, st>>>(s);
   return launch_status();
 }
 
@@ -1365,11 +1382,12 @@ int dropout_launch(const T* x, const T* residual, T* y, const void* rng, size_t 
   if (!x || !y) return TF_ERR_INVALID_ARG;
   if (!is_aligned(x, 16) || !is_aligned(residual, 16) || !is_aligned(y, 16))
     return TF_ERR_MISALIGNED;
-  if (n > (size_t)1 << 40) return TF_ERR_TOO_LARGE;
-  const size_t blocks = (n / 8 + 255) / 256;
-  const unsigned grid = (unsigned)std::max<size_t>(1, std::min<size_t>(blocks, 148 * 8));
-  dropout_kernel<T><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(x, residual, y,
-                                                                         (long long)n, d);
+  if (n > (size_t)1 << 35) return TF_ERR_TOO_LARGE;  // also without a generator
+  if (int e = ensure_device_setup()) return e;
+  const size_t chunks = (n * sizeof(T) + kDropChunkBytes - 1) / kDropChunkBytes;
+  const unsigned grid = (unsigned)std::min<size_t>(chunks, kDropCtas);
+  dropout_kernel<T><<<grid, 256, kDropSmem, static_cast<cudaStream_t>(stream)>>>(
+      x, residual, y, (long long)n, d);
   return launch_status();
 }
 

@@ -112,10 +112,10 @@ def test_block_norm_bwd_refusals(native_lib):
     assert norm_bwd(gr=5) == TF_ERR_INVALID_ARG
     size = lambda r, c: _capi.raw("tf_b200_block_norm_bwd_workspace_size", r, c)
     assert size(0, 64) == 0 and size(4, 12) == 0
-    assert size(1, 64) == 1 * 64 * 16
-    # at most 296 CTAs' teams, whatever the rows: four fp32 rows of columns each
-    assert size(1 << 30, 4096) <= 296 * 4096 * 16
-    assert size(1 << 30, 512) <= 296 * 8 * 512 * 16
+    assert size(1, 64) == (1 + 1) * 2 * 64 * 4
+    # at most 296 CTAs, whatever the rows: two fp32 rows of columns for each and its teams
+    assert size(1 << 30, 4096) <= 296 * (1 + 1) * 2 * 4096 * 4
+    assert size(1 << 30, 512) <= 296 * (1 + 8) * 2 * 512 * 4
 
 
 @pytest.mark.parametrize("fn", ["tf_b200_dropout_bf16", "tf_b200_dropout_f32"])
