@@ -60,6 +60,7 @@ struct BlockNormParams {
 // forward pass of 16384 x 4096 took 100 us and the backward pass 370 us, bound
 // by load latency (4.7 and more stalled cycles an instruction).
 constexpr int kBnStages = 3;
+constexpr int kBnRed = 4 * 24;       // team_sum: at most 4 teams of several warps
 constexpr int kBnCtas = 296;  // two CTAs on each of 148 SMs
 constexpr int kBnRingBytes = 98304;  // a CTA's stages, where a row is not longer
 
@@ -118,13 +119,13 @@ __device__ __forceinline__ float bn_hsum(uint64_t v) {
   f2_split(v, lo, hi);
   return lo + hi;
 }
-// Dropout of eight elements held as pairs.
-__device__ __forceinline__ void bn_dropout(const DropoutParams& d, const PhiloxState& s,
-                                           uint32_t group, uint64_t (&f)[4]) {
+// dropout_select8 of elements held as pairs.
+__device__ __forceinline__ void bn_select(const DropoutParams& d, const PhiloxState& s,
+                                          uint32_t group, uint64_t (&f)[4]) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) f2_split(f[i], v[2 * i], v[2 * i + 1]);
-  dropout8(d, s, group, v);
+  dropout_select8(d, s, group, v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = f2_make(v[2 * i], v[2 * i + 1]);
 }
@@ -176,45 +177,70 @@ __device__ __forceinline__ void team_sync(int team) {
     named_bar_sync(1 + team, WPR * 32);
 }
 
-// Sums NV <= 4 values over a team's threads.  `buf` alternates between calls:
-// a thread can only write buffer b again after the team's barrier of the call
-// in between, which every thread reaches after its reads of b.
+// Sums NV (1 or 3) values over a team's threads.  `buf` alternates between
+// calls: a thread can only write buffer b again after the team's barrier of
+// the call in between, which every thread reaches after its reads of b.
+// Instruction counts matter here (an eighth of the backward pass): three
+// values over a warp in 6 shuffles (lanes 0, 8, 16 end with one value each),
+// and the warps' sums in one load, 3 shuffles and a broadcast a value.
 template <int WPR, int NV>
-__device__ __forceinline__ void team_sum(float (&v)[NV], float4 (*red)[kBnWarps], int& buf,
-                                         int team, int warp_in_team) {
+__device__ __forceinline__ void team_sum(float (&v)[NV], float (*red)[kBnRed], int& buf, int team,
+                                         int warp_in_team) {
+  static_assert(NV == 1 || NV == 3, "one or three values");
+  constexpr unsigned ALL = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  if constexpr (WPR == 1) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-    for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  if constexpr (WPR > 1) {
-    float4* r = red[buf] + team * WPR;
-    buf ^= 1;
-    if ((threadIdx.x & 31) == 0)
-      r[warp_in_team] = make_float4(v[0], NV > 1 ? v[1 % NV] : 0.0f, NV > 2 ? v[2 % NV] : 0.0f, 0.0f);
-    named_bar_sync(1 + team, WPR * 32);
-    float4 t = r[0];
-#pragma unroll
-    for (int w = 1; w < WPR; ++w) {
-      const float4 a = r[w];
-      t.x += a.x;
-      if (NV > 1) t.y += a.y;
-      if (NV > 2) t.z += a.z;
+      for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(ALL, v[k], o);
+  } else {
+    float t;
+    if constexpr (NV == 3) {
+      const bool up = lane & 16, mid = lane & 8;
+      // the lower half keeps values 0 and 1, the upper half value 2
+      float a = up ? v[2] : v[0];
+      a += __shfl_xor_sync(ALL, up ? v[0] : v[2], 16);
+      float b = up ? 0.0f : v[1];
+      b += __shfl_xor_sync(ALL, up ? v[1] : 0.0f, 16);
+      t = mid ? b : a;
+      t += __shfl_xor_sync(ALL, mid ? a : b, 8);
+    } else {
+      t = v[0] + __shfl_xor_sync(ALL, v[0], 16);
+      t += __shfl_xor_sync(ALL, t, 8);
     }
-    v[0] = t.x;
-    if constexpr (NV > 1) v[1] = t.y;
-    if constexpr (NV > 2) v[2] = t.z;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
+    float* r = red[buf] + team * 24;  // 8 slots a value, WPR of them used
+    buf ^= 1;
+    if constexpr (NV == 3) {
+      if ((lane & 7) == 0 && lane < 24) r[lane + warp_in_team] = t;
+      named_bar_sync(1 + team, WPR * 32);
+      t = (lane < 24 && (lane & 7) < WPR) ? r[lane] : 0.0f;
+    } else {
+      if (lane == 0) r[warp_in_team] = t;
+      named_bar_sync(1 + team, WPR * 32);
+      t = (lane & 7) < WPR ? r[lane & 7] : 0.0f;
+    }
+#pragma unroll
+    for (int o = WPR / 2; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] = NV == 1 && WPR == 8 ? t : __shfl_sync(ALL, t, 8 * k);
   }
 }
 
 // ---------------------------------------------------------------- forward
-// VPT vectors a thread; the weights stay in registers over the team's rows
+// VPT vectors a thread; a vector past the row's end reads zeros from `zero`, so
+// that nothing but the stores is predicated.  ALL: f, w_post and w_pre are
+// given (a block's usual case: no branches on them).  The weights stay in registers over the team's rows
 // (gate * w_post as their fp32 product, renewed where the gate's row changes).
-template <int WPR, int VPT>
+template <int WPR, int VPT, bool ALL>
 __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
     block_norm_fwd_kernel(const BlockNormParams p, const BlockNormTeams tm) {
   constexpr int TT = WPR * 32;
   extern __shared__ uint4 bn_stages[];
-  __shared__ float4 red[2][kBnWarps];
+  __shared__ float red[2][kBnRed];
+  __shared__ uint4 zero_cell;
   __shared__ uint64_t bars[kBnWarps * kBnStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -223,11 +249,18 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_word = 0;
+    zero_cell = make_uint4(0, 0, 0, 0);
     fence_mbar_init();
   }
   __syncthreads();
   if (team >= tm.n_teams) return;  // whole teams leave: their barriers are their own
   const int nvec = p.cols / 8;
+  const bool has_f = ALL || p.f, post = ALL || (p.f && p.w_post), pre = ALL || p.w_pre;
+  const uint32_t zero = smem_u32(&zero_cell);
+  auto lds = [&](uint32_t row, int i) {
+    const int v = tid + i * TT;
+    return bn_lds(v < nvec ? row + v * 16 : zero);
+  };
   BnRing<2> ring;
   ring.src[0] = p.f, ring.src[1] = p.x;
   ring.present = p.f ? 2 : 1;
@@ -254,9 +287,10 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
     const int v = tid + i * TT;
     wn[i] = p.w_pre && v < nvec ? reinterpret_cast<const uint4*>(p.w_pre)[v] : make_uint4(0, 0, 0, 0);
   }
-  int gate_row = -1;
+  const float branch = p.branch_scale * (p.drop.rng ? p.drop.scale : 1.0f);
+  long long gate_end = 0;  // the first row of the next gate row
   auto load_gate = [&](int g) {
-    gate_row = g;
+    gate_end = ((long long)g + 1) * p.rows_per_gate;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = tid + i * TT;
@@ -272,7 +306,7 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
       }
     }
   };
-  if (p.f) load_gate(ring.row0 / p.rows_per_gate);
+  if (has_f) load_gate(ring.row0 / p.rows_per_gate);
 
   int k = 0;
   for (long long r = ring.row0; r < ring.row1; r += ring.step, ++k) {
@@ -283,44 +317,41 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
       const long long base = (long long)row * p.cols;
       const uint32_t fa = ring.at(k, 0, j), xa = ring.at(k, 1, j);
       float r_f = 1.0f;
-      if (p.f && p.w_post) {
+      if (post) {
         uint64_t ss = 0;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-          if (tid + i * TT < nvec) {
-            uint64_t a[4];
-            bn_unpack(bn_lds(fa + (tid + i * TT) * 16), a);
+        for (int i = 0; i < VPT; ++i) {
+          uint64_t a[4];
+          bn_unpack(lds(fa, i), a);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ss = f2_fma(a[e], a[e], ss);
-          }
+          for (int e = 0; e < 4; ++e) ss = f2_fma(a[e], a[e], ss);
+        }
         float s1[1] = {bn_hsum(ss)};
         team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
         r_f = rsqrtf(s1[0] * inv_c + p.eps);
       }
-      if (p.gate && row / p.rows_per_gate != gate_row) load_gate(row / p.rows_per_gate);
-      const float bf = p.branch_scale * r_f;
+      if (p.gate && row >= gate_end) load_gate(row / p.rows_per_gate);
+      const float bf = branch * r_f;
       const uint64_t bf2 = f2_make(bf, bf);
       uint64_t y[VPT][4], ssy = 0;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int v = tid + i * TT;
-        if (v < nvec) {
-          bn_unpack(bn_lds(xa + v * 16), y[i]);
-          if (p.f) {
-            uint64_t b[4];
-            bn_unpack(bn_lds(fa + v * 16), b);
+        bn_unpack(lds(xa, i), y[i]);
+        if (has_f) {
+          uint64_t b[4];
+          bn_unpack(lds(fa, i), b);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = f2_mul(b[e], wg[i][e]);
-            if (p.drop.rng) bn_dropout(p.drop, rng, (uint32_t)(base / 8 + v), b);
+          for (int e = 0; e < 4; ++e) b[e] = f2_mul(b[e], wg[i][e]);
+          if (p.drop.rng) bn_select(p.drop, rng, (uint32_t)(base / 8 + v), b);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[i][e] = f2_fma(b[e], bf2, f2_mul(y[i][e], rs2));
-            reinterpret_cast<uint4*>(p.y + base)[v] = bn_pack(y[i]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ssy = f2_fma(y[i][e], y[i][e], ssy);
+          for (int e = 0; e < 4; ++e) y[i][e] = f2_fma(b[e], bf2, f2_mul(y[i][e], rs2));
+          if (v < nvec) reinterpret_cast<uint4*>(p.y + base)[v] = bn_pack(y[i]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ssy = f2_fma(y[i][e], y[i][e], ssy);
       }
-      if (p.w_pre) {
+      if (pre) {
         float s1[1] = {bn_hsum(ssy)};
         team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
         const float r_y = rsqrtf(s1[0] * inv_c + p.eps);
@@ -328,13 +359,11 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const int v = tid + i * TT;
-          if (v < nvec) {
-            uint64_t w[4];
-            bn_unpack(wn[i], w);
+          uint64_t w[4];
+          bn_unpack(wn[i], w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = f2_mul(f2_mul(y[i][e], ry2), w[e]);
-            reinterpret_cast<uint4*>(p.h + base)[v] = bn_pack(w);
-          }
+          for (int e = 0; e < 4; ++e) w[e] = f2_mul(f2_mul(y[i][e], ry2), w[e]);
+          if (v < nvec) reinterpret_cast<uint4*>(p.h + base)[v] = bn_pack(w);
         }
       }
     }
@@ -361,6 +390,7 @@ struct BlockNormBwdParams {
   float* part_pre;              // [n_ctas, cols]
   float* part_gate;             // [n_teams, 2, cols]
   int rows, cols, rows_per_gate;
+  int cyclic;  // teams take rows in turn; 0: contiguous rows
   float eps, residual_scale, branch_scale;
   DropoutParams drop;
 };
@@ -368,12 +398,13 @@ struct BlockNormBwdParams {
 // The column sums need one product a row and element: with c = sum over a
 // gate row's rows of dv f r_f, the gate's gradient is w_post c, and c times
 // the gate's row adds to dw_post.
-template <int WPR, int VPT>
+template <int WPR, int VPT, bool ALL>
 __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
     block_norm_bwd_kernel(const BlockNormBwdParams p, const BlockNormTeams tm) {
   constexpr int TT = WPR * 32, TEAMS = kBnWarps / WPR;
   extern __shared__ uint4 bn_stages[];
-  __shared__ float4 red[2][kBnWarps];
+  __shared__ float red[2][kBnRed];
+  __shared__ uint4 zero_cell;
   __shared__ uint64_t bars[kBnWarps * kBnStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -382,11 +413,18 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_word = 0;
+    zero_cell = make_uint4(0, 0, 0, 0);
     fence_mbar_init();
   }
   __syncthreads();
   const int nvec = p.cols / 8;
-  const bool has_f = p.df && (p.w_post || p.gate);
+  const bool branch = ALL || p.df, post = ALL || p.w_post, pre = ALL || p.w_pre;
+  const bool has_f = ALL || (p.df && (p.w_post || p.gate)), has_dy = ALL || p.dy;
+  const uint32_t zero = smem_u32(&zero_cell);
+  auto lds = [&](uint32_t row, int i) {
+    const int v = tid + i * TT;
+    return bn_lds(v < nvec ? row + v * 16 : zero);
+  };
   BnRing<4> ring;
   ring.src[0] = has_f ? p.f : nullptr;
   ring.src[1] = p.w_pre ? p.y : nullptr;
@@ -394,9 +432,11 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
   ring.src[3] = p.w_pre ? p.dh : nullptr;
   ring.present = (has_f ? 1 : 0) + (p.w_pre ? 2 : 0) + (p.dy ? 1 : 0);
   ring.cols = p.cols, ring.rows_per_stage = tm.rows_per_stage;
-  ring.row0 = (int)min((long long)p.rows, (long long)team * tm.rows_per_team);  // past the last
-  ring.row1 = (int)min((long long)p.rows, (long long)ring.row0 + tm.rows_per_team);  // team: none
-  ring.step = tm.rows_per_stage;
+  // teams past the last have no rows
+  const long long start = (long long)team * (p.cyclic ? tm.rows_per_stage : tm.rows_per_team);
+  ring.row0 = team < tm.n_teams ? (int)start : p.rows;
+  ring.row1 = p.cyclic ? p.rows : (int)min((long long)p.rows, (long long)ring.row0 + tm.rows_per_team);
+  ring.step = p.cyclic ? (long long)tm.n_teams * tm.rows_per_stage : tm.rows_per_stage;
   ring.slot = (uint32_t)tm.rows_per_stage * p.cols * 2;
   ring.stage = 4 * ring.slot;
   ring.bar = smem_u32(bars + team_in_cta * kBnStages);
@@ -408,7 +448,8 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
   if (p.drop.rng) rng = philox_state(p.drop);
   const float inv_c = 1.0f / (float)p.cols;
   const uint64_t rs2 = f2_make(p.residual_scale, p.residual_scale);
-  const uint64_t bs2 = f2_make(p.branch_scale, p.branch_scale);
+  const float bs = p.branch_scale * (p.drop.rng ? p.drop.scale : 1.0f);
+  const uint64_t bs2 = f2_make(bs, bs);
 
   uint64_t a_post[VPT][4], a_pre[VPT][4], a_c[VPT][4];
   uint64_t wg[VPT][4];  // gate * w_post
@@ -420,9 +461,12 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) a_post[i][e] = a_pre[i][e] = a_c[i][e] = 0;
   }
-  int gate_row = -1;
-  auto load_gate = [&](int g) {
-    gate_row = g;
+  int gate_row = 0, seg_first = 0, seg_end = 0;  // this team's rows in the gate's row so far
+  long long gate_end = 0;                        // the first row of the next gate row
+  auto load_gate = [&](int row) {
+    const int g = row / p.rows_per_gate;
+    gate_row = g, seg_first = row;
+    gate_end = ((long long)g + 1) * p.rows_per_gate;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = tid + i * TT;
@@ -438,14 +482,14 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
       }
     }
   };
-  int gate_first = ring.row0;  // the first of this team's rows in the gate's row
-  if (has_f && ring.row0 < ring.row1) load_gate(ring.row0 / p.rows_per_gate);
-  // Hands over the sums of the gate row's rows up to `end` (exclusive).
-  auto flush = [&](int end) {
-    const bool whole = p.gate && gate_first == (long long)gate_row * p.rows_per_gate &&
-                       end == ((long long)gate_row + 1) * p.rows_per_gate;
+  if (has_f && ring.row0 < ring.row1) load_gate(ring.row0);
+  // Hands over the sums of a gate row's rows seg_first .. seg_end - 1.
+  auto flush = [&]() {
+    // (rows in turn with one gate for all: every team has a part of it)
+    const bool whole = p.gate && (!p.cyclic || p.rows_per_gate == 1) &&
+                       seg_first == (long long)gate_row * p.rows_per_gate && seg_end == gate_end;
     // a segment that starts at the team's first row goes to slot 0
-    float* part = p.part_gate + ((long long)team * 2 + (gate_first == ring.row0 ? 0 : 1)) * p.cols;
+    float* part = p.part_gate + ((long long)team * 2 + (seg_first == ring.row0 ? 0 : 1)) * p.cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = tid + i * TT;
@@ -477,114 +521,105 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) a_c[i][e] = 0;
     }
-    gate_first = end;
   };
 
   int k = 0;
-  for (int r = ring.row0; r < ring.row1; r += tm.rows_per_stage, ++k) {
+  for (long long r = ring.row0; r < ring.row1; r += ring.step, ++k) {
     ring.wait(k, abort_flag, 943);
-    const int here = min(tm.rows_per_stage, ring.row1 - r);
+    const int here = (int)min((long long)tm.rows_per_stage, ring.row1 - r);
     for (int j = 0; j < here; ++j) {
-      const int row = r + j;
+      const int row = (int)r + j;
       const long long base = (long long)row * p.cols;
       const uint32_t fa = ring.at(k, 0, j), ya = ring.at(k, 1, j), ga = ring.at(k, 2, j),
                      ha = ring.at(k, 3, j);
-      float s3[3] = {0.0f, 0.0f, 0.0f};  // y^2, dh w_pre y, f^2
+      if (p.gate && has_f && row >= gate_end) {
+        flush();
+        load_gate(row);
+      }
+      seg_end = row + 1;
+      float s3[3];  // y^2, dh w_pre y, f^2
       {
         uint64_t a0 = 0, a1 = 0, a2 = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-          const int v = tid + i * TT;
-          if (v < nvec) {
-            if (p.w_pre) {
-              uint64_t y4[4], d4[4], w4[4];
-              bn_unpack(bn_lds(ya + v * 16), y4);
-              bn_unpack(bn_lds(ha + v * 16), d4);
-              bn_unpack(wn[i], w4);
+          if (pre) {
+            uint64_t y4[4], d4[4], w4[4];
+            bn_unpack(lds(ya, i), y4);
+            bn_unpack(lds(ha, i), d4);
+            bn_unpack(wn[i], w4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                a0 = f2_fma(y4[e], y4[e], a0);
-                a1 = f2_fma(f2_mul(d4[e], w4[e]), y4[e], a1);
-              }
+            for (int e = 0; e < 4; ++e) {
+              a0 = f2_fma(y4[e], y4[e], a0);
+              a1 = f2_fma(f2_mul(d4[e], w4[e]), y4[e], a1);
             }
-            if (has_f && p.w_post) {
-              uint64_t f4[4];
-              bn_unpack(bn_lds(fa + v * 16), f4);
+          }
+          if (has_f && post) {
+            uint64_t f4[4];
+            bn_unpack(lds(fa, i), f4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) a2 = f2_fma(f4[e], f4[e], a2);
-            }
+            for (int e = 0; e < 4; ++e) a2 = f2_fma(f4[e], f4[e], a2);
           }
         }
         s3[0] = bn_hsum(a0), s3[1] = bn_hsum(a1), s3[2] = bn_hsum(a2);
       }
-      if (p.w_pre || p.w_post) team_sum<WPR, 3>(s3, red, buf, team_in_cta, tid >> 5);
+      if (pre || post) team_sum<WPR, 3>(s3, red, buf, team_in_cta, tid >> 5);
       const float r_y = rsqrtf(s3[0] * inv_c + p.eps);
       const float m_y = -(s3[1] * inv_c) * r_y * r_y * r_y;  // -r_y^3 mean(dh w_pre y)
-      const float r_f = p.w_post ? rsqrtf(s3[2] * inv_c + p.eps) : 1.0f;
+      const float r_f = post ? rsqrtf(s3[2] * inv_c + p.eps) : 1.0f;
       const uint64_t ry2 = f2_make(r_y, r_y), my2 = f2_make(m_y, m_y), rf2 = f2_make(r_f, r_f);
       uint64_t q[VPT][4], s1p = 0;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int v = tid + i * TT;
-        if (v < nvec) {
-          uint64_t t[4];
-          if (p.dy) {
-            bn_unpack(bn_lds(ga + v * 16), t);
-          } else {
+        uint64_t t[4] = {0, 0, 0, 0};
+        if (has_dy) bn_unpack(lds(ga, i), t);
+        if (pre) {
+          uint64_t y4[4], d4[4], w4[4];
+          bn_unpack(lds(ya, i), y4);
+          bn_unpack(lds(ha, i), d4);
+          bn_unpack(wn[i], w4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = 0;
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t dr = f2_mul(d4[e], ry2);
+            a_pre[i][e] = f2_fma(dr, y4[e], a_pre[i][e]);
+            t[e] = f2_fma(dr, w4[e], f2_fma(y4[e], my2, t[e]));
           }
-          if (p.w_pre) {
-            uint64_t y4[4], d4[4], w4[4];
-            bn_unpack(bn_lds(ya + v * 16), y4);
-            bn_unpack(bn_lds(ha + v * 16), d4);
-            bn_unpack(wn[i], w4);
+        }
+        if (branch) {
+          uint64_t b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = f2_mul(t[e], bs2);
+          if (p.drop.rng) bn_select(p.drop, rng, (uint32_t)(base / 8 + v), b);
+          if (has_f) {
+            uint64_t n[4];
+            bn_unpack(lds(fa, i), n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t dr = f2_mul(d4[e], ry2);
-              a_pre[i][e] = f2_fma(dr, y4[e], a_pre[i][e]);
-              t[e] = f2_fma(dr, w4[e], f2_fma(y4[e], my2, t[e]));
+              n[e] = f2_mul(n[e], rf2);
+              a_c[i][e] = f2_fma(b[e], n[e], a_c[i][e]);
+              b[e] = f2_mul(b[e], wg[i][e]);
+              s1p = f2_fma(b[e], n[e], s1p);
             }
           }
-          if (p.df) {
-            uint64_t b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = f2_mul(t[e], bs2);
-            if (p.drop.rng) bn_dropout(p.drop, rng, (uint32_t)(base / 8 + v), b);
-            if (has_f) {
-              uint64_t n[4];
-              bn_unpack(bn_lds(fa + v * 16), n);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                n[e] = f2_mul(n[e], rf2);
-                a_c[i][e] = f2_fma(b[e], n[e], a_c[i][e]);
-                b[e] = f2_mul(b[e], wg[i][e]);
-                s1p = f2_fma(b[e], n[e], s1p);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[i][e] = b[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = f2_mul(t[e], rs2);
-          reinterpret_cast<uint4*>(p.dx + base)[v] = bn_pack(t);
+          for (int e = 0; e < 4; ++e) q[i][e] = b[e];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = f2_mul(t[e], rs2);
+        if (v < nvec) reinterpret_cast<uint4*>(p.dx + base)[v] = bn_pack(t);
       }
-      if (p.df) {
-        if (p.w_post) {
+      if (branch) {
+        if (post) {
           float s1[1] = {bn_hsum(s1p)};
           team_sum<WPR, 1>(s1, red, buf, team_in_cta, tid >> 5);
           const float m_f = -(s1[0] * inv_c) * r_f * r_f;  // -r_f mean(q w_post n), times r_f f
           const uint64_t mf2 = f2_make(m_f, m_f);
 #pragma unroll
           for (int i = 0; i < VPT; ++i) {
-            const int v = tid + i * TT;
-            if (v < nvec) {
-              uint64_t f4[4];
-              bn_unpack(bn_lds(fa + v * 16), f4);
+            uint64_t f4[4];
+            bn_unpack(lds(fa, i), f4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) q[i][e] = f2_fma(q[i][e], rf2, f2_mul(f4[e], mf2));
-            }
+            for (int e = 0; e < 4; ++e) q[i][e] = f2_fma(q[i][e], rf2, f2_mul(f4[e], mf2));
           }
         }
 #pragma unroll
@@ -592,20 +627,13 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
           if (tid + i * TT < nvec)
             reinterpret_cast<uint4*>(p.df + base)[tid + i * TT] = bn_pack(q[i]);
       }
-      if (p.gate && has_f) {
-        const long long gate_end = ((long long)gate_row + 1) * p.rows_per_gate;
-        if (row + 1 == gate_end) {
-          flush(row + 1);
-          if (row + 1 < ring.row1) load_gate(gate_row + 1);
-        }
-      }
     }
     team_sync<WPR>(team_in_cta);  // every thread has read the stage
     if (tid == 0) ring.issue(k + kBnStages);
   }
   if (*abort_flag && tid == 0)  // copies in flight land before the shared memory goes away
     for (int u = max(0, k - kBnStages); u < k; ++u) ring.wait(u, nullptr, 944);
-  if (has_f && gate_first < ring.row1) flush(ring.row1);
+  if (has_f && ring.row0 < ring.row1) flush();
 
   // the weights' sums: the CTA's teams joined in order through the (idle) stages
   if constexpr (TEAMS > 1) {

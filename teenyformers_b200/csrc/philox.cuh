@@ -23,10 +23,10 @@
 namespace tfb {
 
 struct DropoutParams {
-  const unsigned long long* rng;  // device: seed, offset (null: no dropout)
+  const unsigned long long* rng;  // device: seed, offset (null: nothing is dropped)
   unsigned site;
-  unsigned threshold;  // t, 0 .. 65536
-  float scale;         // 65536 / t (0 when t == 0: everything is dropped)
+  unsigned limit;  // t << 16, t = 0 .. 65535 (t = 65536 drops nothing: no rng)
+  float scale;     // 65536 / t (0 when t == 0: everything is dropped)
 };
 
 struct PhiloxState {
@@ -60,18 +60,27 @@ __device__ __forceinline__ uint4 philox4x32_10(const PhiloxState& s, uint32_t gr
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Applies dropout to the eight elements of group g.  A dropped element is 0
-// whatever it held (a select, so an infinity or NaN that is dropped leaves no
-// NaN behind).
-__device__ __forceinline__ void dropout8(const DropoutParams& d, const PhiloxState& s,
-                                         uint32_t group, float (&v)[8]) {
+// Which of the eight elements of group g stay: the others become 0 whatever
+// they held (a select, so an infinity or NaN that is dropped leaves no NaN
+// behind).  The caller multiplies by d.scale.  A half is compared with t in
+// the upper 16 bits of a word: below a high half nothing can tip the compare.
+__device__ __forceinline__ void dropout_select8(const DropoutParams& d, const PhiloxState& s,
+                                                uint32_t group, float (&v)[8]) {
   const uint4 r = philox4x32_10(s, group);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t bits = (e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xffffu);
-    v[e] = bits < d.threshold ? v[e] * d.scale : 0.0f;
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = (w[i] << 16) < d.limit ? v[2 * i] : 0.0f;
+    v[2 * i + 1] = w[i] < d.limit ? v[2 * i + 1] : 0.0f;
   }
+}
+
+// ... and with the scale.
+__device__ __forceinline__ void dropout8(const DropoutParams& d, const PhiloxState& s,
+                                         uint32_t group, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= d.scale;
+  dropout_select8(d, s, group, v);
 }
 
 }  // namespace tfb

@@ -164,9 +164,11 @@ int ensure_device_setup() {
     // 8192 columns: one row a stage of three
     const int bn_fwd = kBnStages * 2 * kBnMaxCols * 2, bn_bwd = kBnStages * 4 * kBnMaxCols * 2;
     static_assert(kBnStages * 4 * kBnMaxCols * 2 <= 227 * 1024 - 2048, "block norm's ring");
-#define TFB_BN_SET(W, V)                                                              \
-  set((const void*)block_norm_fwd_kernel<W, V>, std::max(bn_fwd, kBnRingBytes));      \
-  set((const void*)block_norm_bwd_kernel<W, V>, std::max(bn_bwd, kBnRingBytes))
+#define TFB_BN_SET(W, V)                                                                  \
+  set((const void*)block_norm_fwd_kernel<W, V, true>, std::max(bn_fwd, kBnRingBytes));    \
+  set((const void*)block_norm_fwd_kernel<W, V, false>, std::max(bn_fwd, kBnRingBytes));   \
+  set((const void*)block_norm_bwd_kernel<W, V, true>, std::max(bn_bwd, kBnRingBytes));    \
+  set((const void*)block_norm_bwd_kernel<W, V, false>, std::max(bn_bwd, kBnRingBytes))
     TFB_BN_SET(1, 1);
     TFB_BN_SET(1, 2);
     TFB_BN_SET(2, 2);
@@ -1233,10 +1235,12 @@ int dropout_params(DropoutParams& d, const void* rng, float p, unsigned site, si
   if (!rng) return TF_ERR_INVALID_ARG;
   if (!is_aligned(rng, 8)) return TF_ERR_MISALIGNED;
   if (n > (size_t)1 << 35) return TF_ERR_TOO_LARGE;  // a group's index is 32 bits of the counter
+  const unsigned t = (unsigned)std::floor((1.0 - (double)p) * 65536.0 + 0.5);
+  if (t == 65536) return TF_OK;  // rounds to no dropout
   d.rng = static_cast<const unsigned long long*>(rng);
   d.site = site;
-  d.threshold = (unsigned)std::floor((1.0 - (double)p) * 65536.0 + 0.5);
-  d.scale = d.threshold ? (float)(65536.0 / d.threshold) : 0.0f;
+  d.limit = t << 16;
+  d.scale = t ? (float)(65536.0 / t) : 0.0f;
   return TF_OK;
 }
 
@@ -1251,15 +1255,20 @@ int block_norm_check(int rows, int cols, bool gate, int gate_rows, float eps, fl
   return TF_OK;
 }
 
-// One launch of a kernel<WPR, VPT> by the shape's team size.
-#define TFB_BN_DISPATCH(T, LAUNCH)                                        \
+// One launch of a kernel<WPR, VPT, ALL> by the shape's team size.
+#define TFB_BN_DISPATCH_ALL(T, ALL, LAUNCH)                               \
   do {                                                                    \
-    if ((T).wpr == 1 && (T).vpt == 1) LAUNCH(1, 1);                       \
-    else if ((T).wpr == 1) LAUNCH(1, 2);                                  \
-    else if ((T).wpr == 2) LAUNCH(2, 2);                                  \
-    else if ((T).wpr == 4) LAUNCH(4, 2);                                  \
-    else if ((T).vpt == 2) LAUNCH(8, 2);                                  \
-    else LAUNCH(8, 4);                                                    \
+    if ((T).wpr == 1 && (T).vpt == 1) LAUNCH(1, 1, ALL);                  \
+    else if ((T).wpr == 1) LAUNCH(1, 2, ALL);                             \
+    else if ((T).wpr == 2) LAUNCH(2, 2, ALL);                             \
+    else if ((T).wpr == 4) LAUNCH(4, 2, ALL);                             \
+    else if ((T).vpt == 2) LAUNCH(8, 2, ALL);                             \
+    else LAUNCH(8, 4, ALL);                                               \
+  } while (0)
+#define TFB_BN_DISPATCH(T, ALL, LAUNCH)               \
+  do {                                                \
+    if (ALL) TFB_BN_DISPATCH_ALL(T, true, LAUNCH);    \
+    else TFB_BN_DISPATCH_ALL(T, false, LAUNCH);       \
   } while (0)
 
 }  // namespace
@@ -1290,10 +1299,10 @@ extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const v
   p.eps = eps, p.residual_scale = residual_scale, p.branch_scale = branch_scale;
   if (int e = ensure_device_setup()) return e;
   const BlockNormTeams t = block_norm_teams(rows, cols, 2);
-#define TFB_BN_FWD(W, V)                                                   \
-  block_norm_fwd_kernel<W, V><<<(unsigned)t.n_ctas, kBnThreads, t.smem,    \
-                                static_cast<cudaStream_t>(stream)>>>(p, t)
-  TFB_BN_DISPATCH(t, TFB_BN_FWD);
+#define TFB_BN_FWD(W, V, A)                                                 \
+  block_norm_fwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem,  \
+                                   static_cast<cudaStream_t>(stream)>>>(p, t)
+  TFB_BN_DISPATCH(t, f && w_post && w_pre, TFB_BN_FWD);
 #undef TFB_BN_FWD
   return launch_status();
 }
@@ -1352,9 +1361,10 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   p.part_post = static_cast<float*>(workspace);
   p.part_pre = p.part_post + (size_t)t.n_ctas * cols;
   p.part_gate = p.part_pre + (size_t)t.n_ctas * cols;
-#define TFB_BN_BWD(W, V) \
-  block_norm_bwd_kernel<W, V><<<(unsigned)t.n_ctas, kBnThreads, t.smem, st>>>(p, t)
-  TFB_BN_DISPATCH(t, TFB_BN_BWD);
+  p.cyclic = !gate || p.rows_per_gate == 1 || gate_rows == 1;
+#define TFB_BN_BWD(W, V, A) \
+  block_norm_bwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem, st>>>(p, t)
+  TFB_BN_DISPATCH(t, w_post && w_pre && dy && df, TFB_BN_BWD);
 #undef TFB_BN_BWD
   if (int e = launch_status()) return e;
   if (!w_post && !w_pre && !gate) return TF_OK;
