@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(1024) block_norm_sum_kernel(const BlockNormSum
     if (!dst) continue;  // the same for every thread of the block
     float acc = 0.0f;
     if (col < p.cols) {
-#pragma unroll 4
+#pragma unroll 8
       for (int t = t0 + part; t <= t1; t += 32) {
         long long at = t;
         if (o >= 2) {

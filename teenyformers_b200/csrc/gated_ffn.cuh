@@ -17,8 +17,8 @@
 //   ffn_pair_kernel    persistent CTA pairs (cta_group::2), 256 x 256 tiles;
 //                      the structure of gemm_sm100.cuh's kernel with operands
 //                      of either major and several products in one launch
-//   ffn_token_kernel   few tokens: the weight rows are the MMA's M, the tokens
-//                      its N; K is split over a cluster and joined through
+//   ffn_tile_kernel    small products (few tokens above all): 128 x 16..128
+//                      tiles, K split over a cluster and joined through
 //                      distributed shared memory
 #pragma once
 
@@ -68,7 +68,7 @@ __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope
   }
 }
 
-__device__ __forceinline__ float ffn_act_rt(int act, float g) {
+__device__ __forceinline__ float ffn_act_rt(int act, float g) {  // (uniform branches)
   if (act == FFN_ACT_SILU) return ffn_act<FFN_ACT_SILU>(g);
   if (act == FFN_ACT_GELU) return ffn_act<FFN_ACT_GELU>(g);
   return ffn_act<FFN_ACT_GELU_TANH>(g);
@@ -543,22 +543,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   }
 }
 
-// ===================================================================== few tokens
-// out[t, j] over a 128-row tile of weights (GLU: 64 gate rows and the 64 up
-// rows of the same outputs) and NT tokens: D[128, NT] = Wtile[128, K] X[NT, K]^T.
-// The block is bound by reading the weights once: a cluster of S CTAs takes
-// one tile, each a contiguous run of k-blocks through its own TMA ring, and
-// the S partial tiles are summed through distributed shared memory, always in
-// rank order, so results repeat bit for bit.
+// ===================================================================== small products
+// out[t, j] over tiles of 128 rows j of A (FFN_GLU: 64 gate rows and the 64 up
+// rows of the same outputs) and NT rows t of B: D[128, NT] = A[128, K] B[NT, K]^T,
+// one CTA a tile and up to three products in one launch.  With the weights as
+// A and a few tokens as B the block is bound by reading the weights once; with
+// more tokens these tiles are small enough to fill the SMs where 256 x 256 ones
+// are not.  A cluster of S CTAs takes one tile, each a contiguous run of
+// k-blocks through its own TMA ring; the S partial tiles are summed through
+// distributed shared memory, always in rank order, so results repeat bit for
+// bit.
 //   warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 move the accumulator
 //   from TMEM to shared memory; all warps join the partials.
-constexpr int kTokThreads = 192;
+constexpr int kTileThreads = 192;
 
 template <int NT>
-struct TokCfg {
-  static constexpr int W_BYTES = 128 * 64 * 2;
-  static constexpr int X_BYTES = NT * 64 * 2;
-  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
+struct TileCfg {
+  static constexpr int A_BYTES = 128 * 64 * 2;
+  static constexpr int B_BYTES = NT * 64 * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 3;
   static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
   static constexpr int SMEM_ALLOC = OFF_BAR + 256 + 1024;
@@ -566,15 +569,24 @@ struct TokCfg {
   static_assert(NT * 128 * 4 <= OFF_BAR, "the partial tile exceeds the ring");
 };
 
-struct TokParams {
-  int m;        // tokens
-  int n_out;    // outputs of a token: d_ff (GLU) or d_model
-  int n_kblk;   // k-blocks of 64
-  int act;      // GLU
-  int pdl;      // launched with programmatic stream serialization
-  __nv_bfloat16* out;             // [m, n_out]
-  float* z;                       // GLU: [m, 2 n_out] or null
-  const __nv_bfloat16* residual;  // [m, n_out] or null
+struct FfnTileProblem {
+  int J, T;      // rows of A (FFN_GLU: outputs, half of them) and of B
+  int n_tt, n_tiles, n_kblk;
+  int split;       // a cluster takes one tile and splits K; 0: a tile for each of its CTAs
+  int n_clusters;
+  int a_mn, b_mn;  // operand stored with its row index innermost (b_mn: NT >= 64)
+  int a_early;     // A is not written by the kernel before this one
+  __nv_bfloat16* out;             // [T, J]
+  const __nv_bfloat16* residual;  // FFN_STORE: [T, J] or null
+};
+
+struct FfnTileParams {
+  FfnTileProblem prob[kFfnMaxProblems];
+  int n_prob, act;
+  int pdl;  // launched with programmatic stream serialization
+  int F;
+  float* z;           // [T, 2F] (FFN_GLU: null if not saved)
+  __nv_bfloat16* dz;  // FFN_DGLU: [T, 2F]; prob[0].out is a
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
@@ -585,9 +597,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
   return v;
 }
 // Programmatic dependent launch: blocks until the kernels this one depends on
@@ -599,12 +614,108 @@ __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-template <int NT, bool GLU>
-__global__ void __launch_bounds__(kTokThreads)
-    ffn_token_kernel(const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_x, const TokParams p) {
-  using C = TokCfg<NT>;
-  constexpr int ROWS = GLU ? 64 : 128;  // outputs of a tile
+__device__ __forceinline__ void ffn_act_grad_rt(int act, float g, float& value, float& slope) {
+  if (act == FFN_ACT_SILU)
+    ffn_act_grad<FFN_ACT_SILU>(g, value, slope);
+  else if (act == FFN_ACT_GELU)
+    ffn_act_grad<FFN_ACT_GELU>(g, value, slope);
+  else
+    ffn_act_grad<FFN_ACT_GELU_TANH>(g, value, slope);
+}
+__device__ __forceinline__ uint2 ffn_pack4(const float (&v)[4]) {
+  return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+// What is done with four joined outputs v (FFN_GLU: and the four u beside
+// them) at row `row` of the output and column `col`.
+template <int MODE>
+__device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, const FfnTileProblem& q,
+                                               long long row, int col, float (&v)[4],
+                                               float (&u)[4]) {
+  if constexpr (MODE == FFN_GLU) {
+    if (p.z) {
+      float* z = p.z + row * 2 * p.F + col;
+      *reinterpret_cast<float4*>(z) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(z + p.F) = make_float4(u[0], u[1], u[2], u[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ffn_act_rt(p.act, v[i]) * u[i];
+  } else if constexpr (MODE == FFN_DGLU) {
+    const float* z = p.z + row * 2 * p.F + col;
+    const float4 g4 = *reinterpret_cast<const float4*>(z);
+    const float4 u4 = *reinterpret_cast<const float4*>(z + p.F);
+    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
+    float dg[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float value, slope;
+      ffn_act_grad_rt(p.act, g[i], value, slope);
+      dg[i] = v[i] * up[i] * slope;
+      u[i] = v[i] * value;
+      v[i] = value * up[i];
+    }
+    __nv_bfloat16* dz = p.dz + row * 2 * p.F + col;
+    *reinterpret_cast<uint2*>(dz) = ffn_pack4(dg);
+    *reinterpret_cast<uint2*>(dz + p.F) = ffn_pack4(u);
+  } else if (q.residual) {
+    const uint2 w = *reinterpret_cast<const uint2*>(q.residual + row * q.J + col);
+    v[0] += __uint_as_float(w.x << 16);
+    v[1] += __uint_as_float(w.x & 0xFFFF0000u);
+    v[2] += __uint_as_float(w.y << 16);
+    v[3] += __uint_as_float(w.y & 0xFFFF0000u);
+  }
+  *reinterpret_cast<uint2*>(q.out + row * q.J + col) = ffn_pack4(v);
+}
+
+// Joins this CTA's share of a tile: ROWS / S outputs of every token, four at a
+// time, summed over the S partial tiles in rank order.  A thread has 8 loads
+// of other CTAs' memory in flight: one after the other, they were half of a
+// small launch's time.
+template <int MODE, int S>
+__device__ __forceinline__ void ffn_join(const FfnTileParams& p, const FfnTileProblem& q,
+                                         uint32_t part, int first, int rank, int j0, int t0,
+                                         int tokens) {
+  constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;
+  constexpr int R4 = ROWS / S / 4, U = 8 / S;
+  const int n = R4 * tokens;
+  for (int e0 = threadIdx.x; e0 < n; e0 += kTileThreads * U) {
+    float4 a[U][S], b[U][S];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int e = min(e0 + k * kTileThreads, n - 1);
+      const uint32_t mine = part + (uint32_t)((e / R4) * 128 + (rank * R4 + e % R4) * 4) * 4;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint32_t at = mapa_cta(mine, first + s);
+        a[k][s] = ld_cluster_f32x4(at);
+        if constexpr (MODE == FFN_GLU) b[k][s] = ld_cluster_f32x4(at + 64 * 4);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int e = e0 + k * kTileThreads;
+      const int col = j0 + (rank * R4 + e % R4) * 4;
+      if (e >= n || col >= q.J) continue;
+      float v[4] = {a[k][0].x, a[k][0].y, a[k][0].z, a[k][0].w}, u[4];
+      if constexpr (MODE == FFN_GLU)
+        u[0] = b[k][0].x, u[1] = b[k][0].y, u[2] = b[k][0].z, u[3] = b[k][0].w;
+#pragma unroll
+      for (int s = 1; s < S; ++s) {
+        v[0] += a[k][s].x, v[1] += a[k][s].y, v[2] += a[k][s].z, v[3] += a[k][s].w;
+        if constexpr (MODE == FFN_GLU)
+          u[0] += b[k][s].x, u[1] += b[k][s].y, u[2] += b[k][s].z, u[3] += b[k][s].w;
+      }
+      ffn_tile_store<MODE>(p, q, (long long)t0 + e / R4, col, v, u);
+    }
+  }
+}
+
+template <int NT, int MODE>
+__global__ void __launch_bounds__(kTileThreads)
+    ffn_tile_kernel(const __grid_constant__ FfnMaps maps,
+                    const __grid_constant__ FfnTileParams p) {
+  using C = TileCfg<NT>;
+  constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;  // outputs of a tile
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;  // same offset in every CTA of the cluster
@@ -616,12 +727,20 @@ __global__ void __launch_bounds__(kTokThreads)
   auto empty = [&](int s) { return smem_u32(bars + C::STAGES + s); };
   const uint32_t done = smem_u32(bars + 2 * C::STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int S = (int)gridDim.z;  // the cluster: CTAs of the same (x, y)
-  const int rank = (int)cluster_ctarank();
-  const int j0 = (int)blockIdx.x * ROWS, t0 = (int)blockIdx.y * NT;
-  const int kb0 = (int)((long long)p.n_kblk * rank / S);
-  const int kb1 = (int)((long long)p.n_kblk * (rank + 1) / S);
-  const int n_kb = kb1 - kb0;  // at least 1: S <= n_kblk
+  const int cluster = (int)gridDim.y, crank = (int)cluster_ctarank();
+  // cluster -> product; -> row tile (slow) and token tile (fast: tiles that
+  // share rows of A run together, so those come from memory once)
+  int at = (int)blockIdx.x, which = 0;
+  while (which + 1 < p.n_prob && at >= p.prob[which].n_clusters) at -= p.prob[which++].n_clusters;
+  const FfnTileProblem& q = p.prob[which];
+  const CUtensorMap* tm_a = &maps.a[which];
+  const CUtensorMap* tm_b = &maps.b[which];
+  const int S = q.split ? cluster : 1, rank = q.split ? crank : 0;  // shares of this tile's K
+  const int tile = q.split ? at : at * cluster + crank;
+  const bool idle = tile >= q.n_tiles;  // the last cluster of a product that is not split
+  const int j0 = (tile / q.n_tt) * ROWS, t0 = (tile % q.n_tt) * NT;
+  const int kb0 = (int)((long long)q.n_kblk * rank / S);
+  const int n_kb = idle ? 0 : (int)((long long)q.n_kblk * (rank + 1) / S) - kb0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -640,25 +759,40 @@ __global__ void __launch_bounds__(kTokThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (GLU) pdl_launch_dependents();
+  pdl_launch_dependents();  // (a kernel behind this one may set itself up)
 
   if (warp == 0) {
-    auto load_w = [&](int kb, int s) {
-      const uint32_t sw = sbase + s * C::STAGE_BYTES;
-      if constexpr (GLU) {
-        tma_load_2d(sw, &tm_w, full(s), (kb0 + kb) * 64, j0);
-        tma_load_2d(sw + 8192, &tm_w, full(s), (kb0 + kb) * 64, p.n_out + j0);
+    const bool a_mn = q.a_mn, b_mn = q.b_mn;
+    auto load_a = [&](int kb, int s) {
+      const uint32_t sa = sbase + s * C::STAGE_BYTES;
+      const int k = (kb0 + kb) * 64;
+      if (MODE == FFN_GLU) {
+        tma_load_2d(sa, tm_a, full(s), k, j0);
+        tma_load_2d(sa + 8192, tm_a, full(s), k, p.F + j0);
+      } else if (a_mn) {
+        tma_load_2d(sa, tm_a, full(s), j0, k);
+        tma_load_2d(sa + 8192, tm_a, full(s), j0 + 64, k);
       } else {
-        tma_load_2d(sw, &tm_w, full(s), (kb0 + kb) * 64, j0);
+        tma_load_2d(sa, tm_a, full(s), k, j0);
       }
     };
-    // the weights do not depend on the kernel before this one: the ring's
-    // first stages are requested before its result is waited for
-    const int early = min(n_kb, C::STAGES);
+    auto load_b = [&](int kb, int s) {
+      const uint32_t sb = sbase + s * C::STAGE_BYTES + C::A_BYTES;
+      const int k = (kb0 + kb) * 64;
+      if (NT >= 64 && b_mn) {
+        for (int h = 0; h < NT / 64; ++h)
+          tma_load_2d(sb + h * 8192, tm_b, full(s), t0 + h * 64, k);
+      } else {
+        tma_load_2d(sb, tm_b, full(s), k, t0);
+      }
+    };
+    // what does not depend on the kernel before this one (the weights): the
+    // ring's first stages are requested before its result is waited for
+    const int early = q.a_early ? min(n_kb, C::STAGES) : 0;
     if (elect_one())
       for (int kb = 0; kb < early; ++kb) {
         mbar_arrive_expect_tx(full(kb), C::STAGE_BYTES);
-        load_w(kb, kb);
+        load_a(kb, kb);
       }
     __syncwarp();
     if (p.pdl) pdl_wait();
@@ -669,11 +803,11 @@ __global__ void __launch_bounds__(kTokThreads)
       if (u > 0) ok = mbar_wait_warp(empty(s), (u - 1) & 1, abort_flag, 931);
       if (!ok) break;
       if (elect_one()) {
-        if (u > 0) {
+        if (kb >= early) {
           mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
-          load_w(kb, s);
+          load_a(kb, s);
         }
-        tma_load_2d(sbase + s * C::STAGE_BYTES + C::W_BYTES, &tm_x, full(s), (kb0 + kb) * 64, t0);
+        load_b(kb, s);
       }
       __syncwarp();
       issued = kb + 1;
@@ -684,9 +818,11 @@ __global__ void __launch_bounds__(kTokThreads)
         if (n_s) (void)mbar_wait(full(s), (n_s - 1) & 1, nullptr, 932);
       }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = make_idesc_bf16(128, NT, 0, 0);
-    const uint64_t dw0 = make_sdesc_sw128(sbase, 16, 1024);
-    const uint64_t dx0 = make_sdesc_sw128(sbase + C::W_BYTES, 16, 1024);
+    const int a_mn = q.a_mn, b_mn = q.b_mn;
+    const uint32_t idesc = make_idesc_bf16(128, NT, a_mn, b_mn);
+    const uint64_t da0 = make_sdesc_sw128(sbase, a_mn ? 8192 : 16, 1024);
+    const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
+    const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
     bool ok = true;
     for (int kb = 0; kb < n_kb; ++kb) {
       const int s = kb % C::STAGES;
@@ -697,7 +833,7 @@ __global__ void __launch_bounds__(kTokThreads)
         const uint32_t off = s * C::STAGE_BYTES;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_ss(tmem, desc_adv(dw0, off + kk * 32), desc_adv(dx0, off + kk * 32), idesc,
+          mma_ss(tmem, desc_adv(da0, off + kk * a_step), desc_adv(db0, off + kk * b_step), idesc,
                  (kb | kk) != 0 ? 1u : 0u);
         tc_commit(empty(s));
       }
@@ -717,7 +853,7 @@ __global__ void __launch_bounds__(kTokThreads)
     const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
     for (int c = 0; c < NT; c += 16) {
-      if (t0 + c >= p.m) break;
+      if (idle || t0 + c >= q.T) break;
       uint32_t r[16];
       tmem_ld16(acc + c, r);
       tmem_wait_ld();
@@ -733,33 +869,14 @@ __global__ void __launch_bounds__(kTokThreads)
     tc_fence_after();
     tmem_dealloc(tmem, C::TM_COLS);
   }
-  if (p.pdl) pdl_wait();  // the residual and the output belong to the stream's order too
-  if (!*abort_flag) {
-    // this CTA joins ROWS / S outputs of every token
-    const int rows = ROWS / S, r0 = rank * rows;
-    const int tokens = min(NT, p.m - t0);
-    const uint32_t part_addr = sbase;
-    for (int e = threadIdx.x; e < rows * tokens; e += kTokThreads) {
-      const int t = e / rows, j = r0 + e % rows;
-      const int col = j0 + j;
-      if (col >= p.n_out) continue;
-      float g = 0.0f, u = 0.0f;
-      for (int s = 0; s < S; ++s) {
-        const uint32_t at = mapa_cta(part_addr + (uint32_t)(t * 128 + j) * 4, s);
-        g += ld_cluster_f32(at);
-        if constexpr (GLU) u += ld_cluster_f32(at + 64 * 4);
-      }
-      const long long row = t0 + t;
-      if constexpr (GLU) {
-        if (p.z) {
-          p.z[row * 2 * p.n_out + col] = g;
-          p.z[row * 2 * p.n_out + p.n_out + col] = u;
-        }
-        g = ffn_act_rt(p.act, g) * u;
-      } else if (p.residual) {
-        g += __bfloat162float(p.residual[row * p.n_out + col]);
-      }
-      p.out[row * p.n_out + col] = __float2bfloat16_rn(g);
+  if (p.pdl) pdl_wait();  // the residual and the outputs belong to the stream's order too
+  if (!*abort_flag && !idle) {
+    const int tokens = min(NT, q.T - t0);
+    switch (S) {
+      case 1: ffn_join<MODE, 1>(p, q, sbase, crank, 0, j0, t0, tokens); break;
+      case 2: ffn_join<MODE, 2>(p, q, sbase, 0, rank, j0, t0, tokens); break;
+      case 4: ffn_join<MODE, 4>(p, q, sbase, 0, rank, j0, t0, tokens); break;
+      default: ffn_join<MODE, 8>(p, q, sbase, 0, rank, j0, t0, tokens); break;
     }
   }
   __syncwarp();

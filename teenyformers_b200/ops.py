@@ -379,7 +379,7 @@ def _dense(x: torch.Tensor, dtype: torch.dtype, what: str, *ts) -> None:
 def _buffer(t: torch.Tensor | None, shape, dtype: torch.dtype, x: torch.Tensor,
             name: str) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=x.device)
+        return x.new_empty(shape, dtype=dtype)
     if (t.shape != shape or t.dtype != dtype or t.get_device() != x.get_device()
             or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {x.device}")
@@ -410,7 +410,7 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
     lead = x.shape[:-1]
     _dense(x, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, residual)
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
-    y = _buffer(out, x.shape, torch.bfloat16, x, "out")
+    y = torch.empty_like(x) if out is None else _buffer(out, x.shape, torch.bfloat16, x, "out")
     a = _buffer(act_out, lead + (d_ff,), torch.bfloat16, x, "act_out")
     z = _buffer(z_out, lead + (2 * d_ff,), torch.float32, x, "z_out") if save else None
     _launch(x, "tf_b200_gated_ffn_fwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
@@ -431,7 +431,8 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor
     _need(dy.shape == x.shape, "dy must have x's shape")
     _need(z.shape == x.shape[:-1] + (2 * d_ff,), "z must be [..., 2 * d_ff]")
     given = (None, None, None) if grads is None else grads
-    g = [_buffer(t, like.shape, torch.bfloat16, x, "a gradient") if on else None
+    g = [None if not on else torch.empty_like(like) if t is None
+         else _buffer(t, like.shape, torch.bfloat16, x, "a gradient")
          for t, like, on in zip(given, (x, w_gate_up, w_down), need)]
     n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d_ff)
     ws = _workspace(n, workspace, x)
@@ -461,7 +462,7 @@ def _rng_addr(p: float, rng: torch.Tensor | None, site: int, x: torch.Tensor):
 
 def _workspace(n: int, ws: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
     if ws is None:
-        return torch.empty(int(n), dtype=torch.uint8, device=x.device)
+        return x.new_empty(n, dtype=torch.uint8)
     if ws.get_device() != x.get_device() or not ws.is_contiguous() or \
             ws.numel() * ws.element_size() < n:
         raise ValueError(f"workspace must be contiguous and have {n} bytes on {x.device}")
@@ -479,7 +480,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
     _need(x.is_cuda, "x must be a CUDA tensor")
     _dense(x, x.dtype, "dropout", x, residual)
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
-    y = _buffer(out, x.shape, x.dtype, x, "out")
+    y = torch.empty_like(x) if out is None else _buffer(out, x.shape, x.dtype, x, "out")
     _launch(x, fn, x.data_ptr(), _addr(residual), y.data_ptr(), _rng_addr(p, rng, site, x),
             x.numel(), float(p), int(site))
     return y
