@@ -33,6 +33,23 @@ namespace tfb {
 
 enum FfnAct : int { FFN_ACT_SILU = 0, FFN_ACT_GELU = 1, FFN_ACT_GELU_TANH = 2 };
 
+// Phi(g), the normal distribution function, and E = exp(-g^2 / 2), by the
+// rational approximation 7.1.26 of Abramowitz and Stegun's Handbook (after
+// Hastings): erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2) + e, t = 1 / (1 + p x),
+// |e| <= 1.5e-7.  It shares its exponential with the slope's density and has
+// no branch.
+__device__ __forceinline__ float ffn_phi(float g, float& E) {
+  const float x = fabsf(g) * 0.70710678118654752f;
+  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f) * t;
+  E = __expf(-0.5f * g * g);
+  q *= 0.5f * E;  // Phi(-|g|)
+  return g < 0.0f ? q : 1.0f - q;
+}
+
 // act(g).  The quotients use __fdividef (2 ulp; 0 for a divisor above 2^126,
 // where the result is below 1e-36): a full fp32 division is a dozen
 // instructions, and the epilogue of a short product is bound by its own.
@@ -41,7 +58,8 @@ __device__ __forceinline__ float ffn_act(float g) {
   if constexpr (ACT == FFN_ACT_SILU) {
     return __fdividef(g, 1.0f + __expf(-g));
   } else if constexpr (ACT == FFN_ACT_GELU) {
-    return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    float E;
+    return g * ffn_phi(g, E);
   } else {
     // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), v = sqrt(2/pi) (g + 0.044715 g^3)
     const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
@@ -49,21 +67,22 @@ __device__ __forceinline__ float ffn_act(float g) {
   }
 }
 
-// act(g) and act'(g)
+// act(g), the same bits as ffn_act's, and act'(g)
 template <int ACT>
 __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope) {
   if constexpr (ACT == FFN_ACT_SILU) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
     value = ffn_act<ACT>(g);
+    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
     slope = s * (1.0f + g * (1.0f - s));
   } else if constexpr (ACT == FFN_ACT_GELU) {
-    value = ffn_act<ACT>(g);
-    slope = 0.5f * (1.0f + erff(g * 0.70710678118654752f)) +
-            g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    float E;
+    const float phi = ffn_phi(g, E);
+    value = g * phi;
+    slope = fmaf(g * 0.39894228040143268f, E, phi);
   } else {
+    value = ffn_act<ACT>(g);
     const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
     const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * v));
-    value = ffn_act<ACT>(g);
     slope = s + g * s * (1.0f - s) * 2.0f * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
   }
 }
@@ -72,6 +91,15 @@ __device__ __forceinline__ float ffn_act_rt(int act, float g) {  // (uniform bra
   if (act == FFN_ACT_SILU) return ffn_act<FFN_ACT_SILU>(g);
   if (act == FFN_ACT_GELU) return ffn_act<FFN_ACT_GELU>(g);
   return ffn_act<FFN_ACT_GELU_TANH>(g);
+}
+
+// Programmatic dependent launch: blocks until the kernels this one depends on
+// have completed and their writes are visible (returns at once without PDL).
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ===================================================================== CTA pairs
@@ -407,6 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   cluster_sync_all();  // both CTAs' barriers initialised before any remote signal
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // (a tile kernel behind this one may set itself up)
 
   if (warp == 0) {
     // ===================== TMA producer (both CTAs) =====================
@@ -544,18 +573,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
 }
 
 // ===================================================================== small products
-// out[t, j] over tiles of 128 rows j of A (FFN_GLU: 64 gate rows and the 64 up
-// rows of the same outputs) and NT rows t of B: D[128, NT] = A[128, K] B[NT, K]^T,
-// one CTA a tile and up to three products in one launch.  With the weights as
-// A and a few tokens as B the block is bound by reading the weights once; with
-// more tokens these tiles are small enough to fill the SMs where 256 x 256 ones
-// are not.  A cluster of S CTAs takes one tile, each a contiguous run of
+// out[t, j] over tiles of 128 weight rows j (FFN_GLU: 64 gate rows and the 64 up
+// rows of the same outputs) and NT tokens t: D[128, NT] = W[128, K] X[NT, K]^T.
+// With few tokens the product is bound by reading the weights once; with more,
+// these tiles fill the SMs where 256 x 256 ones are too few.  A cluster of S CTAs takes one tile, each a contiguous run of
 // k-blocks through its own TMA ring; the S partial tiles are summed through
 // distributed shared memory, always in rank order, so results repeat bit for
 // bit.
-//   warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 move the accumulator
-//   from TMEM to shared memory; all warps join the partials.
-constexpr int kTileThreads = 192;
+//   warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 move the accumulator
+//   from TMEM to shared memory (two a lane quarter, half the columns each);
+//   all warps join the partials.
+constexpr int kTileThreads = 320;
 
 template <int NT>
 struct TileCfg {
@@ -569,24 +597,14 @@ struct TileCfg {
   static_assert(NT * 128 * 4 <= OFF_BAR, "the partial tile exceeds the ring");
 };
 
-struct FfnTileProblem {
-  int J, T;      // rows of A (FFN_GLU: outputs, half of them) and of B
-  int n_tt, n_tiles, n_kblk;
-  int split;       // a cluster takes one tile and splits K; 0: a tile for each of its CTAs
-  int n_clusters;
-  int a_mn, b_mn;  // operand stored with its row index innermost (b_mn: NT >= 64)
-  int a_early;     // A is not written by the kernel before this one
-  __nv_bfloat16* out;             // [T, J]
-  const __nv_bfloat16* residual;  // FFN_STORE: [T, J] or null
-};
-
 struct FfnTileParams {
-  FfnTileProblem prob[kFfnMaxProblems];
-  int n_prob, act;
-  int pdl;  // launched with programmatic stream serialization
-  int F;
-  float* z;           // [T, 2F] (FFN_GLU: null if not saved)
-  __nv_bfloat16* dz;  // FFN_DGLU: [T, 2F]; prob[0].out is a
+  int J, T;  // outputs of a token, tokens
+  int n_tt, n_kblk;
+  int act;   // FFN_GLU
+  int pdl;   // launched with programmatic stream serialization
+  __nv_bfloat16* out;             // [T, J]
+  float* z;                       // FFN_GLU: [T, 2 J] or null
+  const __nv_bfloat16* residual;  // FFN_STORE: [T, J] or null
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
@@ -605,23 +623,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
-// Programmatic dependent launch: blocks until the kernels this one depends on
-// have completed and their writes are visible (returns at once without PDL).
-__device__ __forceinline__ void pdl_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void pdl_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
-__device__ __forceinline__ void ffn_act_grad_rt(int act, float g, float& value, float& slope) {
-  if (act == FFN_ACT_SILU)
-    ffn_act_grad<FFN_ACT_SILU>(g, value, slope);
-  else if (act == FFN_ACT_GELU)
-    ffn_act_grad<FFN_ACT_GELU>(g, value, slope);
-  else
-    ffn_act_grad<FFN_ACT_GELU_TANH>(g, value, slope);
-}
 __device__ __forceinline__ uint2 ffn_pack4(const float (&v)[4]) {
   return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
@@ -629,42 +630,24 @@ __device__ __forceinline__ uint2 ffn_pack4(const float (&v)[4]) {
 // What is done with four joined outputs v (FFN_GLU: and the four u beside
 // them) at row `row` of the output and column `col`.
 template <int MODE>
-__device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, const FfnTileProblem& q,
-                                               long long row, int col, float (&v)[4],
-                                               float (&u)[4]) {
+__device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, long long row, int col,
+                                               float (&v)[4], float (&u)[4]) {
   if constexpr (MODE == FFN_GLU) {
     if (p.z) {
-      float* z = p.z + row * 2 * p.F + col;
+      float* z = p.z + row * 2 * p.J + col;
       *reinterpret_cast<float4*>(z) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(z + p.F) = make_float4(u[0], u[1], u[2], u[3]);
+      *reinterpret_cast<float4*>(z + p.J) = make_float4(u[0], u[1], u[2], u[3]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = ffn_act_rt(p.act, v[i]) * u[i];
-  } else if constexpr (MODE == FFN_DGLU) {
-    const float* z = p.z + row * 2 * p.F + col;
-    const float4 g4 = *reinterpret_cast<const float4*>(z);
-    const float4 u4 = *reinterpret_cast<const float4*>(z + p.F);
-    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, up[4] = {u4.x, u4.y, u4.z, u4.w};
-    float dg[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float value, slope;
-      ffn_act_grad_rt(p.act, g[i], value, slope);
-      dg[i] = v[i] * up[i] * slope;
-      u[i] = v[i] * value;
-      v[i] = value * up[i];
-    }
-    __nv_bfloat16* dz = p.dz + row * 2 * p.F + col;
-    *reinterpret_cast<uint2*>(dz) = ffn_pack4(dg);
-    *reinterpret_cast<uint2*>(dz + p.F) = ffn_pack4(u);
-  } else if (q.residual) {
-    const uint2 w = *reinterpret_cast<const uint2*>(q.residual + row * q.J + col);
+  } else if (p.residual) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p.residual + row * p.J + col);
     v[0] += __uint_as_float(w.x << 16);
     v[1] += __uint_as_float(w.x & 0xFFFF0000u);
     v[2] += __uint_as_float(w.y << 16);
     v[3] += __uint_as_float(w.y & 0xFFFF0000u);
   }
-  *reinterpret_cast<uint2*>(q.out + row * q.J + col) = ffn_pack4(v);
+  *reinterpret_cast<uint2*>(p.out + row * p.J + col) = ffn_pack4(v);
 }
 
 // Joins this CTA's share of a tile: ROWS / S outputs of every token, four at a
@@ -672,9 +655,8 @@ __device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, const Ffn
 // of other CTAs' memory in flight: one after the other, they were half of a
 // small launch's time.
 template <int MODE, int S>
-__device__ __forceinline__ void ffn_join(const FfnTileParams& p, const FfnTileProblem& q,
-                                         uint32_t part, int first, int rank, int j0, int t0,
-                                         int tokens) {
+__device__ __forceinline__ void ffn_join(const FfnTileParams& p, uint32_t part, int rank, int j0,
+                                         int t0, int tokens) {
   constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;
   constexpr int R4 = ROWS / S / 4, U = 8 / S;
   const int n = R4 * tokens;
@@ -686,7 +668,7 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, const FfnTilePr
       const uint32_t mine = part + (uint32_t)((e / R4) * 128 + (rank * R4 + e % R4) * 4) * 4;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const uint32_t at = mapa_cta(mine, first + s);
+        const uint32_t at = mapa_cta(mine, s);
         a[k][s] = ld_cluster_f32x4(at);
         if constexpr (MODE == FFN_GLU) b[k][s] = ld_cluster_f32x4(at + 64 * 4);
       }
@@ -695,7 +677,7 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, const FfnTilePr
     for (int k = 0; k < U; ++k) {
       const int e = e0 + k * kTileThreads;
       const int col = j0 + (rank * R4 + e % R4) * 4;
-      if (e >= n || col >= q.J) continue;
+      if (e >= n || col >= p.J) continue;
       float v[4] = {a[k][0].x, a[k][0].y, a[k][0].z, a[k][0].w}, u[4];
       if constexpr (MODE == FFN_GLU)
         u[0] = b[k][0].x, u[1] = b[k][0].y, u[2] = b[k][0].z, u[3] = b[k][0].w;
@@ -705,15 +687,15 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, const FfnTilePr
         if constexpr (MODE == FFN_GLU)
           u[0] += b[k][s].x, u[1] += b[k][s].y, u[2] += b[k][s].z, u[3] += b[k][s].w;
       }
-      ffn_tile_store<MODE>(p, q, (long long)t0 + e / R4, col, v, u);
+      ffn_tile_store<MODE>(p, (long long)t0 + e / R4, col, v, u);
     }
   }
 }
 
 template <int NT, int MODE>
 __global__ void __launch_bounds__(kTileThreads)
-    ffn_tile_kernel(const __grid_constant__ FfnMaps maps,
-                    const __grid_constant__ FfnTileParams p) {
+    ffn_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
+                    const __grid_constant__ CUtensorMap tm_b, const FfnTileParams p) {
   using C = TileCfg<NT>;
   constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;  // outputs of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -727,20 +709,12 @@ __global__ void __launch_bounds__(kTileThreads)
   auto empty = [&](int s) { return smem_u32(bars + C::STAGES + s); };
   const uint32_t done = smem_u32(bars + 2 * C::STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cluster = (int)gridDim.y, crank = (int)cluster_ctarank();
-  // cluster -> product; -> row tile (slow) and token tile (fast: tiles that
-  // share rows of A run together, so those come from memory once)
-  int at = (int)blockIdx.x, which = 0;
-  while (which + 1 < p.n_prob && at >= p.prob[which].n_clusters) at -= p.prob[which++].n_clusters;
-  const FfnTileProblem& q = p.prob[which];
-  const CUtensorMap* tm_a = &maps.a[which];
-  const CUtensorMap* tm_b = &maps.b[which];
-  const int S = q.split ? cluster : 1, rank = q.split ? crank : 0;  // shares of this tile's K
-  const int tile = q.split ? at : at * cluster + crank;
-  const bool idle = tile >= q.n_tiles;  // the last cluster of a product that is not split
-  const int j0 = (tile / q.n_tt) * ROWS, t0 = (tile % q.n_tt) * NT;
-  const int kb0 = (int)((long long)q.n_kblk * rank / S);
-  const int n_kb = idle ? 0 : (int)((long long)q.n_kblk * (rank + 1) / S) - kb0;
+  const int S = (int)gridDim.y, rank = (int)cluster_ctarank();  // shares of this tile's K
+  // row tiles are slow, token tiles fast: tiles that share rows of A run
+  // together, so those come from memory once
+  const int j0 = (int)blockIdx.x / p.n_tt * ROWS, t0 = (int)blockIdx.x % p.n_tt * NT;
+  const int kb0 = (int)((long long)p.n_kblk * rank / S);
+  const int n_kb = (int)((long long)p.n_kblk * (rank + 1) / S) - kb0;  // at least 1
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -762,33 +736,15 @@ __global__ void __launch_bounds__(kTileThreads)
   pdl_launch_dependents();  // (a kernel behind this one may set itself up)
 
   if (warp == 0) {
-    const bool a_mn = q.a_mn, b_mn = q.b_mn;
     auto load_a = [&](int kb, int s) {
       const uint32_t sa = sbase + s * C::STAGE_BYTES;
       const int k = (kb0 + kb) * 64;
-      if (MODE == FFN_GLU) {
-        tma_load_2d(sa, tm_a, full(s), k, j0);
-        tma_load_2d(sa + 8192, tm_a, full(s), k, p.F + j0);
-      } else if (a_mn) {
-        tma_load_2d(sa, tm_a, full(s), j0, k);
-        tma_load_2d(sa + 8192, tm_a, full(s), j0 + 64, k);
-      } else {
-        tma_load_2d(sa, tm_a, full(s), k, j0);
-      }
+      tma_load_2d(sa, &tm_a, full(s), k, j0);
+      if (MODE == FFN_GLU) tma_load_2d(sa + 8192, &tm_a, full(s), k, p.J + j0);
     };
-    auto load_b = [&](int kb, int s) {
-      const uint32_t sb = sbase + s * C::STAGE_BYTES + C::A_BYTES;
-      const int k = (kb0 + kb) * 64;
-      if (NT >= 64 && b_mn) {
-        for (int h = 0; h < NT / 64; ++h)
-          tma_load_2d(sb + h * 8192, tm_b, full(s), t0 + h * 64, k);
-      } else {
-        tma_load_2d(sb, tm_b, full(s), k, t0);
-      }
-    };
-    // what does not depend on the kernel before this one (the weights): the
-    // ring's first stages are requested before its result is waited for
-    const int early = q.a_early ? min(n_kb, C::STAGES) : 0;
+    // the weights do not depend on the kernel before this one: the ring's first
+    // stages of them are requested before its result is waited for
+    const int early = min(n_kb, C::STAGES);
     if (elect_one())
       for (int kb = 0; kb < early; ++kb) {
         mbar_arrive_expect_tx(full(kb), C::STAGE_BYTES);
@@ -807,7 +763,7 @@ __global__ void __launch_bounds__(kTileThreads)
           mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
           load_a(kb, s);
         }
-        load_b(kb, s);
+        tma_load_2d(sbase + s * C::STAGE_BYTES + C::A_BYTES, &tm_b, full(s), (kb0 + kb) * 64, t0);
       }
       __syncwarp();
       issued = kb + 1;
@@ -818,11 +774,9 @@ __global__ void __launch_bounds__(kTileThreads)
         if (n_s) (void)mbar_wait(full(s), (n_s - 1) & 1, nullptr, 932);
       }
   } else if (warp == 1) {
-    const int a_mn = q.a_mn, b_mn = q.b_mn;
-    const uint32_t idesc = make_idesc_bf16(128, NT, a_mn, b_mn);
-    const uint64_t da0 = make_sdesc_sw128(sbase, a_mn ? 8192 : 16, 1024);
-    const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
-    const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+    constexpr uint32_t idesc = make_idesc_bf16(128, NT, 0, 0);
+    const uint64_t da0 = make_sdesc_sw128(sbase, 16, 1024);
+    const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, 16, 1024);
     bool ok = true;
     for (int kb = 0; kb < n_kb; ++kb) {
       const int s = kb % C::STAGES;
@@ -833,7 +787,7 @@ __global__ void __launch_bounds__(kTileThreads)
         const uint32_t off = s * C::STAGE_BYTES;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_ss(tmem, desc_adv(da0, off + kk * a_step), desc_adv(db0, off + kk * b_step), idesc,
+          mma_ss(tmem, desc_adv(da0, off + kk * 32), desc_adv(db0, off + kk * 32), idesc,
                  (kb | kk) != 0 ? 1u : 0u);
         tc_commit(empty(s));
       }
@@ -852,8 +806,8 @@ __global__ void __launch_bounds__(kTileThreads)
     const int quarter = warp & 3;
     const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-    for (int c = 0; c < NT; c += 16) {
-      if (idle || t0 + c >= q.T) break;
+    for (int c = ((warp - 2) >> 2) * 16; c < NT; c += 32) {
+      if (t0 + c >= p.T) break;
       uint32_t r[16];
       tmem_ld16(acc + c, r);
       tmem_wait_ld();
@@ -870,13 +824,13 @@ __global__ void __launch_bounds__(kTileThreads)
     tmem_dealloc(tmem, C::TM_COLS);
   }
   if (p.pdl) pdl_wait();  // the residual and the outputs belong to the stream's order too
-  if (!*abort_flag && !idle) {
-    const int tokens = min(NT, q.T - t0);
+  if (!*abort_flag) {
+    const int tokens = min(NT, p.T - t0);
     switch (S) {
-      case 1: ffn_join<MODE, 1>(p, q, sbase, crank, 0, j0, t0, tokens); break;
-      case 2: ffn_join<MODE, 2>(p, q, sbase, 0, rank, j0, t0, tokens); break;
-      case 4: ffn_join<MODE, 4>(p, q, sbase, 0, rank, j0, t0, tokens); break;
-      default: ffn_join<MODE, 8>(p, q, sbase, 0, rank, j0, t0, tokens); break;
+      case 1: ffn_join<MODE, 1>(p, sbase, 0, j0, t0, tokens); break;
+      case 2: ffn_join<MODE, 2>(p, sbase, rank, j0, t0, tokens); break;
+      case 4: ffn_join<MODE, 4>(p, sbase, rank, j0, t0, tokens); break;
+      default: ffn_join<MODE, 8>(p, sbase, rank, j0, t0, tokens); break;
     }
   }
   __syncwarp();

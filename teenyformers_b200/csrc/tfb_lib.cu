@@ -159,7 +159,6 @@ int ensure_device_setup() {
     TFB_TILE_SET(64);
     TFB_TILE_SET(128);
 #undef TFB_TILE_SET
-    set((const void*)ffn_tile_kernel<128, FFN_DGLU>, TileCfg<128>::SMEM_ALLOC);
     set((const void*)dropout_kernel<__nv_bfloat16>, kDropSmem);
     set((const void*)dropout_kernel<float>, kDropSmem);
     // 8192 columns: one row a stage of three
@@ -1056,53 +1055,24 @@ int ffn_pair_launch_act(int act, const FfnMaps& maps, FfnPairParams& prm, cudaSt
   }
 }
 
-// A product of the tile kernel; `nt` rows of B a tile.
-void ffn_tile_problem(FfnTileProblem& q, int J, int T, int K, int a_mn, int b_mn, int rows, int nt,
-                      int a_early, void* out, const void* residual) {
-  q.J = J, q.T = T;
-  q.n_tt = (T + nt - 1) / nt;
-  q.n_tiles = (J + rows - 1) / rows * q.n_tt;
-  q.n_kblk = (K + kGemmBK - 1) / kGemmBK;
-  q.a_mn = a_mn, q.b_mn = b_mn, q.a_early = a_early;
-  q.out = static_cast<__nv_bfloat16*>(out);
-  q.residual = static_cast<const __nv_bfloat16*>(residual);
-}
-
-bool ffn_tile_operand(CUtensorMap* map, const void* base, int mn, int k, int mn_major, int box) {
-  return mn_major ? make_bf16_2d_map(map, base, mn, k, 64)
-                  : make_bf16_2d_map(map, base, k, mn, box);
-}
-
-// CTAs that take one tile's K: a power of two up to 8, until the launch has
-// kTileCtas CTAs or a CTA's share of the longest K falls under four k-blocks.
-// Products with less than half that K are not split.
-#ifndef TFB_TILE_CTAS
-#define TFB_TILE_CTAS 148
-#endif
-constexpr int kTileCtas = TFB_TILE_CTAS;
-
+// One product of the tile kernel: `w` has w_rows rows (FFN_GLU: 2 J) of k.
+// A cluster of S CTAs takes a tile: a power of two up to 8, until the launch
+// has 148 CTAs or a CTA's share of K falls under four k-blocks.
 template <int NT, int MODE>
-int ffn_tile_launch(const FfnMaps& maps, FfnTileParams& prm, cudaStream_t st) {
-  int longest = 0;
-  for (int i = 0; i < prm.n_prob; ++i) longest = std::max(longest, prm.prob[i].n_kblk);
-  for (int i = 0; i < prm.n_prob; ++i) prm.prob[i].split = 2 * prm.prob[i].n_kblk >= longest;
-  auto ctas = [&](int s) {
-    long long n = 0;
-    for (int i = 0; i < prm.n_prob; ++i)
-      n += (long long)prm.prob[i].n_tiles * (prm.prob[i].split ? s : 1);
-    return n;
-  };
-  if (!fits_i32(ctas(1))) return TF_ERR_TOO_LARGE;
+int ffn_tile_launch(const void* w, int w_rows, const void* x, int k, FfnTileParams& prm,
+                    cudaStream_t st) {
+  constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;
+  CUtensorMap ta, tb;
+  if (!make_bf16_2d_map(&ta, w, k, w_rows, ROWS) || !make_bf16_2d_map(&tb, x, k, prm.T, NT))
+    return TF_ERR_CUDA;
+  prm.n_kblk = (k + kGemmBK - 1) / kGemmBK;
+  prm.n_tt = (prm.T + NT - 1) / NT;
+  const long long tiles = (long long)((prm.J + ROWS - 1) / ROWS) * prm.n_tt;
+  if (!fits_i32(tiles)) return TF_ERR_TOO_LARGE;
   int S = 1;
-  while (S < 8 && ctas(S) < kTileCtas && longest >= 8 * S) S *= 2;
-  long long clusters = 0;
-  for (int i = 0; i < prm.n_prob; ++i) {
-    FfnTileProblem& q = prm.prob[i];
-    q.n_clusters = q.split ? q.n_tiles : (q.n_tiles + S - 1) / S;
-    clusters += q.n_clusters;
-  }
+  while (S < 8 && tiles * S < 148 && prm.n_kblk >= 8 * S) S *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)clusters, (unsigned)S, 1);
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)S, 1);
   cfg.blockDim = dim3(kTileThreads, 1, 1);
   cfg.dynamicSmemBytes = TileCfg<NT>::SMEM_ALLOC;
   cfg.stream = st;
@@ -1115,42 +1085,37 @@ int ffn_tile_launch(const FfnMaps& maps, FfnTileParams& prm, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = prm.pdl ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, ffn_tile_kernel<NT, MODE>, maps, prm) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, ffn_tile_kernel<NT, MODE>, ta, tb, prm) != cudaSuccess) {
     (void)cudaGetLastError();
     return TF_ERR_CUDA;
   }
   return launch_status();
 }
 
-// Forward with the tile kernel: the weights' rows are A, the tokens B.
-template <int NT>
-int ffn_tile_fwd(const void* x, const void* w_gate_up, const void* w_down, const void* residual,
-                 void* a, float* z, void* y, int m, int d, int F, int act, cudaStream_t st) {
-  FfnMaps maps;
-  FfnTileParams g{};
-  g.n_prob = 1, g.act = act, g.F = F, g.z = z;
-  ffn_tile_problem(g.prob[0], F, m, d, 0, 0, 64, NT, 1, a, nullptr);
-  if (!ffn_tile_operand(&maps.a[0], w_gate_up, 2 * F, d, 0, 64) ||
-      !ffn_tile_operand(&maps.b[0], x, m, d, 0, NT))
-    return TF_ERR_CUDA;
-  if (int e = ffn_tile_launch<NT, FFN_GLU>(maps, g, st)) return e;
-  FfnTileParams o{};
-  o.n_prob = 1, o.pdl = 1;
-  ffn_tile_problem(o.prob[0], d, m, F, 0, 0, 128, NT, 1, y, residual);
-  if (!ffn_tile_operand(&maps.a[0], w_down, d, F, 0, 128) ||
-      !ffn_tile_operand(&maps.b[0], a, m, F, 0, NT))
-    return TF_ERR_CUDA;
-  return ffn_tile_launch<NT, FFN_STORE>(maps, o, st);
+template <int MODE>
+int ffn_tile_launch_nt(const void* w, int w_rows, const void* x, int k, FfnTileParams& prm,
+                       cudaStream_t st) {
+  if (prm.T <= 16) return ffn_tile_launch<16, MODE>(w, w_rows, x, k, prm, st);
+  if (prm.T <= 32) return ffn_tile_launch<32, MODE>(w, w_rows, x, k, prm, st);
+  if (prm.T <= 64) return ffn_tile_launch<64, MODE>(w, w_rows, x, k, prm, st);
+  return ffn_tile_launch<128, MODE>(w, w_rows, x, k, prm, st);
 }
 
-#ifndef TFB_TILE_FWD_MAX
-#define TFB_TILE_FWD_MAX 128
+// Whether a forward product of J outputs (`rows` a tile of the tile kernel,
+// `pair_cols` a tile of the pair kernel) and T tokens goes to the tile kernel.
+// Both kernels are bound by the loads of an SM (some 50 bytes a cycle) once
+// their SMs are busy: a k-block costs an SM of the pair kernel 32 KB and each
+// tile of the tile kernel 16 KB for its weights and 128 bytes a token.
+bool ffn_use_tiles(int J, int T, int rows, int pair_cols) {
+#ifdef TFB_FORCE_TILES
+  return TFB_FORCE_TILES;
 #endif
-#ifndef TFB_TILE_BWD_MAX
-#define TFB_TILE_BWD_MAX 0
-#endif
-bool ffn_fwd_tiles(int m, int d, int F) { return m <= TFB_TILE_FWD_MAX; }
-bool ffn_bwd_tiles(int m, int d, int F) { return m <= TFB_TILE_BWD_MAX; }
+  const long long tiles = (long long)((J + rows - 1) / rows) * ((T + 127) / 128);
+  const long long pairs = (long long)((J + pair_cols - 1) / pair_cols) * ((T + 255) / 256);
+  const int n_pairs = std::max(1, g_pair_clusters[current_device()]);
+  const double tile_cost = (double)tiles * (128 + std::min(T, 128)) / 256 / (2 * n_pairs);
+  return tile_cost < (double)((pairs + n_pairs - 1) / n_pairs);
+}
 
 int ffn_check(int m, int d_model, int d_ff, int act) {
   if (m < 0 || d_model < 0 || d_ff < 0) return TF_ERR_INVALID_ARG;
@@ -1174,26 +1139,37 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
     return TF_ERR_MISALIGNED;
   if (int st = ensure_device_setup()) return st;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (ffn_fwd_tiles(m, d_model, d_ff)) {
-    const auto run = m <= 16   ? ffn_tile_fwd<16>
-                     : m <= 32 ? ffn_tile_fwd<32>
-                     : m <= 64 ? ffn_tile_fwd<64>
-                               : ffn_tile_fwd<128>;
-    return run(x, w_gate_up, w_down, residual, a, z, y, m, d_model, d_ff, act, st);
+  // a = act(x Wg^T) * (x Wu^T)
+  if (ffn_use_tiles(d_ff, m, 64, 128)) {
+    FfnTileParams g{};
+    g.J = d_ff, g.T = m, g.act = act;
+    g.out = static_cast<__nv_bfloat16*>(a);
+    g.z = z;
+    if (int e = ffn_tile_launch_nt<FFN_GLU>(w_gate_up, 2 * d_ff, x, d_model, g, st)) return e;
+  } else {
+    FfnMaps maps;
+    FfnPairParams prm{};
+    prm.n_prob = 1;
+    prm.F = d_ff;
+    prm.a = static_cast<__nv_bfloat16*>(a);
+    prm.z = z;
+    ffn_problem(prm.prob[0], m, 2 * d_ff, d_model, 0, 0, nullptr, nullptr);
+    prm.prob[0].n_nblk = (d_ff + 127) / 128;  // 128 gate and 128 up rows a tile
+    prm.prob[0].n_tiles = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
+    if (!ffn_operand(&maps.a[0], x, m, d_model, 0) ||
+        !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0))
+      return TF_ERR_CUDA;
+    if (int e = ffn_pair_launch_act<FFN_GLU>(act, maps, prm, st)) return e;
+  }
+  // y = a Wd^T (+ residual)
+  if (ffn_use_tiles(d_model, m, 128, 256)) {
+    FfnTileParams o{};
+    o.J = d_model, o.T = m, o.pdl = 1;
+    o.out = static_cast<__nv_bfloat16*>(y);
+    o.residual = static_cast<const __nv_bfloat16*>(residual);
+    return ffn_tile_launch_nt<FFN_STORE>(w_down, d_model, a, d_ff, o, st);
   }
   FfnMaps maps;
-  FfnPairParams prm{};
-  prm.n_prob = 1;
-  prm.F = d_ff;
-  prm.a = static_cast<__nv_bfloat16*>(a);
-  prm.z = z;
-  ffn_problem(prm.prob[0], m, 2 * d_ff, d_model, 0, 0, nullptr, nullptr);
-  prm.prob[0].n_nblk = (d_ff + 127) / 128;  // 128 gate and 128 up rows a tile
-  prm.prob[0].n_tiles = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
-  if (!ffn_operand(&maps.a[0], x, m, d_model, 0) ||
-      !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0))
-    return TF_ERR_CUDA;
-  if (int e = ffn_pair_launch_act<FFN_GLU>(act, maps, prm, st)) return e;
   FfnPairParams down{};
   down.n_prob = 1;
   ffn_problem(down.prob[0], m, d_model, d_ff, 0, 0, y, residual);
@@ -1230,40 +1206,6 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
   if (int e = ensure_device_setup()) return e;
   __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(workspace);
   __nv_bfloat16* a = dz + (size_t)m * 2 * d_ff;
-  if (ffn_bwd_tiles(m, d_model, d_ff)) {
-    FfnMaps maps;
-    FfnTileParams g{};
-    g.n_prob = 1, g.act = act, g.F = d_ff, g.z = const_cast<float*>(z), g.dz = dz;
-    ffn_tile_problem(g.prob[0], d_ff, m, d_model, 1, 0, 128, 128, 1, a, nullptr);
-    if (!ffn_tile_operand(&maps.a[0], w_down, d_ff, d_model, 1, 0) ||
-        !ffn_tile_operand(&maps.b[0], dy, m, d_model, 0, 128))
-      return TF_ERR_CUDA;
-    if (int e = ffn_tile_launch<128, FFN_DGLU>(maps, g, st)) return e;
-    FfnTileParams o{};
-    o.pdl = 1;
-    bool ok = true;
-    // an output's innermost index is A's row
-    if (dx) {
-      const int i = o.n_prob++;
-      ffn_tile_problem(o.prob[i], d_model, m, 2 * d_ff, 1, 0, 128, 128, 1, dx, nullptr);
-      ok = ok && ffn_tile_operand(&maps.a[i], w_gate_up, d_model, 2 * d_ff, 1, 0) &&
-           ffn_tile_operand(&maps.b[i], dz, m, 2 * d_ff, 0, 128);
-    }
-    if (dw_gate_up) {
-      const int i = o.n_prob++;
-      ffn_tile_problem(o.prob[i], d_model, 2 * d_ff, m, 1, 1, 128, 128, 1, dw_gate_up, nullptr);
-      ok = ok && ffn_tile_operand(&maps.a[i], x, d_model, m, 1, 0) &&
-           ffn_tile_operand(&maps.b[i], dz, 2 * d_ff, m, 1, 0);
-    }
-    if (dw_down) {
-      const int i = o.n_prob++;
-      ffn_tile_problem(o.prob[i], d_ff, d_model, m, 1, 1, 128, 128, 0, dw_down, nullptr);
-      ok = ok && ffn_tile_operand(&maps.a[i], a, d_ff, m, 1, 0) &&
-           ffn_tile_operand(&maps.b[i], dy, d_model, m, 1, 0);
-    }
-    if (!ok) return TF_ERR_CUDA;
-    return ffn_tile_launch<128, FFN_STORE>(maps, o, st);
-  }
   FfnMaps maps;
   FfnPairParams prm{};
   prm.n_prob = 1;
