@@ -50,41 +50,39 @@ __device__ __forceinline__ float ffn_phi(float g, float& E) {
   return g < 0.0f ? q : 1.0f - q;
 }
 
-// act(g).  The quotients use __fdividef (2 ulp; 0 for a divisor above 2^126,
-// where the result is below 1e-36): a full fp32 division is a dozen
-// instructions, and the epilogue of a short product is bound by its own.
-template <int ACT>
-__device__ __forceinline__ float ffn_act(float g) {
-  if constexpr (ACT == FFN_ACT_SILU) {
-    return __fdividef(g, 1.0f + __expf(-g));
-  } else if constexpr (ACT == FFN_ACT_GELU) {
-    float E;
-    return g * ffn_phi(g, E);
-  } else {
-    // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), v = sqrt(2/pi) (g + 0.044715 g^3)
-    const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    return __fdividef(g, 1.0f + __expf(-2.0f * v));
-  }
+// 1 / (1 + exp(-v)).  __fdividef (2 ulp) gives 0 for a divisor above 2^126, where
+// the quotient is below 1e-37: a full fp32 division is a dozen instructions, and
+// the epilogue of a short product is bound by its own.
+__device__ __forceinline__ float ffn_sigmoid(float v) {
+  return __fdividef(1.0f, 1.0f + __expf(-v));
 }
 
-// act(g), the same bits as ffn_act's, and act'(g)
+// act(g) and act'(g).  The forward pass and the backward pass, which computes a
+// again, take the value from the same expression: the same bits.
 template <int ACT>
 __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope) {
   if constexpr (ACT == FFN_ACT_SILU) {
-    value = ffn_act<ACT>(g);
-    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-    slope = s * (1.0f + g * (1.0f - s));
+    const float s = ffn_sigmoid(g);
+    value = g * s;
+    slope = fmaf(value, 1.0f - s, s);
   } else if constexpr (ACT == FFN_ACT_GELU) {
     float E;
     const float phi = ffn_phi(g, E);
     value = g * phi;
     slope = fmaf(g * 0.39894228040143268f, E, phi);
   } else {
-    value = ffn_act<ACT>(g);
-    const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * v));
-    slope = s + g * s * (1.0f - s) * 2.0f * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
+    // (1 + tanh v) / 2 = sigmoid(2 v), v = sqrt(2 / pi) (g + 0.044715 g^3)
+    const float g2 = g * g;
+    const float s = ffn_sigmoid(1.5957691216057308f * g * fmaf(0.044715f, g2, 1.0f));
+    value = g * s;
+    slope = fmaf(value * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f, g2, 1.0f), s);
   }
+}
+template <int ACT>
+__device__ __forceinline__ float ffn_act(float g) {
+  float value, slope;
+  ffn_act_grad<ACT>(g, value, slope);
+  return value;
 }
 
 __device__ __forceinline__ float ffn_act_rt(int act, float g) {  // (uniform branches)
