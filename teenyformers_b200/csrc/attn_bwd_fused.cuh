@@ -43,9 +43,6 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32
       "r"(smem_src), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ void bulk_wait_group_read1() {
-  asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-}
 // AND of `v` over the `nthreads` threads of named barrier `id` (all of them
 // get the same answer, so they take the same branch afterwards).
 __device__ __forceinline__ bool named_bar_and(int id, int nthreads, bool v) {

@@ -132,7 +132,47 @@ struct FfnPairParams {
 
 struct FfnMaps {
   CUtensorMap a[kFfnMaxProblems], b[kFfnMaxProblems];
+  // FFN_STORE: each product's output; FFN_GLU: a, z; FFN_DGLU: a, dz, z
+  CUtensorMap out[3];
 };
+
+// The pair kernel's shared memory: a ring of 32 KB stages and 8 KB a warp for
+// the epilogue (six stages and 4 KB measured the same main loop).
+constexpr int kFfnStages = 5;
+constexpr int kFfnEpiWarps = 8;
+constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
+constexpr int kFfnEpiBytes = 8192;  // a warp's
+
+struct FfnPairCfg {
+  static constexpr int A_BYTES = 128 * kGemmBK * 2;  // this CTA's 128 rows of A
+  static constexpr int B_BYTES = 128 * kGemmBK * 2;  // and of B
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int OFF_EPI = kFfnStages * STAGE_BYTES;
+  static constexpr int OFF_BAR = OFF_EPI + kFfnEpiWarps * kFfnEpiBytes;
+  static constexpr int SMEM_ALLOC = OFF_BAR + 512 + 1024;
+  static constexpr int TM_COLS = 2 * kGemmBN;
+};
+static_assert(FfnPairCfg::SMEM_ALLOC <= 232448, "the pair kernel's shared memory exceeds the limit");
+
+enum {
+  GB_FULL = 0,
+  GB_EMPTY = kFfnStages,
+  GB_AFULL = 2 * kFfnStages,
+  GB_AEMPTY = 2 * kFfnStages + 2,
+  GB_DRAIN = 2 * kFfnStages + 4,
+  GB_Z = 2 * kFfnStages + 5,  // FFN_DGLU: two for each epilogue warp
+  GB_COUNT = GB_Z + 2 * kFfnEpiWarps
+};
+static_assert((GB_COUNT + 1) * 8 <= 512, "barriers");
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int c0,
+                                             int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_src), "r"(c0), "r"(c1)
+      : "memory");
+}
 
 // The i-th tile of a pair, in the concatenated list of all products' tiles
 // (those with the longer K first); -1 at the end.  Heavy tiles go round robin;
@@ -174,16 +214,9 @@ __device__ __forceinline__ int ffn_tile(const FfnPairParams& p, int t, int& mb, 
   return k;
 }
 
-// Stages a warp's 32 rows x 32 columns of fp32 (row = lane) as 128-byte rows of
-// 16-byte chunks XOR-swizzled by row.
-__device__ __forceinline__ void ffn_stage32(uint32_t stg, const uint32_t (&r)[32], int lane) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    gemm_sts128(stg + lane * 128 + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2],
-                r[4 * j + 3]);
-}
-// ... and reads them back 4 columns a lane: iteration `it` gives row it * 4 +
-// lane / 8, columns 4 (lane % 8)..
+// Reads 32 staged rows of 32 fp32 (128-byte rows, 16-byte chunks XOR-swizzled by
+// row) 4 columns a lane: iteration `it` gives row it * 4 + lane / 8, columns
+// 4 (lane % 8)..
 __device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) {
   const int rr = it * 4 + (lane >> 3);
   const uint4 v = gemm_lds128(stg + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
@@ -191,29 +224,48 @@ __device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) 
                      __uint_as_float(v.w));
 }
 
-constexpr int kFfnEpiWarps = 8;
-constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
-constexpr int kFfnEpiBytes = GemmPairCfg::EPI_WARP_BYTES * 4 / kFfnEpiWarps;  // a warp's staging
-
 // Epilogue of one accumulator tile for one warp: TMEM columns acc.. of this
 // warp's lane quarter, output rows row0..row0+31, column block nb, the half
 // `hf` of the tile's columns (two warps share a lane quarter: the epilogue of
 // a tile with a short K, bound by its instructions, then takes half the time).
-// Values pass through the warp's 4 KB of shared memory, so that global loads
-// and stores are whole 64- or 128-byte row segments.  wait_acc() blocks until
-// the accumulator is complete; what does not depend on it is loaded first.
+// A lane works on its own row.  Values leave through the warp's shared memory
+// `stg` as bulk tensor stores (and FFN_DGLU's z comes in as bulk tensor loads):
+// with global loads and stores of the lanes, the load/store unit bound the
+// epilogues of short products (FFN_DGLU 17 us a tile).  Bulk stores clip rows
+// past M and columns past the output's.  wait_acc() blocks until the
+// accumulator is complete; what does not depend on it is loaded first.
+// zbar: this warp's two barriers, zn: its z chunks so far (FFN_DGLU).
 template <int MODE, int ACT, class Wait, class Release>
 __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
-                                                  uint32_t acc, int row0, int nb, int hf, int lane,
-                                                  uint32_t stg, Wait&& wait_acc,
+                                                  const FfnMaps& maps, int k, uint32_t acc,
+                                                  int row0, int nb, int hf, int lane, uint32_t stg,
+                                                  uint32_t zbar, int& zn, Wait&& wait_acc,
                                                   Release&& release_acc) {
   if (row0 >= q.M) {
     if (!wait_acc()) return false;
     release_acc();
     return true;
   }
-  const int rows_valid = q.M - row0;
-  const int r4 = lane >> 3, c4 = (lane & 7) * 4;  // ffn_unstage32: row in a group of 4, column
+  // the two 4 KB halves of stg in turn: the half is free once the store
+  // before last has read it
+  int half = 0;
+  auto next_half = [&]() {
+    if (lane == 0) bulk_wait_group_read1();
+    __syncwarp();
+    half ^= 1;
+    return stg + half * 4096;
+  };
+  // a lane's 32 fp32 as a 128-byte row, chunks XOR-swizzled by row
+  auto stage32 = [&](uint32_t buf, const uint32_t (&r)[32]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      gemm_sts128(buf + lane * 128 + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2],
+                  r[4 * j + 3]);
+  };
+  auto staged = [&]() {  // this warp's shared memory writes, before a bulk store reads them
+    fence_proxy_async_smem();
+    __syncwarp();
+  };
   if constexpr (MODE == FFN_GLU) {
     // columns 0..127 of the accumulator are gate, 128..255 up of outputs 128 nb..
     if (!wait_acc()) return false;
@@ -226,100 +278,116 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_wait_ld();
       if (hh == 1) release_acc();
       // a: 64-byte rows of 16-byte chunks, XOR-swizzled by pairs of rows
+      const uint32_t ab = next_half();
 #pragma unroll
       for (int jc = 0; jc < 4; ++jc) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int k = 8 * jc + 2 * e;
-          w[e] = pack_bf16x2(ffn_act<ACT>(__uint_as_float(gr[k])) * __uint_as_float(ur[k]),
-                             ffn_act<ACT>(__uint_as_float(gr[k + 1])) * __uint_as_float(ur[k + 1]));
+          const int i = 8 * jc + 2 * e;
+          w[e] = pack_bf16x2(ffn_act<ACT>(__uint_as_float(gr[i])) * __uint_as_float(ur[i]),
+                             ffn_act<ACT>(__uint_as_float(gr[i + 1])) * __uint_as_float(ur[i + 1]));
         }
-        gemm_sts128(stg + lane * 64 + ((jc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+        gemm_sts128(ab + lane * 64 + ((jc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
       }
-      __syncwarp();
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int rr = it * 8 + (lane >> 2), jc = lane & 3;
-        const uint4 v = gemm_lds128(stg + rr * 64 + ((jc ^ ((rr >> 1) & 3)) << 4));
-        if (rr < rows_valid && col0 + jc * 8 < p.F)
-          *reinterpret_cast<uint4*>(p.a + (long long)(row0 + rr) * p.F + col0 + jc * 8) = v;
-      }
-      __syncwarp();
+      staged();
+      const bool inside = lane == 0 && col0 < p.F;  // (a box wholly past the edge is not stored)
+      if (inside) tma_store_2d(&maps.out[0], ab, col0, row0);
+      if (lane == 0) bulk_commit_group();
       if (p.z) {
-        for (int half = 0; half < 2; ++half) {
-          if (half == 0)
-            ffn_stage32(stg, gr, lane);
-          else
-            ffn_stage32(stg, ur, lane);
-          __syncwarp();
-          float* z_row0 = p.z + (long long)row0 * 2 * p.F + (half ? p.F : 0) + col0 + c4;
-#pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const float4 v = ffn_unstage32(stg, it, lane);
-            const int rr = it * 4 + r4;
-            if (rr < rows_valid && col0 + c4 < p.F)
-              *reinterpret_cast<float4*>(z_row0 + (long long)rr * 2 * p.F) = v;
-          }
-          __syncwarp();
-        }
+        uint32_t zb = next_half();
+        stage32(zb, gr);
+        staged();
+        if (inside) tma_store_3d(&maps.out[1], zb, col0, 0, row0);
+        if (lane == 0) bulk_commit_group();
+        zb = next_half();
+        stage32(zb, ur);
+        staged();
+        if (inside) tma_store_3d(&maps.out[1], zb, col0, 1, row0);
+        if (lane == 0) bulk_commit_group();
       }
     }
   } else if constexpr (MODE == FFN_DGLU) {
-    float4 g[8], u[8];
-    auto load_z = [&](int c) {
-      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int rr = it * 4 + r4;
-        if (rr < rows_valid && col < p.F) {
-          const float* zr = p.z + (long long)(row0 + rr) * 2 * p.F + col;
-          g[it] = *reinterpret_cast<const float4*>(zr);
-          u[it] = *reinterpret_cast<const float4*>(zr + p.F);
-        }
-      }
+    // chunks of 16 columns through the two halves: z comes in (gate 2 KB, up
+    // 2 KB: 64-byte rows), dg, du and a go out (1 KB each: 32-byte rows)
+    const int col_h = nb * kGemmBN + hf * 128;
+    auto load_z = [&](int c) {  // (lane 0) chunk c of this tile into half c % 2
+      const uint32_t dst = stg + (c & 1) * 4096, bar = zbar + (c & 1) * 8;
+      mbar_arrive_expect_tx(bar, 4096);
+      tma_load_3d(dst, &maps.out[2], bar, col_h + c * 16, 0, row0);
+      tma_load_3d(dst + 2048, &maps.out[2], bar, col_h + c * 16, 1, row0);
     };
-    load_z(0);
-    if (!wait_acc()) return false;
-    for (int c = 0; c < 4; ++c) {
-      uint32_t r[32];
-      tmem_ld32(acc + hf * 128 + c * 32, r);
+    if (lane == 0) {
+      bulk_wait_group_read0();  // the tile before
+      load_z(0);
+      load_z(1);
+    }
+    __syncwarp();
+    // a load of z needs nothing of the other roles: its wait does not look at
+    // their giving up, and both loads have landed when this warp does
+    auto wait_z = [&](int i) {
+      return mbar_wait_warp(zbar + (i & 1) * 8, (i >> 1) & 1, nullptr, 927);
+    };
+    if (!wait_acc()) {
+      (void)wait_z(zn);
+      (void)wait_z(zn + 1);
+      return false;
+    }
+    for (int c = 0; c < 8; ++c, ++zn) {  // (chunk zn of this warp is in half zn % 2 = c % 2)
+      uint32_t r[16];
+      tmem_ld16(acc + hf * 128 + c * 16, r);
       tmem_wait_ld();
-      if (c == 3) release_acc();
-      ffn_stage32(stg, r, lane);
-      __syncwarp();
-      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
+      if (c == 7) release_acc();
+      if (!wait_z(zn)) return false;
+      const uint32_t buf = stg + (c & 1) * 4096;
+      uint32_t dg[8], du[8], av[8];
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const float4 d4 = ffn_unstage32(stg, it, lane);
-        const int rr = it * 4 + r4;
-        if (rr < rows_valid && col < p.F) {
-          const float d[4] = {d4.x, d4.y, d4.z, d4.w};
-          const float gv[4] = {g[it].x, g[it].y, g[it].z, g[it].w};
-          const float uv[4] = {u[it].x, u[it].y, u[it].z, u[it].w};
-          float dg[4], du[4], av[4];
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+        const uint4 g4 = gemm_lds128(at), u4 = gemm_lds128(at + 2048);
+        const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+        float x[4], y[4], w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float value, slope;
-            ffn_act_grad<ACT>(gv[e], value, slope);
-            av[e] = value * uv[e];
-            du[e] = d[e] * value;
-            dg[e] = d[e] * uv[e] * slope;
-          }
-          const long long row = row0 + rr;
-          *reinterpret_cast<uint2*>(p.dz + row * 2 * p.F + col) =
-              make_uint2(pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3]));
-          *reinterpret_cast<uint2*>(p.dz + row * 2 * p.F + p.F + col) =
-              make_uint2(pack_bf16x2(du[0], du[1]), pack_bf16x2(du[2], du[3]));
-          *reinterpret_cast<uint2*>(p.a + row * p.F + col) =
-              make_uint2(pack_bf16x2(av[0], av[1]), pack_bf16x2(av[2], av[3]));
+        for (int e = 0; e < 4; ++e) {
+          float value, slope;
+          const float d = __uint_as_float(r[4 * j + e]), u = __uint_as_float(uw[e]);
+          ffn_act_grad<ACT>(__uint_as_float(gw[e]), value, slope);
+          w[e] = value * u;
+          y[e] = d * value;
+          x[e] = d * u * slope;
+        }
+        dg[2 * j] = pack_bf16x2(x[0], x[1]), dg[2 * j + 1] = pack_bf16x2(x[2], x[3]);
+        du[2 * j] = pack_bf16x2(y[0], y[1]), du[2 * j + 1] = pack_bf16x2(y[2], y[3]);
+        av[2 * j] = pack_bf16x2(w[0], w[1]), av[2 * j + 1] = pack_bf16x2(w[2], w[3]);
+      }
+      __syncwarp();  // every lane has read its z
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t at = buf + lane * 32 + ((j ^ ((lane >> 2) & 1)) << 4);
+        gemm_sts128(at, dg[4 * j], dg[4 * j + 1], dg[4 * j + 2], dg[4 * j + 3]);
+        gemm_sts128(at + 1024, du[4 * j], du[4 * j + 1], du[4 * j + 2], du[4 * j + 3]);
+        gemm_sts128(at + 2048, av[4 * j], av[4 * j + 1], av[4 * j + 2], av[4 * j + 3]);
+      }
+      staged();
+      if (lane == 0) {
+        const int col = col_h + c * 16;
+        if (col < p.F) {
+          tma_store_3d(&maps.out[1], buf, col, 0, row0);
+          tma_store_3d(&maps.out[1], buf + 1024, col, 1, row0);
+          tma_store_2d(&maps.out[0], buf + 2048, col, row0);
+        }
+        bulk_commit_group();
+        if (c < 6) {
+          bulk_wait_group_read0();
+          load_z(c + 2);
         }
       }
-      if (c < 3) load_z(c + 1);
       __syncwarp();
     }
   } else if (q.residual) {
     // the residual is added to the fp32 product: one rounding
+    const int r4 = lane >> 3, c4 = (lane & 7) * 4;  // ffn_unstage32: row in a group of 4, column
+    const int rows_valid = q.M - row0;
     uint2 res[8];
     auto load_res = [&](int c) {
       const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
@@ -337,7 +405,7 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_ld32(acc + hf * 128 + c * 32, r);
       tmem_wait_ld();
       if (c == 3) release_acc();
-      ffn_stage32(stg, r, lane);
+      stage32(stg, r);
       __syncwarp();
       const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
 #pragma unroll
@@ -365,21 +433,23 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_ld32(acc + hf * 128 + c * 64 + 32, r1);
       tmem_wait_ld();
       if (c == 1) release_acc();
+      const uint32_t buf = next_half();
 #pragma unroll
       for (int jc = 0; jc < 8; ++jc) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int k = 8 * jc + 2 * e;
-          w[e] = pack_bf16x2(__uint_as_float(k < 32 ? r0[k] : r1[k - 32]),
-                             __uint_as_float(k + 1 < 32 ? r0[k + 1] : r1[k + 1 - 32]));
+          const int i = 8 * jc + 2 * e;
+          w[e] = pack_bf16x2(__uint_as_float(i < 32 ? r0[i] : r1[i - 32]),
+                             __uint_as_float(i + 1 < 32 ? r0[i + 1] : r1[i + 1 - 32]));
         }
-        gemm_sts128(stg + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+        gemm_sts128(buf + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
       }
-      __syncwarp();
-      gemm_store_rows64(stg, q.out + (long long)row0 * q.N + col0, nullptr, q.N, lane, rows_valid,
-                        q.N - col0);
-      __syncwarp();
+      staged();
+      if (lane == 0) {
+        if (col0 < q.N) tma_store_2d(&maps.out[k], buf, col0, row0);
+        bulk_commit_group();
+      }
     }
   }
   return true;
@@ -394,13 +464,13 @@ template <int MODE, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     ffn_pair_kernel(const __grid_constant__ FfnMaps maps,
                     const __grid_constant__ FfnPairParams p) {
-  using C = GemmPairCfg;
+  using C = FfnPairCfg;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;  // same offset in both CTAs
   uint8_t* sptr = smem_raw + (sbase - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sptr + C::OFF_BAR);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PB_COUNT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + GB_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -409,15 +479,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   const int pair = (int)cluster_id_x(), n_pairs = (int)cluster_count_x();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
-      mbar_init(bar(PB_FULL + s), 1);
-      mbar_init(bar(PB_EMPTY + s), 1);
+    for (int s = 0; s < kFfnStages; ++s) {
+      mbar_init(bar(GB_FULL + s), 1);
+      mbar_init(bar(GB_EMPTY + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(PB_AFULL + b), 1);
-      mbar_init(bar(PB_AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
+      mbar_init(bar(GB_AFULL + b), 1);
+      mbar_init(bar(GB_AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
     }
-    mbar_init(bar(PB_DRAIN), 1);
+    mbar_init(bar(GB_DRAIN), 1);
+    for (int i = 0; i < 2 * kFfnEpiWarps; ++i) mbar_init(bar(GB_Z + i), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -429,6 +500,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     tma_prefetch_desc(&maps.a[lane]);
     tma_prefetch_desc(&maps.b[lane]);
   }
+  if (warp == 2 && lane < (MODE == FFN_STORE ? (p.prob[0].residual ? 0 : p.n_prob)
+                           : MODE == FFN_DGLU ? 3 : p.z ? 2 : 1))
+    tma_prefetch_desc(&maps.out[lane]);
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers initialised before any remote signal
   tc_fence_after();
@@ -437,7 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
 
   if (warp == 0) {
     // ===================== TMA producer (both CTAs) =====================
-    const uint32_t full0 = mapa_cta(bar(PB_FULL), 0);  // the even CTA's FULL[0]
+    const uint32_t full0 = mapa_cta(bar(GB_FULL), 0);  // the even CTA's FULL[0]
     int g = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -453,13 +527,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
                                      : nb * 256 + (int)crank * 128;
       const bool a_mn = q.a_mn, b_mn = q.b_mn;
       for (int kb = 0; kb < q.n_kblk; ++kb, ++g) {
-        const int s = g % kPairStages, u = g / kPairStages;
-        if (u > 0) ok = mbar_wait_warp(bar(PB_EMPTY + s), (u - 1) & 1, abort_flag, 921);
+        const int s = g % kFfnStages, u = g / kFfnStages;
+        if (u > 0) ok = mbar_wait_warp(bar(GB_EMPTY + s), (u - 1) & 1, abort_flag, 921);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t sa = sbase + s * C::STAGE_BYTES;
           const uint32_t fb = full0 + s * 8;
-          if (leader) mbar_arrive_expect_tx(bar(PB_FULL + s), 2 * C::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(bar(GB_FULL + s), 2 * C::STAGE_BYTES);
           if (a_mn) {
             tma_load_2d_pair(sa, tm_a, fb, m0, kb * kGemmBK);
             tma_load_2d_pair(sa + 8192, tm_a, fb, m0 + 64, kb * kGemmBK);
@@ -479,9 +553,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     if (!ok) {
       if (leader) {
         // the last copies counted on each stage (both CTAs') land first
-        for (int s = 0; s < kPairStages; ++s) {
-          const int n_s = g > s ? (g - s - 1) / kPairStages + 1 : 0;
-          if (n_s) (void)mbar_wait(bar(PB_FULL + s), (n_s - 1) & 1, nullptr, 922);
+        for (int s = 0; s < kFfnStages; ++s) {
+          const int n_s = g > s ? (g - s - 1) / kFfnStages + 1 : 0;
+          if (n_s) (void)mbar_wait(bar(GB_FULL + s), (n_s - 1) & 1, nullptr, 922);
         }
       } else {
         // the odd CTA cannot see the even CTA's barrier: give copies in flight
@@ -505,13 +579,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
         const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
         const int b = i & 1, use = i >> 1;
-        if (use > 0) ok = mbar_wait_warp(bar(PB_AEMPTY + b), (use - 1) & 1, abort_flag, 923);
+        if (use > 0) ok = mbar_wait_warp(bar(GB_AEMPTY + b), (use - 1) & 1, abort_flag, 923);
         if (!ok) break;
         tc_fence_after();
         const uint32_t acc = tmem + b * kGemmBN;
         for (int kb = 0; kb < n_kblk; ++kb, ++g) {
-          const int s = g % kPairStages;
-          ok = mbar_wait_warp(bar(PB_FULL + s), (g / kPairStages) & 1, abort_flag, 924);
+          const int s = g % kFfnStages;
+          ok = mbar_wait_warp(bar(GB_FULL + s), (g / kFfnStages) & 1, abort_flag, 924);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -520,34 +594,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
             for (int kk = 0; kk < kGemmBK / 16; ++kk)
               mma_ss_pair(acc, desc_adv(da0, off + kk * a_step), desc_adv(db0, off + kk * b_step),
                           idesc, (kb | kk) != 0 ? 1u : 0u);
-            tc_commit_pair_mc(bar(PB_EMPTY + s), 0x3);  // the stage is free in both CTAs
+            tc_commit_pair_mc(bar(GB_EMPTY + s), 0x3);  // the stage is free in both CTAs
           }
           __syncwarp();
         }
         if (!ok) break;
-        if (elect_one()) tc_commit_pair_mc(bar(PB_AFULL + b), 0x3);
+        if (elect_one()) tc_commit_pair_mc(bar(GB_AFULL + b), 0x3);
         __syncwarp();
       }
       // every pair MMA has completed before either CTA frees TMEM or exits
-      if (elect_one()) tc_commit_pair(bar(PB_DRAIN));
+      if (elect_one()) tc_commit_pair(bar(GB_DRAIN));
       __syncwarp();
-      (void)mbar_wait(bar(PB_DRAIN), 0, nullptr, 925);
+      (void)mbar_wait(bar(GB_DRAIN), 0, nullptr, 925);
     }
   } else {
     // ===================== epilogue (both CTAs) =========================
     const int quarter = warp & 3, hf = (warp - 2) >> 2;
     const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * kFfnEpiBytes;
-    const uint32_t aempty0 = mapa_cta(bar(PB_AEMPTY), 0);
+    const uint32_t aempty0 = mapa_cta(bar(GB_AEMPTY), 0);
+    int zn = 0;
     for (int i = 0;; ++i) {
       const int t = ffn_next(p, pair, n_pairs, i);
       if (t < 0) break;
       int mb, nb;
-      const FfnProblem& q = p.prob[ffn_tile(p, t, mb, nb)];
+      const int k = ffn_tile(p, t, mb, nb);
+      const FfnProblem& q = p.prob[k];
       const int b = i & 1, use = i >> 1;
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * kGemmBN;
       const int row0 = mb * 256 + (int)crank * 128 + quarter * 32;
       auto wait_acc = [&]() {
-        const bool ok = mbar_wait_warp(bar(PB_AFULL + b), use & 1, abort_flag, 926);
+        const bool ok = mbar_wait_warp(bar(GB_AFULL + b), use & 1, abort_flag, 926);
         tc_fence_after();
         return ok;
       };
@@ -556,9 +632,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
       };
-      if (!ffn_epilogue_warp<MODE, ACT>(p, q, acc, row0, nb, hf, lane, stg, wait_acc, release_acc))
+      if (!ffn_epilogue_warp<MODE, ACT>(p, q, maps, k, acc, row0, nb, hf, lane, stg,
+                                        bar(GB_Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
         break;
     }
+    if (lane == 0) bulk_wait_group0();  // the stores, before the shared memory goes away
+    __syncwarp();
   }
 
   tc_fence_before();

@@ -144,13 +144,13 @@ int ensure_device_setup() {
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_SWIGLU>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_QKV_ROPE>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_PUSH>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, GemmPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
 #define TFB_TILE_SET(NT)                                                            \
   set((const void*)ffn_tile_kernel<NT, FFN_GLU>, TileCfg<NT>::SMEM_ALLOC);          \
   set((const void*)ffn_tile_kernel<NT, FFN_STORE>, TileCfg<NT>::SMEM_ALLOC)
@@ -1028,6 +1028,26 @@ bool ffn_operand(CUtensorMap* map, const void* base, int mn, int k, int mn_major
                   : make_bf16_2d_map(map, base, k, mn, 128);
 }
 
+// The epilogue's boxes: `cols` x 32 rows of a row-major [m, n] bf16 matrix, and
+// the same of one half of the rows of [m, 2 F] (dims F, 2, m: nothing written
+// past column F of a half).
+bool ffn_box(CUtensorMap* map, const void* base, long long n, long long m, int halves, int cols,
+             CUtensorMapDataType type, CUtensorMapSwizzle swizzle) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t bytes = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)n, 2, (cuuint64_t)m};
+  cuuint64_t strides[2] = {(cuuint64_t)n * bytes, 2 * (cuuint64_t)n * bytes};
+  cuuint32_t box[3] = {(cuuint32_t)cols, 1, 32};
+  cuuint32_t estr[3] = {1, 1, 1};
+  if (!halves) dims[1] = (cuuint64_t)m, box[1] = 32;
+  return enc(map, type, halves ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+constexpr CUtensorMapDataType kBf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+constexpr CUtensorMapDataType kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+
 template <int MODE, int ACT>
 int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
   // products come longest K first; those of the first one's K are the heavy tiles
@@ -1042,8 +1062,13 @@ int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
     prm.bal_rounds = (int)std::min<long long>(
         prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
   ffn_pair_kernel<MODE, ACT>
-      <<<(unsigned)(2 * clusters), kFfnThreads, GemmPairCfg::SMEM_ALLOC, st>>>(maps, prm);
+      <<<(unsigned)(2 * clusters), kFfnThreads, FfnPairCfg::SMEM_ALLOC, st>>>(maps, prm);
   return launch_status();
+}
+
+// FFN_STORE: the i-th product's output [m, n]
+bool ffn_out(FfnMaps* maps, int i, const void* out, int m, int n) {
+  return ffn_box(&maps->out[i], out, n, m, 0, 64, kBf16, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int MODE>
@@ -1157,7 +1182,9 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
     prm.prob[0].n_nblk = (d_ff + 127) / 128;  // 128 gate and 128 up rows a tile
     prm.prob[0].n_tiles = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
     if (!ffn_operand(&maps.a[0], x, m, d_model, 0) ||
-        !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0))
+        !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0) ||
+        !ffn_box(&maps.out[0], a, d_ff, m, 0, 32, kBf16, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        (z && !ffn_box(&maps.out[1], z, d_ff, m, 1, 32, kF32, CU_TENSOR_MAP_SWIZZLE_128B)))
       return TF_ERR_CUDA;
     if (int e = ffn_pair_launch_act<FFN_GLU>(act, maps, prm, st)) return e;
   }
@@ -1173,7 +1200,8 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
   FfnPairParams down{};
   down.n_prob = 1;
   ffn_problem(down.prob[0], m, d_model, d_ff, 0, 0, y, residual);
-  if (!ffn_operand(&maps.a[0], a, m, d_ff, 0) || !ffn_operand(&maps.b[0], w_down, d_model, d_ff, 0))
+  if (!ffn_operand(&maps.a[0], a, m, d_ff, 0) ||
+      !ffn_operand(&maps.b[0], w_down, d_model, d_ff, 0) || !ffn_out(&maps, 0, y, m, d_model))
     return TF_ERR_CUDA;
   return ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, down, st);
 }
@@ -1215,7 +1243,10 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
   prm.dz = dz;
   ffn_problem(prm.prob[0], m, d_ff, d_model, 0, 1, nullptr, nullptr);
   if (!ffn_operand(&maps.a[0], dy, m, d_model, 0) ||
-      !ffn_operand(&maps.b[0], w_down, d_ff, d_model, 1))
+      !ffn_operand(&maps.b[0], w_down, d_ff, d_model, 1) ||
+      !ffn_box(&maps.out[0], a, d_ff, m, 0, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
+      !ffn_box(&maps.out[1], dz, d_ff, m, 1, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
+      !ffn_box(&maps.out[2], z, d_ff, m, 1, 16, kF32, CU_TENSOR_MAP_SWIZZLE_64B))
     return TF_ERR_CUDA;
   if (int e = ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st)) return e;
 
@@ -1227,19 +1258,22 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
     const int i = g.n_prob++;
     ffn_problem(g.prob[i], m, d_model, 2 * d_ff, 0, 1, dx, nullptr);
     ok = ok && ffn_operand(&maps.a[i], dz, m, 2 * d_ff, 0) &&
-         ffn_operand(&maps.b[i], w_gate_up, d_model, 2 * d_ff, 1);
+         ffn_operand(&maps.b[i], w_gate_up, d_model, 2 * d_ff, 1) &&
+         ffn_out(&maps, i, dx, m, d_model);
   };
   if (2 * d_ff >= m) add_dx();
   if (dw_gate_up) {
     const int i = g.n_prob++;
     ffn_problem(g.prob[i], 2 * d_ff, d_model, m, 1, 1, dw_gate_up, nullptr);
     ok = ok && ffn_operand(&maps.a[i], dz, 2 * d_ff, m, 1) &&
-         ffn_operand(&maps.b[i], x, d_model, m, 1);
+         ffn_operand(&maps.b[i], x, d_model, m, 1) &&
+         ffn_out(&maps, i, dw_gate_up, 2 * d_ff, d_model);
   }
   if (dw_down) {
     const int i = g.n_prob++;
     ffn_problem(g.prob[i], d_model, d_ff, m, 1, 1, dw_down, nullptr);
-    ok = ok && ffn_operand(&maps.a[i], dy, d_model, m, 1) && ffn_operand(&maps.b[i], a, d_ff, m, 1);
+    ok = ok && ffn_operand(&maps.a[i], dy, d_model, m, 1) &&
+         ffn_operand(&maps.b[i], a, d_ff, m, 1) && ffn_out(&maps, i, dw_down, d_model, d_ff);
   }
   if (2 * d_ff < m) add_dx();
   if (!ok) return TF_ERR_CUDA;
