@@ -136,34 +136,30 @@ struct FfnMaps {
   CUtensorMap out[3];
 };
 
-// The pair kernel's shared memory: a ring of 32 KB stages and 8 KB a warp for
-// the epilogue (six stages and 4 KB measured the same main loop).
-constexpr int kFfnStages = 5;
 constexpr int kFfnEpiWarps = 8;
 constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
-constexpr int kFfnEpiBytes = 8192;  // a warp's
 
+// The pair kernel's shared memory: a ring of 32 KB stages, and each epilogue
+// warp's part.  Of 8192 x 4096 x 14336, five stages and six take the same time
+// (forward 2.12 ms), four the same but for FFN_GLU's z (+3%), three 7% more.
+template <int MODE>
 struct FfnPairCfg {
+  static constexpr int STAGES = MODE == FFN_DGLU ? 4 : 5;
+  static constexpr int EPI_BYTES = MODE == FFN_DGLU ? 12288 : 8192;  // a warp's
   static constexpr int A_BYTES = 128 * kGemmBK * 2;  // this CTA's 128 rows of A
   static constexpr int B_BYTES = 128 * kGemmBK * 2;  // and of B
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int OFF_EPI = kFfnStages * STAGE_BYTES;
-  static constexpr int OFF_BAR = OFF_EPI + kFfnEpiWarps * kFfnEpiBytes;
+  static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
+  static constexpr int OFF_BAR = OFF_EPI + kFfnEpiWarps * EPI_BYTES;
   static constexpr int SMEM_ALLOC = OFF_BAR + 512 + 1024;
   static constexpr int TM_COLS = 2 * kGemmBN;
+  static_assert(SMEM_ALLOC <= 232448, "the pair kernel's shared memory exceeds the limit");
+  // barriers
+  static constexpr int FULL = 0, EMPTY = STAGES, AFULL = 2 * STAGES, AEMPTY = AFULL + 2,
+                       DRAIN = AEMPTY + 2, Z = DRAIN + 1 /* FFN_DGLU: two a warp */,
+                       COUNT = Z + 2 * kFfnEpiWarps;
+  static_assert((COUNT + 1) * 8 <= 512, "barriers");
 };
-static_assert(FfnPairCfg::SMEM_ALLOC <= 232448, "the pair kernel's shared memory exceeds the limit");
-
-enum {
-  GB_FULL = 0,
-  GB_EMPTY = kFfnStages,
-  GB_AFULL = 2 * kFfnStages,
-  GB_AEMPTY = 2 * kFfnStages + 2,
-  GB_DRAIN = 2 * kFfnStages + 4,
-  GB_Z = 2 * kFfnStages + 5,  // FFN_DGLU: two for each epilogue warp
-  GB_COUNT = GB_Z + 2 * kFfnEpiWarps
-};
-static_assert((GB_COUNT + 1) * 8 <= 512, "barriers");
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int c0,
                                              int c1) {
@@ -308,9 +304,11 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       }
     }
   } else if constexpr (MODE == FFN_DGLU) {
-    // chunks of 16 columns through the two halves: z comes in (gate 2 KB, up
-    // 2 KB: 64-byte rows), dg, du and a go out (1 KB each: 32-byte rows)
+    // chunks of 16 columns: z comes in through the two halves (gate 2 KB, up
+    // 2 KB: 64-byte rows), two chunks ahead; dg, du and a go out through the
+    // third 4 KB (1 KB each: 32-byte rows)
     const int col_h = nb * kGemmBN + hf * 128;
+    const uint32_t out = stg + 8192;
     auto load_z = [&](int c) {  // (lane 0) chunk c of this tile into half c % 2
       const uint32_t dst = stg + (c & 1) * 4096, bar = zbar + (c & 1) * 8;
       mbar_arrive_expect_tx(bar, 4096);
@@ -318,13 +316,12 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tma_load_3d(dst + 2048, &maps.out[2], bar, col_h + c * 16, 1, row0);
     };
     if (lane == 0) {
-      bulk_wait_group_read0();  // the tile before
       load_z(0);
       load_z(1);
     }
     __syncwarp();
     // a load of z needs nothing of the other roles: its wait does not look at
-    // their giving up, and both loads have landed when this warp does
+    // their giving up, and the loads have landed when this warp does
     auto wait_z = [&](int i) {
       return mbar_wait_warp(zbar + (i & 1) * 8, (i >> 1) & 1, nullptr, 927);
     };
@@ -361,9 +358,14 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
         av[2 * j] = pack_bf16x2(w[0], w[1]), av[2 * j + 1] = pack_bf16x2(w[2], w[3]);
       }
       __syncwarp();  // every lane has read its z
+      if (lane == 0) {
+        if (c < 6) load_z(c + 2);
+        bulk_wait_group_read0();  // the chunk before has left `out`
+      }
+      __syncwarp();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t at = buf + lane * 32 + ((j ^ ((lane >> 2) & 1)) << 4);
+        const uint32_t at = out + lane * 32 + ((j ^ ((lane >> 2) & 1)) << 4);
         gemm_sts128(at, dg[4 * j], dg[4 * j + 1], dg[4 * j + 2], dg[4 * j + 3]);
         gemm_sts128(at + 1024, du[4 * j], du[4 * j + 1], du[4 * j + 2], du[4 * j + 3]);
         gemm_sts128(at + 2048, av[4 * j], av[4 * j + 1], av[4 * j + 2], av[4 * j + 3]);
@@ -372,17 +374,12 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       if (lane == 0) {
         const int col = col_h + c * 16;
         if (col < p.F) {
-          tma_store_3d(&maps.out[1], buf, col, 0, row0);
-          tma_store_3d(&maps.out[1], buf + 1024, col, 1, row0);
-          tma_store_2d(&maps.out[0], buf + 2048, col, row0);
+          tma_store_3d(&maps.out[1], out, col, 0, row0);
+          tma_store_3d(&maps.out[1], out + 1024, col, 1, row0);
+          tma_store_2d(&maps.out[0], out + 2048, col, row0);
         }
         bulk_commit_group();
-        if (c < 6) {
-          bulk_wait_group_read0();
-          load_z(c + 2);
-        }
       }
-      __syncwarp();
     }
   } else if (q.residual) {
     // the residual is added to the fp32 product: one rounding
@@ -464,13 +461,13 @@ template <int MODE, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     ffn_pair_kernel(const __grid_constant__ FfnMaps maps,
                     const __grid_constant__ FfnPairParams p) {
-  using C = FfnPairCfg;
+  using C = FfnPairCfg<MODE>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;  // same offset in both CTAs
   uint8_t* sptr = smem_raw + (sbase - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sptr + C::OFF_BAR);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + GB_COUNT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -479,16 +476,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   const int pair = (int)cluster_id_x(), n_pairs = (int)cluster_count_x();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kFfnStages; ++s) {
-      mbar_init(bar(GB_FULL + s), 1);
-      mbar_init(bar(GB_EMPTY + s), 1);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(bar(C::FULL + s), 1);
+      mbar_init(bar(C::EMPTY + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(GB_AFULL + b), 1);
-      mbar_init(bar(GB_AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
+      mbar_init(bar(C::AFULL + b), 1);
+      mbar_init(bar(C::AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
     }
-    mbar_init(bar(GB_DRAIN), 1);
-    for (int i = 0; i < 2 * kFfnEpiWarps; ++i) mbar_init(bar(GB_Z + i), 1);
+    mbar_init(bar(C::DRAIN), 1);
+    for (int i = 0; i < 2 * kFfnEpiWarps; ++i) mbar_init(bar(C::Z + i), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -500,8 +497,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     tma_prefetch_desc(&maps.a[lane]);
     tma_prefetch_desc(&maps.b[lane]);
   }
-  if (warp == 2 && lane < (MODE == FFN_STORE ? (p.prob[0].residual ? 0 : p.n_prob)
-                           : MODE == FFN_DGLU ? 3 : p.z ? 2 : 1))
+  if (warp == 2 && lane < (MODE == FFN_GLU ? 1 + (p.z != nullptr) : MODE == FFN_DGLU ? 3 : p.n_prob))
     tma_prefetch_desc(&maps.out[lane]);
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers initialised before any remote signal
@@ -511,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
 
   if (warp == 0) {
     // ===================== TMA producer (both CTAs) =====================
-    const uint32_t full0 = mapa_cta(bar(GB_FULL), 0);  // the even CTA's FULL[0]
+    const uint32_t full0 = mapa_cta(bar(C::FULL), 0);  // the even CTA's FULL[0]
     int g = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -527,13 +523,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
                                      : nb * 256 + (int)crank * 128;
       const bool a_mn = q.a_mn, b_mn = q.b_mn;
       for (int kb = 0; kb < q.n_kblk; ++kb, ++g) {
-        const int s = g % kFfnStages, u = g / kFfnStages;
-        if (u > 0) ok = mbar_wait_warp(bar(GB_EMPTY + s), (u - 1) & 1, abort_flag, 921);
+        const int s = g % C::STAGES, u = g / C::STAGES;
+        if (u > 0) ok = mbar_wait_warp(bar(C::EMPTY + s), (u - 1) & 1, abort_flag, 921);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t sa = sbase + s * C::STAGE_BYTES;
           const uint32_t fb = full0 + s * 8;
-          if (leader) mbar_arrive_expect_tx(bar(GB_FULL + s), 2 * C::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::STAGE_BYTES);
           if (a_mn) {
             tma_load_2d_pair(sa, tm_a, fb, m0, kb * kGemmBK);
             tma_load_2d_pair(sa + 8192, tm_a, fb, m0 + 64, kb * kGemmBK);
@@ -553,9 +549,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     if (!ok) {
       if (leader) {
         // the last copies counted on each stage (both CTAs') land first
-        for (int s = 0; s < kFfnStages; ++s) {
-          const int n_s = g > s ? (g - s - 1) / kFfnStages + 1 : 0;
-          if (n_s) (void)mbar_wait(bar(GB_FULL + s), (n_s - 1) & 1, nullptr, 922);
+        for (int s = 0; s < C::STAGES; ++s) {
+          const int n_s = g > s ? (g - s - 1) / C::STAGES + 1 : 0;
+          if (n_s) (void)mbar_wait(bar(C::FULL + s), (n_s - 1) & 1, nullptr, 922);
         }
       } else {
         // the odd CTA cannot see the even CTA's barrier: give copies in flight
@@ -579,13 +575,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
         const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
         const int b = i & 1, use = i >> 1;
-        if (use > 0) ok = mbar_wait_warp(bar(GB_AEMPTY + b), (use - 1) & 1, abort_flag, 923);
+        if (use > 0) ok = mbar_wait_warp(bar(C::AEMPTY + b), (use - 1) & 1, abort_flag, 923);
         if (!ok) break;
         tc_fence_after();
         const uint32_t acc = tmem + b * kGemmBN;
         for (int kb = 0; kb < n_kblk; ++kb, ++g) {
-          const int s = g % kFfnStages;
-          ok = mbar_wait_warp(bar(GB_FULL + s), (g / kFfnStages) & 1, abort_flag, 924);
+          const int s = g % C::STAGES;
+          ok = mbar_wait_warp(bar(C::FULL + s), (g / C::STAGES) & 1, abort_flag, 924);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -594,24 +590,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
             for (int kk = 0; kk < kGemmBK / 16; ++kk)
               mma_ss_pair(acc, desc_adv(da0, off + kk * a_step), desc_adv(db0, off + kk * b_step),
                           idesc, (kb | kk) != 0 ? 1u : 0u);
-            tc_commit_pair_mc(bar(GB_EMPTY + s), 0x3);  // the stage is free in both CTAs
+            tc_commit_pair_mc(bar(C::EMPTY + s), 0x3);  // the stage is free in both CTAs
           }
           __syncwarp();
         }
         if (!ok) break;
-        if (elect_one()) tc_commit_pair_mc(bar(GB_AFULL + b), 0x3);
+        if (elect_one()) tc_commit_pair_mc(bar(C::AFULL + b), 0x3);
         __syncwarp();
       }
       // every pair MMA has completed before either CTA frees TMEM or exits
-      if (elect_one()) tc_commit_pair(bar(GB_DRAIN));
+      if (elect_one()) tc_commit_pair(bar(C::DRAIN));
       __syncwarp();
-      (void)mbar_wait(bar(GB_DRAIN), 0, nullptr, 925);
+      (void)mbar_wait(bar(C::DRAIN), 0, nullptr, 925);
     }
   } else {
     // ===================== epilogue (both CTAs) =========================
     const int quarter = warp & 3, hf = (warp - 2) >> 2;
-    const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * kFfnEpiBytes;
-    const uint32_t aempty0 = mapa_cta(bar(GB_AEMPTY), 0);
+    const uint32_t stg = sbase + C::OFF_EPI + (warp - 2) * C::EPI_BYTES;
+    const uint32_t aempty0 = mapa_cta(bar(C::AEMPTY), 0);
     int zn = 0;
     for (int i = 0;; ++i) {
       const int t = ffn_next(p, pair, n_pairs, i);
@@ -623,7 +619,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * kGemmBN;
       const int row0 = mb * 256 + (int)crank * 128 + quarter * 32;
       auto wait_acc = [&]() {
-        const bool ok = mbar_wait_warp(bar(GB_AFULL + b), use & 1, abort_flag, 926);
+        const bool ok = mbar_wait_warp(bar(C::AFULL + b), use & 1, abort_flag, 926);
         tc_fence_after();
         return ok;
       };
@@ -633,7 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
       };
       if (!ffn_epilogue_warp<MODE, ACT>(p, q, maps, k, acc, row0, nb, hf, lane, stg,
-                                        bar(GB_Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
+                                        bar(C::Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
         break;
     }
     if (lane == 0) bulk_wait_group0();  // the stores, before the shared memory goes away

@@ -144,13 +144,13 @@ int ensure_device_setup() {
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_SWIGLU>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_QKV_ROPE>, GemmPairCfg::SMEM_ALLOC);
     set((const void*)gemm_bf16_sm100_pair_kernel<GEMM_EPI_PUSH>, GemmPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, FfnPairCfg::SMEM_ALLOC);
-    set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, FfnPairCfg::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_SILU>, FfnPairCfg<FFN_GLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, FfnPairCfg<FFN_GLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, FfnPairCfg<FFN_GLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, FfnPairCfg<FFN_STORE>::SMEM_ALLOC);
 #define TFB_TILE_SET(NT)                                                            \
   set((const void*)ffn_tile_kernel<NT, FFN_GLU>, TileCfg<NT>::SMEM_ALLOC);          \
   set((const void*)ffn_tile_kernel<NT, FFN_STORE>, TileCfg<NT>::SMEM_ALLOC)
@@ -1062,7 +1062,7 @@ int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
     prm.bal_rounds = (int)std::min<long long>(
         prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
   ffn_pair_kernel<MODE, ACT>
-      <<<(unsigned)(2 * clusters), kFfnThreads, FfnPairCfg::SMEM_ALLOC, st>>>(maps, prm);
+      <<<(unsigned)(2 * clusters), kFfnThreads, FfnPairCfg<MODE>::SMEM_ALLOC, st>>>(maps, prm);
   return launch_status();
 }
 
