@@ -417,6 +417,7 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
     fence_mbar_init();
   }
   __syncthreads();
+  pdl_launch_dependents();  // (the sums behind this kernel wait for it themselves)
   const int nvec = p.cols / 8;
   const bool branch = ALL || p.df, post = ALL || p.w_post, pre = ALL || p.w_pre;
   const bool has_f = ALL || (p.df && (p.w_post || p.gate)), has_dy = ALL || p.dy;
@@ -682,6 +683,7 @@ struct BlockNormSumParams {
 };
 
 __global__ void __launch_bounds__(1024) block_norm_sum_kernel(const BlockNormSumParams p) {
+  pdl_wait();
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int col = (int)blockIdx.x * 32 + lane;

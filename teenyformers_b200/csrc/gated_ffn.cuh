@@ -91,15 +91,6 @@ __device__ __forceinline__ float ffn_act_rt(int act, float g) {  // (uniform bra
   return ffn_act<FFN_ACT_GELU_TANH>(g);
 }
 
-// Programmatic dependent launch: blocks until the kernels this one depends on
-// have completed and their writes are visible (returns at once without PDL).
-__device__ __forceinline__ void pdl_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void pdl_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // ===================================================================== CTA pairs
 enum FfnMode : int {
   FFN_GLU = 0,    // A = x, B = W (gate rows to the even CTA, up rows to the odd one): a (, z)
@@ -121,6 +112,7 @@ struct FfnProblem {
 struct FfnPairParams {
   FfnProblem prob[kFfnMaxProblems];
   int n_prob;
+  int pdl;  // launched with programmatic stream serialization
   // static schedule (ffn_next): T0 tiles of the longer K, then `light` tiles
   int heavy, light, bal_rounds;
   // FFN_GLU / FFN_DGLU
@@ -507,6 +499,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
 
   if (warp == 0) {
     // ===================== TMA producer (both CTAs) =====================
+    // (the other roles' global reads and writes follow a product's loads, or are
+    // of what the kernel before this one does not write)
+    if (p.pdl) pdl_wait();
     const uint32_t full0 = mapa_cta(bar(C::FULL), 0);  // the even CTA's FULL[0]
     int g = 0;
     bool ok = true;

@@ -337,6 +337,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
 }
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch: pdl_wait blocks until the kernels this one depends on
+// have completed and their writes are visible (returns at once without PDL).
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Lets the kernel behind this one be launched before this one ends.
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
 // Small numeric helpers (hardware instructions, not library maths)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float ex2_approx(float x) {

@@ -1008,6 +1008,40 @@ extern "C" int tf_b200_flash_attn2_bwd_bf16_noalloc(const void* q, const void* k
 // ===================================================================== gated feed-forward
 namespace {
 
+// A launch with a cluster of `cluster_y` CTAs (0: as the kernel says) and, with
+// `pdl`, before the kernel ahead of it in the stream ends (the kernel waits for
+// that itself: pdl_wait).
+template <class... Params, class... Args>
+int launch_ex(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st,
+              int cluster_y, int pdl, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (cluster_y) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1;
+    attr[n].val.clusterDim.y = (unsigned)cluster_y;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kernel, Params(args)...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return TF_ERR_CUDA;
+  }
+  return launch_status();
+}
+
 void ffn_problem(FfnProblem& q, int M, int N, int K, int a_mn, int b_mn, void* out,
                  const void* residual) {
   q.M = M, q.N = N;
@@ -1061,9 +1095,8 @@ int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
   if (light > 0 && r > 0)
     prm.bal_rounds = (int)std::min<long long>(
         prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
-  ffn_pair_kernel<MODE, ACT>
-      <<<(unsigned)(2 * clusters), kFfnThreads, FfnPairCfg<MODE>::SMEM_ALLOC, st>>>(maps, prm);
-  return launch_status();
+  return launch_ex(ffn_pair_kernel<MODE, ACT>, dim3((unsigned)(2 * clusters)), kFfnThreads,
+                   FfnPairCfg<MODE>::SMEM_ALLOC, st, 0, prm.pdl, maps, prm);
 }
 
 // FFN_STORE: the i-th product's output [m, n]
@@ -1096,25 +1129,8 @@ int ffn_tile_launch(const void* w, int w_rows, const void* x, int k, FfnTilePara
   if (!fits_i32(tiles)) return TF_ERR_TOO_LARGE;
   int S = 1;
   while (S < 8 && tiles * S < 148 && prm.n_kblk >= 8 * S) S *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)tiles, (unsigned)S, 1);
-  cfg.blockDim = dim3(kTileThreads, 1, 1);
-  cfg.dynamicSmemBytes = TileCfg<NT>::SMEM_ALLOC;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = (unsigned)S;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = prm.pdl ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, ffn_tile_kernel<NT, MODE>, ta, tb, prm) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return TF_ERR_CUDA;
-  }
-  return launch_status();
+  return launch_ex(ffn_tile_kernel<NT, MODE>, dim3((unsigned)tiles, (unsigned)S), kTileThreads,
+                   TileCfg<NT>::SMEM_ALLOC, st, S, prm.pdl, ta, tb, prm);
 }
 
 template <int MODE>
@@ -1199,6 +1215,7 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
   FfnMaps maps;
   FfnPairParams down{};
   down.n_prob = 1;
+  down.pdl = 1;
   ffn_problem(down.prob[0], m, d_model, d_ff, 0, 0, y, residual);
   if (!ffn_operand(&maps.a[0], a, m, d_ff, 0) ||
       !ffn_operand(&maps.b[0], w_down, d_model, d_ff, 0) || !ffn_out(&maps, 0, y, m, d_model))
@@ -1252,6 +1269,7 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
 
   // the three products that follow in one launch, those with the longer K first
   FfnPairParams g{};
+  g.pdl = 1;
   bool ok = true;
   auto add_dx = [&] {
     if (!dx) return;
@@ -1433,8 +1451,7 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   s.rows_per_gate = p.rows_per_gate, s.gate_rows = gate ? gate_rows : 0;
   const int outs = 2 + (s.dgate ? gate_rows : 0);
   const dim3 sgrid((unsigned)((cols + 31) / 32), (unsigned)std::min(outs, 1024));
-  block_norm_sum_kernel<<<sgrid, 1024, 0, st>>>(s);
-  return launch_status();
+  return launch_ex(block_norm_sum_kernel, sgrid, 1024, 0, st, 0, 1, s);
 }
 
 namespace {
