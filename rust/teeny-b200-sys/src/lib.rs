@@ -95,7 +95,8 @@ pub mod ffi {
             w_down: *const c_void, residual: *const c_void, a: *mut c_void, z: *mut f32,
             y: *mut c_void, m: c_int, d_model: c_int, d_ff: c_int, act: c_int,
             stream: *mut c_void) -> c_int;
-        pub fn tf_b200_gated_ffn_bwd_workspace_size(m: c_int, d_ff: c_int) -> usize;
+        pub fn tf_b200_gated_ffn_bwd_workspace_size(m: c_int, d_model: c_int,
+            d_ff: c_int) -> usize;
         pub fn tf_b200_gated_ffn_bwd_bf16(x: *const c_void, w_gate_up: *const c_void,
             w_down: *const c_void, z: *const f32, dy: *const c_void, dx: *mut c_void,
             dw_gate_up: *mut c_void, dw_down: *mut c_void, workspace: *mut c_void, m: c_int,

@@ -59,7 +59,7 @@ SIGNATURES = {
     "tf_b200_gemm_qkv_rope_bf16": (I, [P] * 6 + [I] * 6 + [P]),
     "tf_b200_gemm_push_bf16": (I, [P, P, ctypes.POINTER(ctypes.c_void_p)] + [I] * 6 + [P]),
     "tf_b200_gated_ffn_fwd_bf16": (I, [P] * 7 + [I] * 4 + [P]),
-    "tf_b200_gated_ffn_bwd_workspace_size": (SZ, [I, I]),
+    "tf_b200_gated_ffn_bwd_workspace_size": (SZ, [I, I, I]),
     "tf_b200_gated_ffn_bwd_bf16": (I, [P] * 9 + [I] * 4 + [P]),
     "tf_b200_block_norm_fwd_bf16": (I, [P] * 8 + [I] * 3 + [F] * 4 + [U, P]),
     "tf_b200_block_norm_bwd_workspace_size": (SZ, [I, I]),

@@ -103,7 +103,11 @@ constexpr int kFfnMaxProblems = 3;
 // One product D[M, N] = A[M, K] B[N, K]^T.  Either operand may be stored with
 // its M / N index innermost (a_mn / b_mn: rows of the stored matrix are K).
 struct FfnProblem {
-  int M, N, n_mblk, n_nblk, n_kblk, n_tiles, group_m;
+  int M, N, n_mblk, n_nblk, n_kblk, group_m;
+  int bn;       // columns of a tile: 256, or 128 (FFN_DGLU)
+  int ks;       // runs of k-blocks that a tile's K is split into (FFN_STORE; each gives fp32
+                // partial sums, joined by ffn_sum_kernel)
+  int n_items;  // ks times the tiles
   int a_mn, b_mn;
   __nv_bfloat16* out;             // FFN_STORE: [M, N]
   const __nv_bfloat16* residual;  // FFN_STORE: [M, N] or null
@@ -113,7 +117,7 @@ struct FfnPairParams {
   FfnProblem prob[kFfnMaxProblems];
   int n_prob;
   int pdl;  // launched with programmatic stream serialization
-  // static schedule (ffn_next): T0 tiles of the longer K, then `light` tiles
+  // static schedule (ffn_next): items of the longer K, then `light` items
   int heavy, light, bal_rounds;
   // FFN_GLU / FFN_DGLU
   int F;
@@ -162,10 +166,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sm
       : "memory");
 }
 
-// The i-th tile of a pair, in the concatenated list of all products' tiles
-// (those with the longer K first); -1 at the end.  Heavy tiles go round robin;
+// The i-th item of a pair, in the concatenated list of all products' items
+// (those with the longer K first); -1 at the end.  Heavy items go round robin;
 // the pairs that get one fewer of them (those from heavy % n_pairs on) then
-// take bal_rounds light tiles each, about one heavy tile's work, before the
+// take bal_rounds light items each, about one heavy item's work, before the
 // round robin over all pairs goes on.
 __device__ __forceinline__ int ffn_next(const FfnPairParams& p, int pair, int n_pairs, int i) {
   const int mine = pair < p.heavy ? (p.heavy - 1 - pair) / n_pairs + 1 : 0;
@@ -184,22 +188,29 @@ __device__ __forceinline__ int ffn_next(const FfnPairParams& p, int pair, int n_
   return l < p.light ? p.heavy + (int)l : -1;
 }
 
-// Tile of the list -> product, row block and column block (grouped order).
-__device__ __forceinline__ int ffn_tile(const FfnPairParams& p, int t, int& mb, int& nb) {
-  int k = 0;
-  while (k + 1 < p.n_prob && t >= p.prob[k].n_tiles) {
-    t -= p.prob[k].n_tiles;
-    ++k;
-  }
-  const FfnProblem& q = p.prob[k];
+// Item of the list -> product k, run of k-blocks, row block and column block
+// (grouped order).
+struct FfnItem {
+  int k, split, mb, nb, kb0, kb1;
+};
+__device__ __forceinline__ FfnItem ffn_item(const FfnPairParams& p, int t) {
+  FfnItem it;
+  it.k = 0;
+  while (it.k + 1 < p.n_prob && t >= p.prob[it.k].n_items) t -= p.prob[it.k++].n_items;
+  const FfnProblem& q = p.prob[it.k];
+  const int tiles = q.n_mblk * q.n_nblk;
+  it.split = t / tiles;
+  t -= it.split * tiles;
+  it.kb0 = (int)((long long)q.n_kblk * it.split / q.ks);
+  it.kb1 = (int)((long long)q.n_kblk * (it.split + 1) / q.ks);
   const int per_group = q.group_m * q.n_nblk;
   const int g = t / per_group;
   const int m_first = g * q.group_m;
   const int gm = min(q.group_m, q.n_mblk - m_first);
   const int local = t - g * per_group;
-  mb = m_first + local % gm;
-  nb = local / gm;
-  return k;
+  it.mb = m_first + local % gm;
+  it.nb = local / gm;
+  return it;
 }
 
 // Reads 32 staged rows of 32 fp32 (128-byte rows, 16-byte chunks XOR-swizzled by
@@ -225,8 +236,8 @@ __device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) 
 // zbar: this warp's two barriers, zn: its z chunks so far (FFN_DGLU).
 template <int MODE, int ACT, class Wait, class Release>
 __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
-                                                  const FfnMaps& maps, int k, uint32_t acc,
-                                                  int row0, int nb, int hf, int lane, uint32_t stg,
+                                                  const FfnMaps& maps, int k, int split,
+                                                  uint32_t acc, int row0, int nb, int hf, int lane, uint32_t stg,
                                                   uint32_t zbar, int& zn, Wait&& wait_acc,
                                                   Release&& release_acc) {
   if (row0 >= q.M) {
@@ -299,7 +310,8 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
     // chunks of 16 columns: z comes in through the two halves (gate 2 KB, up
     // 2 KB: 64-byte rows), two chunks ahead; dg, du and a go out through the
     // third 4 KB (1 KB each: 32-byte rows)
-    const int col_h = nb * kGemmBN + hf * 128;
+    const int half_cols = q.bn / 2, chunks = q.bn / 32;
+    const int col_h = nb * q.bn + hf * half_cols;
     const uint32_t out = stg + 8192;
     auto load_z = [&](int c) {  // (lane 0) chunk c of this tile into half c % 2
       const uint32_t dst = stg + (c & 1) * 4096, bar = zbar + (c & 1) * 8;
@@ -322,11 +334,11 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       (void)wait_z(zn + 1);
       return false;
     }
-    for (int c = 0; c < 8; ++c, ++zn) {  // (chunk zn of this warp is in half zn % 2 = c % 2)
+    for (int c = 0; c < chunks; ++c, ++zn) {  // (chunk zn of this warp is in half zn % 2 = c % 2)
       uint32_t r[16];
-      tmem_ld16(acc + hf * 128 + c * 16, r);
+      tmem_ld16(acc + hf * half_cols + c * 16, r);
       tmem_wait_ld();
-      if (c == 7) release_acc();
+      if (c == chunks - 1) release_acc();
       if (!wait_z(zn)) return false;
       const uint32_t buf = stg + (c & 1) * 4096;
       uint32_t dg[8], du[8], av[8];
@@ -351,7 +363,7 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       }
       __syncwarp();  // every lane has read its z
       if (lane == 0) {
-        if (c < 6) load_z(c + 2);
+        if (c + 2 < chunks) load_z(c + 2);
         bulk_wait_group_read0();  // the chunk before has left `out`
       }
       __syncwarp();
@@ -412,6 +424,23 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       }
       if (c < 3) load_res(c + 1);
       __syncwarp();
+    }
+  } else if (q.ks > 1) {
+    // fp32 partial sums of this run of k-blocks: [ks, M, N]
+    if (!wait_acc()) return false;
+    for (int c = 0; c < 4; ++c) {
+      const int col0 = nb * kGemmBN + hf * 128 + c * 32;
+      uint32_t r[32];
+      tmem_ld32(acc + hf * 128 + c * 32, r);
+      tmem_wait_ld();
+      if (c == 3) release_acc();
+      const uint32_t buf = next_half();
+      stage32(buf, r);
+      staged();
+      if (lane == 0) {
+        if (col0 < q.N) tma_store_3d(&maps.out[k], buf, col0, row0, split);
+        bulk_commit_group();
+      }
     }
   } else {
     if (!wait_acc()) return false;
@@ -508,23 +537,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     for (int i = 0; ok; ++i) {
       const int t = ffn_next(p, pair, n_pairs, i);
       if (t < 0) break;
-      int mb, nb;
-      const int k = ffn_tile(p, t, mb, nb);
-      const FfnProblem& q = p.prob[k];
-      const CUtensorMap* tm_a = &maps.a[k];
-      const CUtensorMap* tm_b = &maps.b[k];
-      const int m0 = mb * 256 + (int)crank * 128;  // this CTA's rows of A
-      const int n0 = MODE == FFN_GLU ? nb * 128 + (int)crank * p.F  // gate rows | up rows
-                                     : nb * 256 + (int)crank * 128;
+      const FfnItem item = ffn_item(p, t);
+      const FfnProblem& q = p.prob[item.k];
+      const CUtensorMap* tm_a = &maps.a[item.k];
+      const CUtensorMap* tm_b = &maps.b[item.k];
+      const int m0 = item.mb * 256 + (int)crank * 128;  // this CTA's rows of A
+      const int n0 = MODE == FFN_GLU ? item.nb * 128 + (int)crank * p.F  // gate rows | up rows
+                                     : item.nb * q.bn + (int)crank * (q.bn / 2);
+      const uint32_t bytes = 2 * (C::A_BYTES + q.bn * kGemmBK);  // both CTAs'
       const bool a_mn = q.a_mn, b_mn = q.b_mn;
-      for (int kb = 0; kb < q.n_kblk; ++kb, ++g) {
+      for (int kb = item.kb0; kb < item.kb1; ++kb, ++g) {
         const int s = g % C::STAGES, u = g / C::STAGES;
         if (u > 0) ok = mbar_wait_warp(bar(C::EMPTY + s), (u - 1) & 1, abort_flag, 921);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t sa = sbase + s * C::STAGE_BYTES;
           const uint32_t fb = full0 + s * 8;
-          if (leader) mbar_arrive_expect_tx(bar(C::FULL + s), 2 * C::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(bar(C::FULL + s), bytes);
           if (a_mn) {
             tma_load_2d_pair(sa, tm_a, fb, m0, kb * kGemmBK);
             tma_load_2d_pair(sa + 8192, tm_a, fb, m0 + 64, kb * kGemmBK);
@@ -533,7 +562,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
           }
           if (b_mn) {
             tma_load_2d_pair(sa + C::A_BYTES, tm_b, fb, n0, kb * kGemmBK);
-            tma_load_2d_pair(sa + C::A_BYTES + 8192, tm_b, fb, n0 + 64, kb * kGemmBK);
+            if (MODE != FFN_DGLU || q.bn == 256)
+              tma_load_2d_pair(sa + C::A_BYTES + 8192, tm_b, fb, n0 + 64, kb * kGemmBK);
           } else {
             tma_load_2d_pair(sa + C::A_BYTES, tm_b, fb, kb * kGemmBK, n0);
           }
@@ -562,10 +592,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       for (int i = 0; ok; ++i) {
         const int t = ffn_next(p, pair, n_pairs, i);
         if (t < 0) break;
-        int mb, nb;
-        const FfnProblem& q = p.prob[ffn_tile(p, t, mb, nb)];
-        const int a_mn = q.a_mn, b_mn = q.b_mn, n_kblk = q.n_kblk;
-        const uint32_t idesc = make_idesc_bf16(256, kGemmBN, a_mn, b_mn);
+        const FfnItem item = ffn_item(p, t);
+        const FfnProblem& q = p.prob[item.k];
+        const int a_mn = q.a_mn, b_mn = q.b_mn, n_kblk = item.kb1 - item.kb0;
+        const uint32_t idesc = make_idesc_bf16(256, q.bn, a_mn, b_mn);
         const uint64_t da0 = make_sdesc_sw128(sbase, a_mn ? 8192 : 16, 1024);
         const uint64_t db0 = make_sdesc_sw128(sbase + C::A_BYTES, b_mn ? 8192 : 16, 1024);
         const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
@@ -607,12 +637,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     for (int i = 0;; ++i) {
       const int t = ffn_next(p, pair, n_pairs, i);
       if (t < 0) break;
-      int mb, nb;
-      const int k = ffn_tile(p, t, mb, nb);
-      const FfnProblem& q = p.prob[k];
+      const FfnItem item = ffn_item(p, t);
+      const FfnProblem& q = p.prob[item.k];
       const int b = i & 1, use = i >> 1;
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * kGemmBN;
-      const int row0 = mb * 256 + (int)crank * 128 + quarter * 32;
+      const int row0 = item.mb * 256 + (int)crank * 128 + quarter * 32;
       auto wait_acc = [&]() {
         const bool ok = mbar_wait_warp(bar(C::AFULL + b), use & 1, abort_flag, 926);
         tc_fence_after();
@@ -623,8 +652,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
       };
-      if (!ffn_epilogue_warp<MODE, ACT>(p, q, maps, k, acc, row0, nb, hf, lane, stg,
-                                        bar(C::Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
+      if (!ffn_epilogue_warp<MODE, ACT>(p, q, maps, item.k, item.split, acc, row0, item.nb, hf,
+                                        lane, stg, bar(C::Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
         break;
     }
     if (lane == 0) bulk_wait_group0();  // the stores, before the shared memory goes away
@@ -637,6 +666,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, C::TM_COLS);
+  }
+}
+
+// Joins the partial sums of products whose K was split: out = sum over the runs,
+// in order, rounded once.
+struct FfnSumParams {
+  const float* part[kFfnMaxProblems];  // [ks, n]
+  __nv_bfloat16* out[kFfnMaxProblems];
+  long long n[kFfnMaxProblems];  // a multiple of 8
+  int ks[kFfnMaxProblems];
+  int n_prob;
+};
+
+__global__ void __launch_bounds__(256) ffn_sum_kernel(const __grid_constant__ FfnSumParams p) {
+  pdl_wait();
+  for (int k = 0; k < p.n_prob; ++k) {
+    const long long n4 = p.n[k] / 4;
+    const float4* part = reinterpret_cast<const float4*>(p.part[k]);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4;
+         i += (long long)gridDim.x * 256) {
+      float4 v = part[i];
+#pragma unroll 4
+      for (int s = 1; s < p.ks[k]; ++s) {
+        const float4 w = part[s * n4 + i];
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      reinterpret_cast<uint2*>(p.out[k])[i] =
+          make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    }
   }
 }
 

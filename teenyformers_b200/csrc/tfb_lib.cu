@@ -1048,7 +1048,9 @@ void ffn_problem(FfnProblem& q, int M, int N, int K, int a_mn, int b_mn, void* o
   q.n_mblk = (M + 255) / 256;
   q.n_nblk = (N + kGemmBN - 1) / kGemmBN;
   q.n_kblk = (K + kGemmBK - 1) / kGemmBK;
-  q.n_tiles = q.n_mblk * q.n_nblk;
+  q.bn = kGemmBN;
+  q.ks = 1;
+  q.n_items = q.n_mblk * q.n_nblk;
   q.group_m = std::min(q.n_mblk, 8);
   q.a_mn = a_mn, q.b_mn = b_mn;
   q.out = static_cast<__nv_bfloat16*>(out);
@@ -1084,17 +1086,16 @@ constexpr CUtensorMapDataType kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
 
 template <int MODE, int ACT>
 int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
-  // products come longest K first; those of the first one's K are the heavy tiles
+  // products come longest (run of) K first; those of the first one's are the heavy items
+  auto run = [&](int i) { return (prm.prob[i].n_kblk + prm.prob[i].ks - 1) / prm.prob[i].ks; };
   long long heavy = 0, light = 0;
-  for (int i = 0; i < prm.n_prob; ++i)
-    (prm.prob[i].n_kblk == prm.prob[0].n_kblk ? heavy : light) += prm.prob[i].n_tiles;
+  for (int i = 0; i < prm.n_prob; ++i) (run(i) == run(0) ? heavy : light) += prm.prob[i].n_items;
   if (!fits_i32(heavy + light)) return TF_ERR_TOO_LARGE;
   const long long clusters = std::min<long long>(heavy + light, g_pair_clusters[current_device()]);
   prm.heavy = (int)heavy, prm.light = (int)light, prm.bal_rounds = 0;
   const long long r = heavy % clusters, q = clusters - r;
   if (light > 0 && r > 0)
-    prm.bal_rounds = (int)std::min<long long>(
-        prm.prob[0].n_kblk / prm.prob[prm.n_prob - 1].n_kblk, light / q);
+    prm.bal_rounds = (int)std::min<long long>(run(0) / run(prm.n_prob - 1), light / q);
   return launch_ex(ffn_pair_kernel<MODE, ACT>, dim3((unsigned)(2 * clusters)), kFfnThreads,
                    FfnPairCfg<MODE>::SMEM_ALLOC, st, 0, prm.pdl, maps, prm);
 }
@@ -1102,6 +1103,20 @@ int ffn_pair_launch(const FfnMaps& maps, FfnPairParams& prm, cudaStream_t st) {
 // FFN_STORE: the i-th product's output [m, n]
 bool ffn_out(FfnMaps* maps, int i, const void* out, int m, int n) {
   return ffn_box(&maps->out[i], out, n, m, 0, 64, kBf16, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// A split product's partial sums [ks, m, n] fp32, boxes of 32 x 32
+bool ffn_part(FfnMaps* maps, int i, const void* part, int m, int n, int ks) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)m, (cuuint64_t)ks};
+  cuuint64_t strides[2] = {(cuuint64_t)n * 4, (cuuint64_t)n * 4 * (cuuint64_t)m};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(&maps->out[i], kF32, 3, const_cast<void*>(part), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int MODE>
@@ -1196,7 +1211,7 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
     prm.z = z;
     ffn_problem(prm.prob[0], m, 2 * d_ff, d_model, 0, 0, nullptr, nullptr);
     prm.prob[0].n_nblk = (d_ff + 127) / 128;  // 128 gate and 128 up rows a tile
-    prm.prob[0].n_tiles = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
+    prm.prob[0].n_items = prm.prob[0].n_mblk * prm.prob[0].n_nblk;
     if (!ffn_operand(&maps.a[0], x, m, d_model, 0) ||
         !ffn_operand(&maps.b[0], w_gate_up, 2 * d_ff, d_model, 0) ||
         !ffn_box(&maps.out[0], a, d_ff, m, 0, 32, kBf16, CU_TENSOR_MAP_SWIZZLE_64B) ||
@@ -1223,9 +1238,56 @@ extern "C" int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, 
   return ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, down, st);
 }
 
-extern "C" size_t tf_b200_gated_ffn_bwd_workspace_size(int m, int d_ff) {
-  if (m <= 0 || d_ff <= 0 || d_ff % 8 != 0) return 0;
-  return (size_t)m * d_ff * 3 * 2;  // dz [m, 2 d_ff] and a [m, d_ff]
+namespace {
+
+// The three products behind dz and a: dx, dw_gate_up, dw_down (M, N, K), and
+// the runs that each one's K is split into where its tiles are few and its K
+// long next to the rest of the work: 129 x 1032 x 2776 has 5 tiles of 87
+// k-blocks for dx, and the other 69 pairs have 5 k-blocks each.  A pure
+// function of the shape (74 pairs), so that the workspace query and the launch
+// agree; splits are chosen for all three products whichever are asked for, so
+// that a result's bits do not depend on the others.
+struct FfnBwdPlan {
+  int M[3], N[3], K[3], ks[3];
+  size_t part[3];   // offset of the partial sums in the workspace, bytes
+  size_t bytes;     // the workspace
+};
+FfnBwdPlan ffn_bwd_plan(int m, int d, int F) {
+  FfnBwdPlan p;
+  const int M[3] = {m, 2 * F, d}, N[3] = {d, d, F}, K[3] = {2 * F, m, m};
+  constexpr double kPairs = 74.0;
+  double work = 0.0;  // k-blocks; a tile's epilogue takes as long as about eight
+  double tiles[3], kblk[3];
+  for (int i = 0; i < 3; ++i) {
+    p.M[i] = M[i], p.N[i] = N[i], p.K[i] = K[i];
+    tiles[i] = std::ceil(M[i] / 256.0) * std::ceil(N[i] / 256.0);
+    kblk[i] = std::ceil(K[i] / 64.0);
+    work += tiles[i] * std::max(kblk[i], 8.0);
+  }
+  const double even = std::max(work / kPairs, 8.0);
+  size_t at = (size_t)m * F * 3 * 2;  // dz [m, 2 F] and a [m, F]
+  at = (at + 255) / 256 * 256;
+  for (int i = 0; i < 3; ++i) {
+    p.ks[i] = 1;
+    // it has to be worth the launch that joins the sums: with 16 k-blocks here a
+    // step of 1111 x 520 x 1416 lost 3 us by it, with 28 777 x 1032 x 2776 gains 6
+    if (kblk[i] > even + 28.0) {
+      const double most = std::min({8.0, kPairs / tiles[i], kblk[i] / 8.0});
+      p.ks[i] = std::max(1, (int)std::min(most, std::ceil(kblk[i] / even)));
+    }
+    p.part[i] = at;
+    if (p.ks[i] > 1) at += (size_t)p.ks[i] * M[i] * N[i] * 4;
+    at = (at + 255) / 256 * 256;
+  }
+  p.bytes = at;
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t tf_b200_gated_ffn_bwd_workspace_size(int m, int d_model, int d_ff) {
+  if (m <= 0 || ffn_check(m, d_model, d_ff, 0) != TF_OK || d_model == 0 || d_ff == 0) return 0;
+  return ffn_bwd_plan(m, d_model, d_ff).bytes;
 }
 
 extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, const void* w_down,
@@ -1259,6 +1321,14 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
   prm.z = const_cast<float*>(z);
   prm.dz = dz;
   ffn_problem(prm.prob[0], m, d_ff, d_model, 0, 1, nullptr, nullptr);
+  // few tiles: half as wide ones, while they are a pair's only one (the epilogue,
+  // some 7 us of a tile, takes half the time)
+  FfnProblem& q = prm.prob[0];
+  if (2LL * q.n_items <= g_pair_clusters[current_device()]) {
+    q.bn = 128;
+    q.n_nblk = (d_ff + 127) / 128;
+    q.n_items = q.n_mblk * q.n_nblk;
+  }
   if (!ffn_operand(&maps.a[0], dy, m, d_model, 0) ||
       !ffn_operand(&maps.b[0], w_down, d_ff, d_model, 1) ||
       !ffn_box(&maps.out[0], a, d_ff, m, 0, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
@@ -1267,35 +1337,45 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
     return TF_ERR_CUDA;
   if (int e = ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st)) return e;
 
-  // the three products that follow in one launch, those with the longer K first
+  // the three products that follow in one launch, those with the longer (run of) K first
+  const FfnBwdPlan plan = ffn_bwd_plan(m, d_model, d_ff);
+  void* outs[3] = {dx, dw_gate_up, dw_down};
+  int order[3] = {0, 1, 2};
+  std::stable_sort(order, order + 3, [&](int a_, int b_) {
+    return (long long)plan.K[a_] * plan.ks[b_] > (long long)plan.K[b_] * plan.ks[a_];
+  });
   FfnPairParams g{};
   g.pdl = 1;
-  bool ok = true;
-  auto add_dx = [&] {
-    if (!dx) return;
+  FfnSumParams sum{};
+  for (const int w : order) {
+    if (!outs[w]) continue;
     const int i = g.n_prob++;
-    ffn_problem(g.prob[i], m, d_model, 2 * d_ff, 0, 1, dx, nullptr);
-    ok = ok && ffn_operand(&maps.a[i], dz, m, 2 * d_ff, 0) &&
-         ffn_operand(&maps.b[i], w_gate_up, d_model, 2 * d_ff, 1) &&
-         ffn_out(&maps, i, dx, m, d_model);
-  };
-  if (2 * d_ff >= m) add_dx();
-  if (dw_gate_up) {
-    const int i = g.n_prob++;
-    ffn_problem(g.prob[i], 2 * d_ff, d_model, m, 1, 1, dw_gate_up, nullptr);
-    ok = ok && ffn_operand(&maps.a[i], dz, 2 * d_ff, m, 1) &&
-         ffn_operand(&maps.b[i], x, d_model, m, 1) &&
-         ffn_out(&maps, i, dw_gate_up, 2 * d_ff, d_model);
+    const int M = plan.M[w], N = plan.N[w], K = plan.K[w], a_mn = w > 0;
+    const void* lhs = w == 2 ? dy : dz;
+    const void* rhs = w == 0 ? w_gate_up : w == 1 ? x : a;
+    ffn_problem(g.prob[i], M, N, K, a_mn, 1, outs[w], nullptr);
+    g.prob[i].ks = plan.ks[w];
+    g.prob[i].n_items *= plan.ks[w];
+    bool ok = ffn_operand(&maps.a[i], lhs, M, K, a_mn) && ffn_operand(&maps.b[i], rhs, N, K, 1);
+    if (plan.ks[w] > 1) {
+      float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.part[w]);
+      ok = ok && ffn_part(&maps, i, part, M, N, plan.ks[w]);
+      const int k = sum.n_prob++;
+      sum.part[k] = part;
+      sum.out[k] = static_cast<__nv_bfloat16*>(outs[w]);
+      sum.n[k] = (long long)M * N;
+      sum.ks[k] = plan.ks[w];
+    } else {
+      ok = ok && ffn_out(&maps, i, outs[w], M, N);
+    }
+    if (!ok) return TF_ERR_CUDA;
   }
-  if (dw_down) {
-    const int i = g.n_prob++;
-    ffn_problem(g.prob[i], d_model, d_ff, m, 1, 1, dw_down, nullptr);
-    ok = ok && ffn_operand(&maps.a[i], dy, d_model, m, 1) &&
-         ffn_operand(&maps.b[i], a, d_ff, m, 1) && ffn_out(&maps, i, dw_down, d_model, d_ff);
-  }
-  if (2 * d_ff < m) add_dx();
-  if (!ok) return TF_ERR_CUDA;
-  return ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, g, st);
+  if (int e = ffn_pair_launch<FFN_STORE, FFN_ACT_SILU>(maps, g, st)) return e;
+  if (sum.n_prob == 0) return TF_OK;
+  long long most = 0;
+  for (int k = 0; k < sum.n_prob; ++k) most = std::max(most, sum.n[k]);
+  return launch_ex(ffn_sum_kernel, dim3((unsigned)std::min<long long>((most / 4 + 255) / 256, 148 * 4)),
+                   256, 0, st, 0, 1, sum);
 }
 
 // ===================================================================== block norm, dropout

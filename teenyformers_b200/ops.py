@@ -434,7 +434,7 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor
     g = [None if not on else torch.empty_like(like) if t is None
          else _buffer(t, like.shape, torch.bfloat16, x, "a gradient")
          for t, like, on in zip(given, (x, w_gate_up, w_down), need)]
-    n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d_ff)
+    n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d, d_ff)
     ws = _workspace(n, workspace, x)
     _launch(x, "tf_b200_gated_ffn_bwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
             w_down.data_ptr(), z.data_ptr(), dy.data_ptr(), _addr(g[0]), _addr(g[1]), _addr(g[2]),

@@ -62,9 +62,15 @@ def test_gated_ffn_bwd_refusals(native_lib):
     for k in ("x", "w1", "w2", "z", "dy", "dx", "d1", "d2", "ws"):
         assert ffn_bwd(**{k: ODD}) == TF_ERR_MISALIGNED
     assert ffn_bwd(dx=None, d1=None, d2=None) == TF_OK       # nothing asked for
-    size = lambda m, F: _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, F)
-    assert size(7, 128) == 7 * 128 * 3 * 2 and size(0, 128) == 0 and size(5, 100) == 0
-    assert size(1 << 20, 1 << 16) == (1 << 36) * 6           # no 32-bit overflow
+    size = lambda m, d, F: _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d, F)
+    up = lambda n: -(-n // 256) * 256
+    assert size(7, 64, 128) == up(7 * 128 * 3 * 2)           # dz and a
+    assert size(0, 64, 128) == size(5, 64, 100) == size(5, 60, 128) == size(5, 0, 128) == 0
+    assert size(1 << 20, 4096, 1 << 16) == (1 << 36) * 6     # no 32-bit overflow
+    # few tokens and a long sum for dx: fp32 partial sums besides
+    assert size(129, 1032, 2776) >= up(129 * 2776 * 6) + 2 * 129 * 1032 * 4
+    # many tokens and small weights: of the weights' gradients
+    assert size(8192, 64, 64) > up(8192 * 64 * 6) + 2 * 2 * 64 * 64 * 4
 
 
 def norm(*, x=FAKE, f=FAKE, wp=FAKE, g=FAKE, wn=FAKE, y=FAKE, h=FAKE, rng=None, rows=6, cols=64,

@@ -31,7 +31,9 @@ def _guarded(shape, dtype, dev):
 
 SIZES = [(1, 8, 8), (1, 64, 128), (2, 520, 1416), (3, 72, 136), (7, 4096, 512), (16, 256, 512),
          (17, 128, 72), (33, 264, 1000), (64, 520, 200), (65, 136, 264), (128, 256, 1024),
-         (129, 256, 128), (200, 64, 64), (300, 520, 1416), (513, 1032, 264)]
+         (129, 256, 128), (200, 64, 64), (300, 520, 1416), (513, 1032, 264),
+         # few tiles and a long sum: of dx, of the weights' gradients, ragged
+         (129, 520, 2776), (5, 8, 5000), (4100, 64, 72), (2056, 8, 8)]
 
 
 @pytest.mark.parametrize("m,d,F", SIZES)
@@ -112,15 +114,16 @@ def test_gradients_against_differences(cuda_device):
 
 def test_skipped_gradients_and_no_tokens(cuda_device):
     import teenyformers_b200 as tfb
-    x, w1, w2 = _inputs(70, 136, 264, cuda_device)
-    dy = seeded_normal((70, 136), 3, cuda_device)
-    _, z = tfb.gated_ffn(x, w1, w2, save=True)
-    full = tfb.gated_ffn_bwd(x, w1, w2, z, dy)
-    for need in [(True, False, False), (False, True, False), (False, False, True),
-                 (True, True, False), (False, True, True), (True, False, True)]:
-        part = tfb.gated_ffn_bwd(x, w1, w2, z, dy, need=need)
-        for on, p, f in zip(need, part, full):
-            assert (p is None) if not on else torch.equal(p, f)
+    for m, d, F in ((129, 136, 2776), (4100, 64, 72), (70, 136, 264)):
+        x, w1, w2 = _inputs(m, d, F, cuda_device)
+        dy = seeded_normal((m, d), 3, cuda_device)
+        _, z = tfb.gated_ffn(x, w1, w2, save=True)
+        full = tfb.gated_ffn_bwd(x, w1, w2, z, dy)
+        for need in [(True, False, False), (False, True, False), (False, False, True),
+                     (True, True, False), (False, True, True), (True, False, True)]:
+            part = tfb.gated_ffn_bwd(x, w1, w2, z, dy, need=need)
+            for on, p, f in zip(need, part, full):
+                assert (p is None) if not on else torch.equal(p, f)
     assert tfb.gated_ffn_bwd(x, w1, w2, z, dy, need=(False, False, False)) == (None, None, None)
     e = x[:0]
     y, z = tfb.gated_ffn(e, w1, w2, save=True)
