@@ -671,7 +671,9 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
 
 // Sums the partials: output 0 is dw_post, 1 is dw_pre (a partial a CTA), 2 + g
 // the gate's row g where more than one team has rows of it (a partial a team).
-// 32 columns a block, 32 strided partial sums a column, joined in a fixed order.
+// 128 columns a block, four a lane; each of 16 warps takes every 16th partial,
+// and the warps' sums are joined in order.
+constexpr int kBnSumThreads = 512;
 struct BlockNormSumParams {
   const float* part_post;
   const float* part_pre;
@@ -682,49 +684,56 @@ struct BlockNormSumParams {
   int cols, n_ctas, rows_per_team, rows_per_gate, gate_rows;
 };
 
-__global__ void __launch_bounds__(1024) block_norm_sum_kernel(const BlockNormSumParams p) {
-  pdl_wait();
-  __shared__ float s[32][33];
+__global__ void __launch_bounds__(kBnSumThreads)
+    block_norm_sum_kernel(const BlockNormSumParams p) {
+  constexpr int WARPS = kBnSumThreads / 32;
+  __shared__ float4 s[WARPS][32];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int col = (int)blockIdx.x * 32 + lane;
+  const int col = (int)blockIdx.x * 128 + lane * 4;
   const int outs = 2 + (p.dgate ? p.gate_rows : 0);
+  pdl_wait();
   for (int o = blockIdx.y; o < outs; o += gridDim.y) {
     const float* src;
     __nv_bfloat16* dst;
-    int t0 = 0, t1 = p.n_ctas - 1;
+    int t0 = 0, t1 = p.n_ctas - 1, inside = -1;
+    long long step = p.cols;
     const int g = o - 2;
     if (o == 0) {
       src = p.part_post, dst = p.dw_post;
     } else if (o == 1) {
       src = p.part_pre, dst = p.dw_pre;
     } else {
+      // a team's slot 0, or 1 where the gate row starts inside its rows: only
+      // the first team can have that
+      const long long row = (long long)g * p.rows_per_gate;
       src = p.part_gate, dst = p.dgate + (long long)g * p.cols;
-      t0 = (int)((long long)g * p.rows_per_gate / p.rows_per_team);
-      t1 = (int)((((long long)g + 1) * p.rows_per_gate - 1) / p.rows_per_team);
+      step = 2LL * p.cols;
+      t0 = (int)(row / p.rows_per_team);
+      t1 = (int)((row + p.rows_per_gate - 1) / p.rows_per_team);
+      if (row > (long long)t0 * p.rows_per_team) inside = t0;
       if (t0 == t1) dst = nullptr;  // written whole by its team
     }
     if (!dst) continue;  // the same for every thread of the block
-    float acc = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (col < p.cols) {
+      const float* at = src + col;
 #pragma unroll 8
-      for (int t = t0 + part; t <= t1; t += 32) {
-        long long at = t;
-        if (o >= 2) {
-          // slot 0 unless the segment starts inside the team's rows
-          const bool inside = (long long)g * p.rows_per_gate > (long long)t * p.rows_per_team;
-          at = 2LL * t + (inside ? 1 : 0);
-        }
-        acc += src[at * p.cols + col];
+      for (int t = t0 + part; t <= t1; t += WARPS) {
+        const float4 v =
+            *reinterpret_cast<const float4*>(at + t * step + (t == inside ? p.cols : 0));
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
       }
     }
     s[part][lane] = acc;
     __syncthreads();
-    // warp w sums column w of the block's 32
-    acc = s[lane][part];
+    const int c = (int)blockIdx.x * 128 + (int)threadIdx.x;
+    if (threadIdx.x < 128 && c < p.cols) {
+      const float* f = reinterpret_cast<const float*>(s) + threadIdx.x;
+      float v = f[0];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
-    const int c = (int)blockIdx.x * 32 + part;
-    if (lane == 0 && c < p.cols) dst[c] = __float2bfloat16_rn(acc);
+      for (int w = 1; w < WARPS; ++w) v += f[w * 128];
+      dst[c] = __float2bfloat16_rn(v);
+    }
     __syncthreads();
   }
 }

@@ -1530,8 +1530,8 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   s.cols = cols, s.n_ctas = t.n_ctas, s.rows_per_team = t.rows_per_team;
   s.rows_per_gate = p.rows_per_gate, s.gate_rows = gate ? gate_rows : 0;
   const int outs = 2 + (s.dgate ? gate_rows : 0);
-  const dim3 sgrid((unsigned)((cols + 31) / 32), (unsigned)std::min(outs, 1024));
-  return launch_ex(block_norm_sum_kernel, sgrid, 1024, 0, st, 0, 1, s);
+  const dim3 sgrid((unsigned)((cols + 127) / 128), (unsigned)std::min(outs, 1024));
+  return launch_ex(block_norm_sum_kernel, sgrid, kBnSumThreads, 0, st, 0, 1, s);
 }
 
 namespace {
