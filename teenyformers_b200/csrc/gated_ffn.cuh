@@ -72,7 +72,8 @@ __device__ __forceinline__ void ffn_act_grad(float g, float& value, float& slope
     slope = fmaf(g * 0.39894228040143268f, E, phi);
   } else {
     // (1 + tanh v) / 2 = sigmoid(2 v), v = sqrt(2 / pi) (g + 0.044715 g^3)
-    const float g2 = g * g;
+    // (past |g| = 1e5 s is 0 or 1, and an infinite g^2 would make 0 x inf of the slope)
+    const float g2 = fminf(g * g, 1e10f);
     const float s = ffn_sigmoid(1.5957691216057308f * g * fmaf(0.044715f, g2, 1.0f));
     value = g * s;
     slope = fmaf(value * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f, g2, 1.0f), s);
@@ -526,11 +527,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();  // (a tile kernel behind this one may set itself up)
 
+  // (every role: the bounded waits below start when the kernel before has ended)
+  if (p.pdl) pdl_wait();
+
   if (warp == 0) {
     // ===================== TMA producer (both CTAs) =====================
-    // (the other roles' global reads and writes follow a product's loads, or are
-    // of what the kernel before this one does not write)
-    if (p.pdl) pdl_wait();
     const uint32_t full0 = mapa_cta(bar(C::FULL), 0);  // the even CTA's FULL[0]
     int g = 0;
     bool ok = true;
@@ -860,6 +861,9 @@ __global__ void __launch_bounds__(kTileThreads)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();  // (a kernel behind this one may set itself up)
+  // the bounded waits of the other roles start when the kernel before has ended;
+  // warp 0 asks for weights first
+  if (p.pdl && warp != 0) pdl_wait();
 
   if (warp == 0) {
     auto load_a = [&](int kb, int s) {
@@ -949,7 +953,6 @@ __global__ void __launch_bounds__(kTileThreads)
     tc_fence_after();
     tmem_dealloc(tmem, C::TM_COLS);
   }
-  if (p.pdl) pdl_wait();  // the residual and the outputs belong to the stream's order too
   if (!*abort_flag) {
     const int tokens = min(NT, p.T - t0);
     switch (S) {

@@ -15,6 +15,7 @@
 #include <cstdint>
 #include <atomic>
 #include <mutex>
+#include <utility>
 
 #include "../../include/teenyformers_b200.h"
 #include "sm100.cuh"
@@ -164,17 +165,21 @@ int ensure_device_setup() {
     // 8192 columns: one row a stage of three
     const int bn_fwd = kBnStages * 2 * kBnMaxCols * 2, bn_bwd = kBnStages * 4 * kBnMaxCols * 2;
     static_assert(kBnStages * 4 * kBnMaxCols * 2 <= 227 * 1024 - 2048, "block norm's ring");
-#define TFB_BN_SET(W, V)                                                                  \
-  set((const void*)block_norm_fwd_kernel<W, V, true>, std::max(bn_fwd, kBnRingBytes));    \
-  set((const void*)block_norm_fwd_kernel<W, V, false>, std::max(bn_fwd, kBnRingBytes));   \
-  set((const void*)block_norm_bwd_kernel<W, V, true>, std::max(bn_bwd, kBnRingBytes));    \
-  set((const void*)block_norm_bwd_kernel<W, V, false>, std::max(bn_bwd, kBnRingBytes))
-    TFB_BN_SET(1, 1);
-    TFB_BN_SET(1, 2);
-    TFB_BN_SET(2, 2);
-    TFB_BN_SET(4, 2);
-    TFB_BN_SET(8, 2);
-    TFB_BN_SET(8, 4);
+#define TFB_BN_SET(W, V, KERNEL, BYTES)                                        \
+  set((const void*)KERNEL<W, V, true>, std::max(BYTES, kBnRingBytes));        \
+  set((const void*)KERNEL<W, V, false>, std::max(BYTES, kBnRingBytes))
+    TFB_BN_SET(1, 1, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(1, 2, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(2, 2, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(4, 2, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(8, 2, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(8, 4, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(1, 1, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(2, 1, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(4, 1, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(8, 1, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(8, 2, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(8, 4, block_norm_bwd_kernel, bn_bwd);
 #undef TFB_BN_SET
     // CTA pairs that fit at once (SMs pair up within a GPC; one CTA per SM)
     g_pair_clusters[dev] = g_num_sms[dev] / 2;
@@ -1178,6 +1183,9 @@ int ffn_check(int m, int d_model, int d_ff, int act) {
   if (act < TF_ACT_SILU || act > TF_ACT_GELU_TANH) return TF_ERR_INVALID_ARG;
   if (d_model % 8 != 0 || d_ff % 8 != 0) return TF_ERR_UNSUPPORTED;
   if (!fits_i32(2LL * d_ff)) return TF_ERR_TOO_LARGE;
+  // tiles of every product (128 x 64 at the smallest, up to eight runs of K)
+  const long long mt = (m + 127LL) / 128, dt = (d_model + 63LL) / 64, ft = (d_ff + 31LL) / 32;
+  if (!fits_i32(mt * dt) || !fits_i32(mt * ft) || !fits_i32(dt * ft)) return TF_ERR_TOO_LARGE;
   return TF_OK;
 }
 
@@ -1341,9 +1349,12 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
   const FfnBwdPlan plan = ffn_bwd_plan(m, d_model, d_ff);
   void* outs[3] = {dx, dw_gate_up, dw_down};
   int order[3] = {0, 1, 2};
-  std::stable_sort(order, order + 3, [&](int a_, int b_) {
-    return (long long)plan.K[a_] * plan.ks[b_] > (long long)plan.K[b_] * plan.ks[a_];
-  });
+  for (int i = 1; i < 3; ++i)
+    for (int j = i; j > 0; --j) {
+      const int u = order[j - 1], v = order[j];
+      if ((long long)plan.K[v] * plan.ks[u] > (long long)plan.K[u] * plan.ks[v])
+        std::swap(order[j - 1], order[j]);
+    }
   FfnPairParams g{};
   g.pdl = 1;
   FfnSumParams sum{};
@@ -1410,19 +1421,23 @@ int block_norm_check(int rows, int cols, bool gate, int gate_rows, float eps, fl
 }
 
 // One launch of a kernel<WPR, VPT, ALL> by the shape's team size.
-#define TFB_BN_DISPATCH_ALL(T, ALL, LAUNCH)                               \
-  do {                                                                    \
-    if ((T).wpr == 1 && (T).vpt == 1) LAUNCH(1, 1, ALL);                  \
-    else if ((T).wpr == 1) LAUNCH(1, 2, ALL);                             \
-    else if ((T).wpr == 2) LAUNCH(2, 2, ALL);                             \
-    else if ((T).wpr == 4) LAUNCH(4, 2, ALL);                             \
-    else if ((T).vpt == 2) LAUNCH(8, 2, ALL);                             \
-    else LAUNCH(8, 4, ALL);                                               \
+#define TFB_BN_FWD_DISPATCH(T, ALL, LAUNCH)            \
+  do {                                                 \
+    if ((T).vpt == 1) LAUNCH(1, 1, ALL);               \
+    else if ((T).vpt == 4) LAUNCH(8, 4, ALL);          \
+    else if ((T).wpr == 1) LAUNCH(1, 2, ALL);          \
+    else if ((T).wpr == 2) LAUNCH(2, 2, ALL);          \
+    else if ((T).wpr == 4) LAUNCH(4, 2, ALL);          \
+    else LAUNCH(8, 2, ALL);                            \
   } while (0)
-#define TFB_BN_DISPATCH(T, ALL, LAUNCH)               \
-  do {                                                \
-    if (ALL) TFB_BN_DISPATCH_ALL(T, true, LAUNCH);    \
-    else TFB_BN_DISPATCH_ALL(T, false, LAUNCH);       \
+#define TFB_BN_BWD_DISPATCH(T, ALL, LAUNCH)            \
+  do {                                                 \
+    if ((T).vpt == 2) LAUNCH(8, 2, ALL);               \
+    else if ((T).vpt == 4) LAUNCH(8, 4, ALL);          \
+    else if ((T).wpr == 1) LAUNCH(1, 1, ALL);          \
+    else if ((T).wpr == 2) LAUNCH(2, 1, ALL);          \
+    else if ((T).wpr == 4) LAUNCH(4, 1, ALL);          \
+    else LAUNCH(8, 1, ALL);                            \
   } while (0)
 
 }  // namespace
@@ -1456,7 +1471,10 @@ extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const v
 #define TFB_BN_FWD(W, V, A)                                                 \
   block_norm_fwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem,  \
                                    static_cast<cudaStream_t>(stream)>>>(p, t)
-  TFB_BN_DISPATCH(t, f && w_post && w_pre, TFB_BN_FWD);
+  if (f && w_post && w_pre)
+    TFB_BN_FWD_DISPATCH(t, true, TFB_BN_FWD);
+  else
+    TFB_BN_FWD_DISPATCH(t, false, TFB_BN_FWD);
 #undef TFB_BN_FWD
   return launch_status();
 }
@@ -1518,7 +1536,10 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   p.cyclic = !gate || p.rows_per_gate == 1 || gate_rows == 1;
 #define TFB_BN_BWD(W, V, A) \
   block_norm_bwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem, st>>>(p, t)
-  TFB_BN_DISPATCH(t, w_post && w_pre && dy && df, TFB_BN_BWD);
+  if (w_post && w_pre && dy && df)
+    TFB_BN_BWD_DISPATCH(t, true, TFB_BN_BWD);
+  else
+    TFB_BN_BWD_DISPATCH(t, false, TFB_BN_BWD);
 #undef TFB_BN_BWD
   if (int e = launch_status()) return e;
   if (!w_post && !w_pre && !gate) return TF_OK;

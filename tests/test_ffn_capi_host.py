@@ -39,6 +39,8 @@ def test_gated_ffn_refusals(native_lib):
     assert ffn(F=100) == TF_ERR_UNSUPPORTED
     assert ffn(F=0) == TF_ERR_UNSUPPORTED
     assert ffn(F=0x7FFFFFF8) == TF_ERR_TOO_LARGE
+    assert ffn(m=1 << 30, d=1 << 16) == TF_ERR_TOO_LARGE     # tiles past 31 bits
+    assert ffn(d=1 << 24, F=1 << 24) == TF_ERR_TOO_LARGE
     for k in ("x", "w1", "w2", "a", "y"):
         assert ffn(**{k: None}) == TF_ERR_INVALID_ARG
         assert ffn(**{k: ODD}) == TF_ERR_MISALIGNED

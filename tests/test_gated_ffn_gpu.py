@@ -112,6 +112,35 @@ def test_gradients_against_differences(cuda_device):
             assert abs(got - want) <= tol, (act, i, got, want, tol)
 
 
+@pytest.mark.parametrize("m", [1, 300])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_saturated_and_huge_pre_activations(cuda_device, m, act):
+    """g far outside the activation's bend: the value is 0 or g, the slope 0 or 1, with no
+    0 * inf on the way.  x picks one column of the weights, so z is known exactly, dz is
+    the first column of dw_gate_up (summed over the tokens) and y that of a's products."""
+    import teenyformers_b200 as tfb
+    g = torch.tensor([0.0, -0.0, 3.0, -3.0, 20.0, -20.0, 90.0, -90.0, 3e4, -3e4, 1e12, -1e12, 1e20,
+                      -1e20, 1e30, -1e30], device=cuda_device)
+    F, d = g.numel(), 8
+    x = torch.zeros((m, d), device=cuda_device, dtype=torch.bfloat16)
+    x[:, 0] = 1
+    w1 = torch.zeros((2 * F, d), device=cuda_device, dtype=torch.bfloat16)
+    w1[:F, 0] = g.bfloat16()
+    w1[F:, 0] = 1
+    w2 = torch.ones((d, F), device=cuda_device, dtype=torch.bfloat16)
+    dy = torch.full((m, d), 0.125, device=cuda_device, dtype=torch.bfloat16)   # da = 1
+    y, z = tfb.gated_ffn(x, w1, w2, NAMES[act], save=True)
+    assert torch.equal(z[0, :F], w1[:F, 0].float()) and (z[:, F:] == 1).all()
+    _, dw1, dw2 = tfb.gated_ffn_bwd(x, w1, w2, z, dy, NAMES[act])
+    ref = gated_ffn64(x, w1, w2, act, dy=dy)
+    assert torch.isfinite(y).all() and torch.isfinite(dw1).all() and torch.isfinite(dw2).all()
+    assert_within("dw_gate_up", dw1, ref["dw_gate_up"])
+    a = dw2[0].double() / (m * 0.125)                                            # mean of a
+    want = torch.where(g.double() > 8, w1[:F, 0].double(), torch.zeros_like(a))
+    far = g.abs() > 8
+    assert ((a - want).abs()[far] <= 3 * U * want.abs()[far] + 1e-6).all()
+
+
 def test_skipped_gradients_and_no_tokens(cuda_device):
     import teenyformers_b200 as tfb
     for m, d, F in ((129, 136, 2776), (4100, 64, 72), (70, 136, 264)):
