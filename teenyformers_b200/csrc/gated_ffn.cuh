@@ -842,6 +842,14 @@ __global__ void __launch_bounds__(kTileThreads)
   const int j0 = (int)blockIdx.x / p.n_tt * ROWS, t0 = (int)blockIdx.x % p.n_tt * NT;
   const int kb0 = (int)((long long)p.n_kblk * rank / S);
   const int n_kb = (int)((long long)p.n_kblk * (rank + 1) / S) - kb0;  // at least 1
+  // Row tiles start at different k-blocks of their run and wrap: all at the same
+  // one read the same lines of X at once (1, 64, 128 tokens x 4096 x 14336:
+  // 59.8, 67.6, 80.2 us without, 57.3, 64.7, 75.8 with).
+  const int first_kb = (int)blockIdx.x / p.n_tt * 5 % n_kb;
+  auto k_of = [&](int kb) {
+    kb += first_kb;
+    return (kb0 + (kb < n_kb ? kb : kb - n_kb)) * 64;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -868,7 +876,7 @@ __global__ void __launch_bounds__(kTileThreads)
   if (warp == 0) {
     auto load_a = [&](int kb, int s) {
       const uint32_t sa = sbase + s * C::STAGE_BYTES;
-      const int k = (kb0 + kb) * 64;
+      const int k = k_of(kb);
       tma_load_2d(sa, &tm_a, full(s), k, j0);
       if (MODE == FFN_GLU) tma_load_2d(sa + 8192, &tm_a, full(s), k, p.J + j0);
     };
@@ -893,7 +901,7 @@ __global__ void __launch_bounds__(kTileThreads)
           mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
           load_a(kb, s);
         }
-        tma_load_2d(sbase + s * C::STAGE_BYTES + C::A_BYTES, &tm_b, full(s), (kb0 + kb) * 64, t0);
+        tma_load_2d(sbase + s * C::STAGE_BYTES + C::A_BYTES, &tm_b, full(s), k_of(kb), t0);
       }
       __syncwarp();
       issued = kb + 1;
