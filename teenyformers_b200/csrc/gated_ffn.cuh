@@ -141,8 +141,8 @@ constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
 // (forward 2.12 ms), four the same but for FFN_GLU's z (+3%), three 7% more.
 template <int MODE>
 struct FfnPairCfg {
-  static constexpr int STAGES = MODE == FFN_DGLU ? 4 : 5;
-  static constexpr int EPI_BYTES = MODE == FFN_DGLU ? 12288 : 8192;  // a warp's
+  static constexpr int STAGES = 5;
+  static constexpr int EPI_BYTES = 8192;  // a warp's
   static constexpr int A_BYTES = 128 * kGemmBK * 2;  // this CTA's 128 rows of A
   static constexpr int B_BYTES = 128 * kGemmBK * 2;  // and of B
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -153,8 +153,8 @@ struct FfnPairCfg {
   static_assert(SMEM_ALLOC <= 232448, "the pair kernel's shared memory exceeds the limit");
   // barriers
   static constexpr int FULL = 0, EMPTY = STAGES, AFULL = 2 * STAGES, AEMPTY = AFULL + 2,
-                       DRAIN = AEMPTY + 2, Z = DRAIN + 1 /* FFN_DGLU: two a warp */,
-                       COUNT = Z + 2 * kFfnEpiWarps;
+                       DRAIN = AEMPTY + 2, Z = DRAIN + 1 /* FFN_DGLU: one a warp */,
+                       COUNT = Z + kFfnEpiWarps;
   static_assert((COUNT + 1) * 8 <= 512, "barriers");
 };
 
@@ -234,7 +234,7 @@ __device__ __forceinline__ float4 ffn_unstage32(uint32_t stg, int it, int lane) 
 // epilogues of short products (FFN_DGLU 17 us a tile).  Bulk stores clip rows
 // past M and columns past the output's.  wait_acc() blocks until the
 // accumulator is complete; what does not depend on it is loaded first.
-// zbar: this warp's two barriers, zn: its z chunks so far (FFN_DGLU).
+// zbar: this warp's barrier, zn: its z chunks so far (FFN_DGLU).
 template <int MODE, int ACT, class Wait, class Release>
 __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const FfnProblem& q,
                                                   const FfnMaps& maps, int k, int split,
@@ -308,72 +308,69 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       }
     }
   } else if constexpr (MODE == FFN_DGLU) {
-    // chunks of 16 columns: z comes in through the two halves (gate 2 KB, up
-    // 2 KB: 64-byte rows), two chunks ahead; dg, du and a go out through the
-    // third 4 KB (1 KB each: 32-byte rows)
+    // chunks of 16 columns: z comes in through the first 4 KB (gate 2 KB, up 2 KB:
+    // 64-byte rows), the next chunk's as soon as a chunk's is in registers; dg,
+    // du and a go out through the second (1 KB each: 32-byte rows)
     const int half_cols = q.bn / 2, chunks = q.bn / 32;
     const int col_h = nb * q.bn + hf * half_cols;
-    const uint32_t out = stg + 8192;
-    auto load_z = [&](int c) {  // (lane 0) chunk c of this tile into half c % 2
-      const uint32_t dst = stg + (c & 1) * 4096, bar = zbar + (c & 1) * 8;
-      mbar_arrive_expect_tx(bar, 4096);
-      tma_load_3d(dst, &maps.out[2], bar, col_h + c * 16, 0, row0);
-      tma_load_3d(dst + 2048, &maps.out[2], bar, col_h + c * 16, 1, row0);
+    const uint32_t out = stg + 4096;
+    auto load_z = [&](int c) {  // (lane 0)
+      mbar_arrive_expect_tx(zbar, 4096);
+      tma_load_3d(stg, &maps.out[2], zbar, col_h + c * 16, 0, row0);
+      tma_load_3d(stg + 2048, &maps.out[2], zbar, col_h + c * 16, 1, row0);
     };
-    if (lane == 0) {
-      load_z(0);
-      load_z(1);
-    }
+    if (lane == 0) load_z(0);
     __syncwarp();
     // a load of z needs nothing of the other roles: its wait does not look at
-    // their giving up, and the loads have landed when this warp does
-    auto wait_z = [&](int i) {
-      return mbar_wait_warp(zbar + (i & 1) * 8, (i >> 1) & 1, nullptr, 927);
-    };
+    // their giving up, and the load has landed when this warp does
+    auto wait_z = [&]() { return mbar_wait_warp(zbar, zn++ & 1, nullptr, 927); };
     if (!wait_acc()) {
-      (void)wait_z(zn);
-      (void)wait_z(zn + 1);
+      (void)wait_z();
       return false;
     }
-    for (int c = 0; c < chunks; ++c, ++zn) {  // (chunk zn of this warp is in half zn % 2 = c % 2)
+    for (int c = 0; c < chunks; ++c) {
       uint32_t r[16];
       tmem_ld16(acc + hf * half_cols + c * 16, r);
-      tmem_wait_ld();
-      if (c == chunks - 1) release_acc();
-      if (!wait_z(zn)) return false;
-      const uint32_t buf = stg + (c & 1) * 4096;
-      uint32_t dg[8], du[8], av[8];
+      if (!wait_z()) return false;
+      uint4 g4[4], u4[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t at = buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
-        const uint4 g4 = gemm_lds128(at), u4 = gemm_lds128(at + 2048);
-        const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
-        float x[4], y[4], w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float value, slope;
-          const float d = __uint_as_float(r[4 * j + e]), u = __uint_as_float(uw[e]);
-          ffn_act_grad<ACT>(__uint_as_float(gw[e]), value, slope);
-          w[e] = value * u;
-          y[e] = d * value;
-          x[e] = d * u * slope;
-        }
-        dg[2 * j] = pack_bf16x2(x[0], x[1]), dg[2 * j + 1] = pack_bf16x2(x[2], x[3]);
-        du[2 * j] = pack_bf16x2(y[0], y[1]), du[2 * j + 1] = pack_bf16x2(y[2], y[3]);
-        av[2 * j] = pack_bf16x2(w[0], w[1]), av[2 * j + 1] = pack_bf16x2(w[2], w[3]);
+        const uint32_t at = stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+        g4[j] = gemm_lds128(at), u4[j] = gemm_lds128(at + 2048);
       }
+      tmem_wait_ld();
+      if (c == chunks - 1) release_acc();
       __syncwarp();  // every lane has read its z
       if (lane == 0) {
-        if (c + 2 < chunks) load_z(c + 2);
+        if (c + 1 < chunks) load_z(c + 1);
         bulk_wait_group_read0();  // the chunk before has left `out`
       }
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t at = out + lane * 32 + ((j ^ ((lane >> 2) & 1)) << 4);
-        gemm_sts128(at, dg[4 * j], dg[4 * j + 1], dg[4 * j + 2], dg[4 * j + 3]);
-        gemm_sts128(at + 1024, du[4 * j], du[4 * j + 1], du[4 * j + 2], du[4 * j + 3]);
-        gemm_sts128(at + 2048, av[4 * j], av[4 * j + 1], av[4 * j + 2], av[4 * j + 3]);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t dg[4], du[4], av[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 gq = g4[2 * h + j], uq = u4[2 * h + j];
+          const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w}, uw[4] = {uq.x, uq.y, uq.z, uq.w};
+          float x[4], y[4], w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float value, slope;
+            const float d = __uint_as_float(r[8 * h + 4 * j + e]), u = __uint_as_float(uw[e]);
+            ffn_act_grad<ACT>(__uint_as_float(gw[e]), value, slope);
+            w[e] = value * u;
+            y[e] = d * value;
+            x[e] = d * u * slope;
+          }
+          dg[2 * j] = pack_bf16x2(x[0], x[1]), dg[2 * j + 1] = pack_bf16x2(x[2], x[3]);
+          du[2 * j] = pack_bf16x2(y[0], y[1]), du[2 * j + 1] = pack_bf16x2(y[2], y[3]);
+          av[2 * j] = pack_bf16x2(w[0], w[1]), av[2 * j + 1] = pack_bf16x2(w[2], w[3]);
+        }
+        const uint32_t at = out + lane * 32 + ((h ^ ((lane >> 2) & 1)) << 4);
+        gemm_sts128(at, dg[0], dg[1], dg[2], dg[3]);
+        gemm_sts128(at + 1024, du[0], du[1], du[2], du[3]);
+        gemm_sts128(at + 2048, av[0], av[1], av[2], av[3]);
       }
       staged();
       if (lane == 0) {
@@ -507,7 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       mbar_init(bar(C::AEMPTY + b), 2 * kFfnEpiWarps);  // both CTAs'
     }
     mbar_init(bar(C::DRAIN), 1);
-    for (int i = 0; i < 2 * kFfnEpiWarps; ++i) mbar_init(bar(C::Z + i), 1);
+    for (int i = 0; i < kFfnEpiWarps; ++i) mbar_init(bar(C::Z + i), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -654,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         if (lane == 0) mbar_arrive_remote(aempty0 + b * 8);
       };
       if (!ffn_epilogue_warp<MODE, ACT>(p, q, maps, item.k, item.split, acc, row0, item.nb, hf,
-                                        lane, stg, bar(C::Z + 2 * (warp - 2)), zn, wait_acc, release_acc))
+                                        lane, stg, bar(C::Z + warp - 2), zn, wait_acc, release_acc))
         break;
     }
     if (lane == 0) bulk_wait_group0();  // the stores, before the shared memory goes away
