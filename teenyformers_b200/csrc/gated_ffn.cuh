@@ -97,6 +97,7 @@ enum FfnMode : int {
   FFN_GLU = 0,    // A = x, B = W (gate rows to the even CTA, up rows to the odd one): a (, z)
   FFN_DGLU = 1,   // A = dy, B = Wd read MN-major: dz and a from z and the product da
   FFN_STORE = 2,  // up to three products, each rounded to bf16 (+ residual)
+  FFN_DGLU_LONG = 3,  // FFN_DGLU for a long K: one more stage, less of the epilogue's memory
 };
 
 constexpr int kFfnMaxProblems = 3;
@@ -137,12 +138,13 @@ constexpr int kFfnEpiWarps = 8;
 constexpr int kFfnThreads = 64 + kFfnEpiWarps * 32;
 
 // The pair kernel's shared memory: a ring of 32 KB stages, and each epilogue
-// warp's part.  Of 8192 x 4096 x 14336, five stages and six take the same time
-// (forward 2.12 ms), four the same but for FFN_GLU's z (+3%), three 7% more.
+// warp's part.  A long K wants the sixth stage (8192 x 2048 x 5632 forward 450
+// us, with five 470; z saved 483, with five 524); FFN_DGLU's epilogue is the
+// longer part of a tile with a short K, and there has 8 KB a warp.
 template <int MODE>
 struct FfnPairCfg {
-  static constexpr int STAGES = 5;
-  static constexpr int EPI_BYTES = 8192;  // a warp's
+  static constexpr int STAGES = MODE == FFN_DGLU ? 5 : 6;
+  static constexpr int EPI_BYTES = MODE == FFN_DGLU ? 8192 : 4096;  // a warp's
   static constexpr int A_BYTES = 128 * kGemmBK * 2;  // this CTA's 128 rows of A
   static constexpr int B_BYTES = 128 * kGemmBK * 2;  // and of B
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -246,14 +248,10 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
     release_acc();
     return true;
   }
-  // the two 4 KB halves of stg in turn: the half is free once the store
-  // before last has read it
-  int half = 0;
-  auto next_half = [&]() {
-    if (lane == 0) bulk_wait_group_read1();
+  // stg is free again once the store before has read it
+  auto free_stg = [&]() {
+    if (lane == 0) bulk_wait_group_read0();
     __syncwarp();
-    half ^= 1;
-    return stg + half * 4096;
   };
   // a lane's 32 fp32 as a 128-byte row, chunks XOR-swizzled by row
   auto stage32 = [&](uint32_t buf, const uint32_t (&r)[32]) {
@@ -278,7 +276,7 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_wait_ld();
       if (hh == 1) release_acc();
       // a: 64-byte rows of 16-byte chunks, XOR-swizzled by pairs of rows
-      const uint32_t ab = next_half();
+      free_stg();
 #pragma unroll
       for (int jc = 0; jc < 4; ++jc) {
         uint32_t w[4];
@@ -288,38 +286,43 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
           w[e] = pack_bf16x2(ffn_act<ACT>(__uint_as_float(gr[i])) * __uint_as_float(ur[i]),
                              ffn_act<ACT>(__uint_as_float(gr[i + 1])) * __uint_as_float(ur[i + 1]));
         }
-        gemm_sts128(ab + lane * 64 + ((jc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+        gemm_sts128(stg + lane * 64 + ((jc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
       }
       staged();
       const bool inside = lane == 0 && col0 < p.F;  // (a box wholly past the edge is not stored)
-      if (inside) tma_store_2d(&maps.out[0], ab, col0, row0);
+      if (inside) tma_store_2d(&maps.out[0], stg, col0, row0);
       if (lane == 0) bulk_commit_group();
       if (p.z) {
-        uint32_t zb = next_half();
-        stage32(zb, gr);
+        free_stg();
+        stage32(stg, gr);
         staged();
-        if (inside) tma_store_3d(&maps.out[1], zb, col0, 0, row0);
+        if (inside) tma_store_3d(&maps.out[1], stg, col0, 0, row0);
         if (lane == 0) bulk_commit_group();
-        zb = next_half();
-        stage32(zb, ur);
+        free_stg();
+        stage32(stg, ur);
         staged();
-        if (inside) tma_store_3d(&maps.out[1], zb, col0, 1, row0);
+        if (inside) tma_store_3d(&maps.out[1], stg, col0, 1, row0);
         if (lane == 0) bulk_commit_group();
       }
     }
-  } else if constexpr (MODE == FFN_DGLU) {
+  } else if constexpr (MODE == FFN_DGLU || MODE == FFN_DGLU_LONG) {
     // chunks of 16 columns: z comes in through the first 4 KB (gate 2 KB, up 2 KB:
-    // 64-byte rows), the next chunk's as soon as a chunk's is in registers; dg,
-    // du and a go out through the second (1 KB each: 32-byte rows)
+    // 64-byte rows), dg, du and a go out (1 KB each: 32-byte rows) through the
+    // second, and the next chunk's z is asked for as soon as a chunk's is in
+    // registers; or (LONG) out through the first, and z after that
+    constexpr bool LONG = MODE == FFN_DGLU_LONG;
     const int half_cols = q.bn / 2, chunks = q.bn / 32;
     const int col_h = nb * q.bn + hf * half_cols;
-    const uint32_t out = stg + 4096;
+    const uint32_t out = LONG ? stg : stg + 4096;
     auto load_z = [&](int c) {  // (lane 0)
       mbar_arrive_expect_tx(zbar, 4096);
       tma_load_3d(stg, &maps.out[2], zbar, col_h + c * 16, 0, row0);
       tma_load_3d(stg + 2048, &maps.out[2], zbar, col_h + c * 16, 1, row0);
     };
-    if (lane == 0) load_z(0);
+    if (lane == 0) {
+      if (LONG) bulk_wait_group_read0();  // the tile before
+      load_z(0);
+    }
     __syncwarp();
     // a load of z needs nothing of the other roles: its wait does not look at
     // their giving up, and the load has landed when this warp does
@@ -341,11 +344,13 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_wait_ld();
       if (c == chunks - 1) release_acc();
       __syncwarp();  // every lane has read its z
-      if (lane == 0) {
-        if (c + 1 < chunks) load_z(c + 1);
-        bulk_wait_group_read0();  // the chunk before has left `out`
+      if (!LONG) {
+        if (lane == 0) {
+          if (c + 1 < chunks) load_z(c + 1);
+          bulk_wait_group_read0();  // the chunk before has left `out`
+        }
+        __syncwarp();
       }
-      __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t dg[4], du[4], av[4];
@@ -381,6 +386,10 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
           tma_store_2d(&maps.out[0], out + 2048, col, row0);
         }
         bulk_commit_group();
+        if (LONG && c + 1 < chunks) {
+          bulk_wait_group_read0();
+          load_z(c + 1);
+        }
       }
     }
   } else if (q.residual) {
@@ -432,11 +441,11 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_ld32(acc + hf * 128 + c * 32, r);
       tmem_wait_ld();
       if (c == 3) release_acc();
-      const uint32_t buf = next_half();
-      stage32(buf, r);
+      free_stg();
+      stage32(stg, r);
       staged();
       if (lane == 0) {
-        if (col0 < q.N) tma_store_3d(&maps.out[k], buf, col0, row0, split);
+        if (col0 < q.N) tma_store_3d(&maps.out[k], stg, col0, row0, split);
         bulk_commit_group();
       }
     }
@@ -449,7 +458,7 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_ld32(acc + hf * 128 + c * 64 + 32, r1);
       tmem_wait_ld();
       if (c == 1) release_acc();
-      const uint32_t buf = next_half();
+      free_stg();
 #pragma unroll
       for (int jc = 0; jc < 8; ++jc) {
         uint32_t w[4];
@@ -459,11 +468,11 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
           w[e] = pack_bf16x2(__uint_as_float(i < 32 ? r0[i] : r1[i - 32]),
                              __uint_as_float(i + 1 < 32 ? r0[i + 1] : r1[i + 1 - 32]));
         }
-        gemm_sts128(buf + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+        gemm_sts128(stg + lane * 128 + ((jc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
       }
       staged();
       if (lane == 0) {
-        if (col0 < q.N) tma_store_2d(&maps.out[k], buf, col0, row0);
+        if (col0 < q.N) tma_store_2d(&maps.out[k], stg, col0, row0);
         bulk_commit_group();
       }
     }
@@ -516,7 +525,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     tma_prefetch_desc(&maps.a[lane]);
     tma_prefetch_desc(&maps.b[lane]);
   }
-  if (warp == 2 && lane < (MODE == FFN_GLU ? 1 + (p.z != nullptr) : MODE == FFN_DGLU ? 3 : p.n_prob))
+  if (warp == 2 && lane < (MODE == FFN_GLU     ? 1 + (p.z != nullptr)
+                             : MODE == FFN_STORE ? p.n_prob
+                                                 : 3))
     tma_prefetch_desc(&maps.out[lane]);
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers initialised before any remote signal

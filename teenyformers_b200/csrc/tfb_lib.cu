@@ -149,8 +149,14 @@ int ensure_device_setup() {
     set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU>, FfnPairCfg<FFN_GLU>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_GLU, FFN_ACT_GELU_TANH>, FfnPairCfg<FFN_GLU>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_SILU>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU_LONG, FFN_ACT_SILU>,
+        FfnPairCfg<FFN_DGLU_LONG>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU_LONG, FFN_ACT_GELU>,
+        FfnPairCfg<FFN_DGLU_LONG>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_DGLU, FFN_ACT_GELU_TANH>, FfnPairCfg<FFN_DGLU>::SMEM_ALLOC);
+    set((const void*)ffn_pair_kernel<FFN_DGLU_LONG, FFN_ACT_GELU_TANH>,
+        FfnPairCfg<FFN_DGLU_LONG>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, FfnPairCfg<FFN_STORE>::SMEM_ALLOC);
 #define TFB_TILE_SET(NT)                                                            \
   set((const void*)ffn_tile_kernel<NT, FFN_GLU>, TileCfg<NT>::SMEM_ALLOC);          \
@@ -1343,7 +1349,11 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
       !ffn_box(&maps.out[1], dz, d_ff, m, 1, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !ffn_box(&maps.out[2], z, d_ff, m, 1, 16, kF32, CU_TENSOR_MAP_SWIZZLE_64B))
     return TF_ERR_CUDA;
-  if (int e = ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st)) return e;
+  // (a tile's epilogue takes as long as some 24 k-blocks, or 40 with LONG's memory)
+  const bool long_k = q.bn == kGemmBN && q.n_kblk >= 40;
+  if (int e = long_k ? ffn_pair_launch_act<FFN_DGLU_LONG>(act, maps, prm, st)
+                     : ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st))
+    return e;
 
   // the three products that follow in one launch, those with the longer (run of) K first
   const FfnBwdPlan plan = ffn_bwd_plan(m, d_model, d_ff);
