@@ -97,7 +97,7 @@ enum FfnMode : int {
   FFN_GLU = 0,    // A = x, B = W (gate rows to the even CTA, up rows to the odd one): a (, z)
   FFN_DGLU = 1,   // A = dy, B = Wd read MN-major: dz and a from z and the product da
   FFN_STORE = 2,  // up to three products, each rounded to bf16 (+ residual)
-  FFN_DGLU_LONG = 3,  // FFN_DGLU for a long K: one more stage, less of the epilogue's memory
+  FFN_DGLU_LONG = 3,  // FFN_DGLU for a long K: its z, dz and a by the lanes' loads and stores
 };
 
 constexpr int kFfnMaxProblems = 3;
@@ -216,6 +216,10 @@ __device__ __forceinline__ FfnItem ffn_item(const FfnPairParams& p, int t) {
   return it;
 }
 
+__device__ __forceinline__ uint2 ffn_pack4(const float (&v)[4]) {
+  return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
 // Reads 32 staged rows of 32 fp32 (128-byte rows, 16-byte chunks XOR-swizzled by
 // row) 4 columns a lane: iteration `it` gives row it * 4 + lane / 8, columns
 // 4 (lane % 8)..
@@ -305,24 +309,75 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
         if (lane == 0) bulk_commit_group();
       }
     }
-  } else if constexpr (MODE == FFN_DGLU || MODE == FFN_DGLU_LONG) {
+  } else if constexpr (MODE == FFN_DGLU_LONG) {
+    // under a long main loop the time of this does not show, but its bulk copies
+    // did, which wait for one another with the operands' (4096 x 4096 x 4096: 126
+    // us, so 117): here the lanes load and store themselves, 4 columns each of
+    // rows of 32
+    const int rows_valid = q.M - row0;
+    const int r4 = lane >> 3, c4 = (lane & 7) * 4;  // ffn_unstage32: row in a group of 4, column
+    float4 g[8], u[8];
+    auto load_z = [&](int c) {
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < p.F) {
+          const float* zr = p.z + (long long)(row0 + rr) * 2 * p.F + col;
+          g[it] = *reinterpret_cast<const float4*>(zr);
+          u[it] = *reinterpret_cast<const float4*>(zr + p.F);
+        }
+      }
+    };
+    load_z(0);
+    if (!wait_acc()) return false;
+    for (int c = 0; c < 4; ++c) {
+      uint32_t r[32];
+      tmem_ld32(acc + hf * 128 + c * 32, r);
+      tmem_wait_ld();
+      if (c == 3) release_acc();
+      stage32(stg, r);
+      __syncwarp();
+      const int col = nb * kGemmBN + hf * 128 + c * 32 + c4;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const float4 d4 = ffn_unstage32(stg, it, lane);
+        const int rr = it * 4 + r4;
+        if (rr < rows_valid && col < p.F) {
+          const float d[4] = {d4.x, d4.y, d4.z, d4.w};
+          const float gv[4] = {g[it].x, g[it].y, g[it].z, g[it].w};
+          const float uv[4] = {u[it].x, u[it].y, u[it].z, u[it].w};
+          float dg[4], du[4], av[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float value, slope;
+            ffn_act_grad<ACT>(gv[e], value, slope);
+            av[e] = value * uv[e];
+            du[e] = d[e] * value;
+            dg[e] = d[e] * uv[e] * slope;
+          }
+          __nv_bfloat16* dz = p.dz + (long long)(row0 + rr) * 2 * p.F + col;
+          *reinterpret_cast<uint2*>(dz) = ffn_pack4(dg);
+          *reinterpret_cast<uint2*>(dz + p.F) = ffn_pack4(du);
+          *reinterpret_cast<uint2*>(p.a + (long long)(row0 + rr) * p.F + col) = ffn_pack4(av);
+        }
+      }
+      if (c < 3) load_z(c + 1);
+      __syncwarp();
+    }
+  } else if constexpr (MODE == FFN_DGLU) {
     // chunks of 16 columns: z comes in through the first 4 KB (gate 2 KB, up 2 KB:
-    // 64-byte rows), dg, du and a go out (1 KB each: 32-byte rows) through the
-    // second, and the next chunk's z is asked for as soon as a chunk's is in
-    // registers; or (LONG) out through the first, and z after that
-    constexpr bool LONG = MODE == FFN_DGLU_LONG;
+    // 64-byte rows), the next chunk's as soon as a chunk's is in registers; dg,
+    // du and a go out through the second (1 KB each: 32-byte rows)
     const int half_cols = q.bn / 2, chunks = q.bn / 32;
     const int col_h = nb * q.bn + hf * half_cols;
-    const uint32_t out = LONG ? stg : stg + 4096;
+    const uint32_t out = stg + 4096;
     auto load_z = [&](int c) {  // (lane 0)
       mbar_arrive_expect_tx(zbar, 4096);
       tma_load_3d(stg, &maps.out[2], zbar, col_h + c * 16, 0, row0);
       tma_load_3d(stg + 2048, &maps.out[2], zbar, col_h + c * 16, 1, row0);
     };
-    if (lane == 0) {
-      if (LONG) bulk_wait_group_read0();  // the tile before
-      load_z(0);
-    }
+    if (lane == 0) load_z(0);
     __syncwarp();
     // a load of z needs nothing of the other roles: its wait does not look at
     // their giving up, and the load has landed when this warp does
@@ -344,13 +399,11 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
       tmem_wait_ld();
       if (c == chunks - 1) release_acc();
       __syncwarp();  // every lane has read its z
-      if (!LONG) {
-        if (lane == 0) {
-          if (c + 1 < chunks) load_z(c + 1);
-          bulk_wait_group_read0();  // the chunk before has left `out`
-        }
-        __syncwarp();
+      if (lane == 0) {
+        if (c + 1 < chunks) load_z(c + 1);
+        bulk_wait_group_read0();  // the chunk before has left `out`
       }
+      __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t dg[4], du[4], av[4];
@@ -386,10 +439,6 @@ __device__ __forceinline__ bool ffn_epilogue_warp(const FfnPairParams& p, const 
           tma_store_2d(&maps.out[0], out + 2048, col, row0);
         }
         bulk_commit_group();
-        if (LONG && c + 1 < chunks) {
-          bulk_wait_group_read0();
-          load_z(c + 1);
-        }
       }
     }
   } else if (q.residual) {
@@ -527,7 +576,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   }
   if (warp == 2 && lane < (MODE == FFN_GLU     ? 1 + (p.z != nullptr)
                              : MODE == FFN_STORE ? p.n_prob
-                                                 : 3))
+                             : MODE == FFN_DGLU  ? 3
+                                                 : 0))
     tma_prefetch_desc(&maps.out[lane]);
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers initialised before any remote signal
@@ -757,9 +807,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
                : "r"(cluster_addr)
                : "memory");
   return v;
-}
-__device__ __forceinline__ uint2 ffn_pack4(const float (&v)[4]) {
-  return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 // What is done with four joined outputs v (FFN_GLU: and the four u beside

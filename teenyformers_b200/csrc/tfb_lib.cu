@@ -1349,8 +1349,8 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
       !ffn_box(&maps.out[1], dz, d_ff, m, 1, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !ffn_box(&maps.out[2], z, d_ff, m, 1, 16, kF32, CU_TENSOR_MAP_SWIZZLE_64B))
     return TF_ERR_CUDA;
-  // (a tile's epilogue takes as long as some 24 k-blocks, or 40 with LONG's memory)
-  const bool long_k = q.bn == kGemmBN && q.n_kblk >= 40;
+  // (FFN_DGLU_LONG's epilogue takes as long as some 48 k-blocks)
+  const bool long_k = q.bn == kGemmBN && q.n_kblk >= 48;
   if (int e = long_k ? ffn_pair_launch_act<FFN_DGLU_LONG>(act, maps, prm, st)
                      : ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st))
     return e;

@@ -33,7 +33,9 @@ SIZES = [(1, 8, 8), (1, 64, 128), (2, 520, 1416), (3, 72, 136), (7, 4096, 512), 
          (17, 128, 72), (33, 264, 1000), (64, 520, 200), (65, 136, 264), (128, 256, 1024),
          (129, 256, 128), (200, 64, 64), (300, 520, 1416), (513, 1032, 264),
          # few tiles and a long sum: of dx, of the weights' gradients, ragged
-         (129, 520, 2776), (5, 8, 5000), (4100, 64, 72), (2056, 8, 8)]
+         (129, 520, 2776), (5, 8, 5000), (4100, 64, 72), (2056, 8, 8),
+         # every product in 256 x 256 tiles, a long K in each
+         (1030, 3208, 2568)]
 
 
 @pytest.mark.parametrize("m,d,F", SIZES)
