@@ -1174,9 +1174,6 @@ int ffn_tile_launch_nt(const void* w, int w_rows, const void* x, int k, FfnTileP
 // their SMs are busy: a k-block costs an SM of the pair kernel 32 KB and each
 // tile of the tile kernel 16 KB for its weights and 128 bytes a token.
 bool ffn_use_tiles(int J, int T, int rows, int pair_cols) {
-#ifdef TFB_FORCE_TILES
-  return TFB_FORCE_TILES;
-#endif
   const long long tiles = (long long)((J + rows - 1) / rows) * ((T + 127) / 128);
   const long long pairs = (long long)((J + pair_cols - 1) / pair_cols) * ((T + 255) / 256);
   const int n_pairs = std::max(1, g_pair_clusters[current_device()]);
@@ -1349,8 +1346,9 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
       !ffn_box(&maps.out[1], dz, d_ff, m, 1, 16, kBf16, CU_TENSOR_MAP_SWIZZLE_32B) ||
       !ffn_box(&maps.out[2], z, d_ff, m, 1, 16, kF32, CU_TENSOR_MAP_SWIZZLE_64B))
     return TF_ERR_CUDA;
-  // (FFN_DGLU_LONG's epilogue takes as long as some 48 k-blocks)
-  const bool long_k = q.bn == kGemmBN && q.n_kblk >= 48;
+  // (the whole backward pass with FFN_DGLU_LONG and with FFN_DGLU: 4096 x K x 4096
+  // at K = 1024, 2048, 2560, 4096: 191, 321, 410, 680 us and 188, 321, 426, 688)
+  const bool long_k = q.bn == kGemmBN && q.n_kblk >= 32;
   if (int e = long_k ? ffn_pair_launch_act<FFN_DGLU_LONG>(act, maps, prm, st)
                      : ffn_pair_launch_act<FFN_DGLU>(act, maps, prm, st))
     return e;

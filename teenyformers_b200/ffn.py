@@ -13,7 +13,7 @@ scales on the branch, dropout.
 ``post_norm``, ``gate`` and ``next_norm`` are optional.  Forward: three launches
 and a fourth for the first norm, which a caller that has h (the sublayer
 before's ``hn``) saves; any number of tokens, from one decoding token on.
-Backward: six.
+Backward: six, and a seventh where few tiles have their sums split.
 """
 from __future__ import annotations
 

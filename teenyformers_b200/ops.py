@@ -22,6 +22,7 @@ here a bad call raises ValueError (shape) or TfError (status from the C ABI).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -357,11 +358,14 @@ def _launch(x: torch.Tensor, name: str, *args) -> None:
     device current (the library launches on the current device)."""
     index = x.get_device()
     stream = torch._C._cuda_getCurrentRawStream(index)
+    fn = getattr(_capi.lib(), name)
     if index == torch._C._cuda_getDevice():
-        call(name, *args, stream)
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            call(name, *args, stream)
+            rc = fn(*args, stream)
+    if rc:
+        raise TfError(name, rc)
 
 
 def _addr(t: torch.Tensor | None):
@@ -419,6 +423,11 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
     return (y, z) if save else y
 
 
+@functools.lru_cache(maxsize=256)
+def _ffn_workspace_size(m: int, d: int, d_ff: int) -> int:  # (of the shape alone)
+    return _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d, d_ff)
+
+
 def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, z: torch.Tensor,
                   dy: torch.Tensor, act: int = TF_ACT_SILU, grads=None, need=(True, True, True),
                   workspace: torch.Tensor | None = None):
@@ -434,8 +443,7 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor
     g = [None if not on else torch.empty_like(like) if t is None
          else _buffer(t, like.shape, torch.bfloat16, x, "a gradient")
          for t, like, on in zip(given, (x, w_gate_up, w_down), need)]
-    n = _capi.raw("tf_b200_gated_ffn_bwd_workspace_size", m, d, d_ff)
-    ws = _workspace(n, workspace, x)
+    ws = _workspace(_ffn_workspace_size(m, d, d_ff), workspace, x)
     _launch(x, "tf_b200_gated_ffn_bwd_bf16", x.data_ptr(), w_gate_up.data_ptr(),
             w_down.data_ptr(), z.data_ptr(), dy.data_ptr(), _addr(g[0]), _addr(g[1]), _addr(g[2]),
             ws.data_ptr(), m, d, d_ff, int(act))
@@ -469,12 +477,15 @@ def _workspace(n: int, ws: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor
     return ws
 
 
+_DROPOUT = {torch.float32: "tf_b200_dropout_f32", torch.bfloat16: "tf_b200_dropout_bf16"}
+
+
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
             residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """dropout(x) (+ residual), bf16 or fp32, the mask drawn from (rng, site) by a
     counter-based generator and never stored.  The backward pass is
     ``dropout(dy, p, rng, site)``.  ``out`` may be x or residual."""
-    fn = {torch.float32: "tf_b200_dropout_f32", torch.bfloat16: "tf_b200_dropout_bf16"}.get(x.dtype)
+    fn = _DROPOUT.get(x.dtype)
     if fn is None:
         raise ValueError(f"unsupported dtype {x.dtype}")
     _need(x.is_cuda, "x must be a CUDA tensor")
@@ -487,17 +498,24 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
 
 
 def _norm_shapes(x, w_post, gate, w_pre):
-    _need(x.is_cuda and x.dim() >= 1, "block_norm tensors must be [..., cols] CUDA tensors")
+    if not x.is_cuda or x.dim() < 1:
+        raise ValueError("block_norm tensors must be [..., cols] CUDA tensors")
     cols = x.shape[-1]
-    rows = x.numel() // max(cols, 1)
-    for w in (w_post, w_pre):
-        _need(w is None or w.numel() == cols, "a norm's weight must have the last dim's size")
-    gate_rows = 1
-    if gate is not None:
-        _need(gate.shape[-1] == cols, "gate must be [gate_rows, cols] or [cols]")
-        gate_rows = gate.numel() // max(cols, 1)
-        _need(gate_rows >= 1 and rows % gate_rows == 0, "the gate's rows must divide x's")
+    rows = x.numel() // (cols or 1)
+    if (w_post is not None and w_post.numel() != cols) or (
+            w_pre is not None and w_pre.numel() != cols):
+        raise ValueError("a norm's weight must have the last dim's size")
+    if gate is None:
+        return rows, cols, 1
+    _need(gate.dim() >= 1 and gate.shape[-1] == cols, "gate must be [gate_rows, cols] or [cols]")
+    gate_rows = gate.numel() // (cols or 1)
+    _need(gate_rows >= 1 and rows % gate_rows == 0, "the gate's rows must divide x's")
     return rows, cols, gate_rows
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_size(rows: int, cols: int) -> int:  # (of the shape alone)
+    return _capi.raw("tf_b200_block_norm_bwd_workspace_size", rows, cols)
 
 
 def block_norm(x: torch.Tensor, f: torch.Tensor | None, w_post: torch.Tensor | None = None,
@@ -538,18 +556,23 @@ def block_norm_bwd(f: torch.Tensor | None, y: torch.Tensor | None, dy: torch.Ten
     _need(like is not None, "dy or dh is needed")
     rows, cols, gate_rows = _norm_shapes(like, w_post, gate, w_pre)
     _dense(like, torch.bfloat16, "block_norm", f, y, dy, dh, w_post, gate, w_pre)
+    shape = like.shape
     for t in (f, y, dy, dh):
-        _need(t is None or t.shape == like.shape, "f, y, dy and dh must have one shape")
-    _need((w_pre is None) == (dh is None), "dh belongs to w_pre")
-    _need(w_pre is None or y is not None, "w_pre needs the forward's y")
-    _need(branch or (f is None and w_post is None and gate is None and not p),
-          "branch=False takes no f, w_post, gate or dropout")
-    _need(f is not None or (w_post is None and gate is None), "w_post and gate need f")
-    new = lambda t: None if t is None else torch.empty_like(t)
-    dx, df = torch.empty_like(like), torch.empty_like(like) if branch else None
-    dw_post, dgate, dw_pre = new(w_post), new(gate), new(w_pre)
-    n = _capi.raw("tf_b200_block_norm_bwd_workspace_size", rows, cols)
-    ws = _workspace(n, workspace, like)
+        if t is not None and t is not like and t.shape != shape:
+            raise ValueError("f, y, dy and dh must have one shape")
+    if (w_pre is None) != (dh is None):
+        raise ValueError("dh belongs to w_pre")
+    if w_pre is not None and y is None:
+        raise ValueError("w_pre needs the forward's y")
+    if f is None:
+        _need(w_post is None and gate is None, "w_post and gate need f")
+    _need(branch or (f is None and not p), "branch=False takes no f, w_post, gate or dropout")
+    dx = torch.empty_like(like)
+    df = torch.empty_like(like) if branch else None
+    dw_post = None if w_post is None else torch.empty_like(w_post)
+    dgate = None if gate is None else torch.empty_like(gate)
+    dw_pre = None if w_pre is None else torch.empty_like(w_pre)
+    ws = _workspace(_norm_workspace_size(rows, cols), workspace, like)
     _launch(like, "tf_b200_block_norm_bwd_bf16", _addr(f), _addr(y), _addr(dy), _addr(dh),
             _addr(w_post), _addr(gate), _addr(w_pre), dx.data_ptr(), _addr(df), _addr(dw_post),
             _addr(dgate), _addr(dw_pre), _rng_addr(p, rng, site, like), ws.data_ptr(), rows, cols,
