@@ -777,16 +777,19 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(const __grid_constant__ Ff
 //   all warps join the partials.
 constexpr int kTileThreads = 320;
 
-template <int NT>
+template <int NT, bool DEEP>
 struct TileCfg {
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int B_BYTES = NT * 64 * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 3;
+  // two CTAs an SM, or a ring twice as deep where there is one
+  static constexpr int STAGES = (NT <= 32 ? 5 : NT == 64 ? 4 : 3) * (DEEP ? 2 : 1);
   static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
   static constexpr int SMEM_ALLOC = OFF_BAR + 256 + 1024;
   static constexpr int TM_COLS = NT < 32 ? 32 : NT;
   static_assert(NT * 128 * 4 <= OFF_BAR, "the partial tile exceeds the ring");
+  static_assert(SMEM_ALLOC <= (DEEP ? 232448 : 115712), "shared memory");
+  static_assert((2 * STAGES + 2) * 8 <= 256, "barriers");
 };
 
 struct FfnTileParams {
@@ -881,11 +884,11 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, uint32_t part, 
   }
 }
 
-template <int NT, int MODE>
+template <int NT, int MODE, bool DEEP>
 __global__ void __launch_bounds__(kTileThreads)
     ffn_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_b, const FfnTileParams p) {
-  using C = TileCfg<NT>;
+  using C = TileCfg<NT, DEEP>;
   constexpr int ROWS = MODE == FFN_GLU ? 64 : 128;  // outputs of a tile
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);

@@ -158,13 +158,16 @@ int ensure_device_setup() {
     set((const void*)ffn_pair_kernel<FFN_DGLU_LONG, FFN_ACT_GELU_TANH>,
         FfnPairCfg<FFN_DGLU_LONG>::SMEM_ALLOC);
     set((const void*)ffn_pair_kernel<FFN_STORE, FFN_ACT_SILU>, FfnPairCfg<FFN_STORE>::SMEM_ALLOC);
-#define TFB_TILE_SET(NT)                                                            \
-  set((const void*)ffn_tile_kernel<NT, FFN_GLU>, TileCfg<NT>::SMEM_ALLOC);          \
-  set((const void*)ffn_tile_kernel<NT, FFN_STORE>, TileCfg<NT>::SMEM_ALLOC)
-    TFB_TILE_SET(16);
-    TFB_TILE_SET(32);
-    TFB_TILE_SET(64);
-    TFB_TILE_SET(128);
+#define TFB_TILE_SET(NT, DEEP)                                                            \
+  set((const void*)ffn_tile_kernel<NT, FFN_GLU, DEEP>, TileCfg<NT, DEEP>::SMEM_ALLOC);    \
+  set((const void*)ffn_tile_kernel<NT, FFN_STORE, DEEP>, TileCfg<NT, DEEP>::SMEM_ALLOC)
+    TFB_TILE_SET(16, false);
+    TFB_TILE_SET(32, false);
+    TFB_TILE_SET(32, true);
+    TFB_TILE_SET(64, false);
+    TFB_TILE_SET(64, true);
+    TFB_TILE_SET(128, false);
+    TFB_TILE_SET(128, true);
 #undef TFB_TILE_SET
     set((const void*)dropout_kernel<__nv_bfloat16>, kDropSmem);
     set((const void*)dropout_kernel<float>, kDropSmem);
@@ -1140,8 +1143,16 @@ int ffn_pair_launch_act(int act, const FfnMaps& maps, FfnPairParams& prm, cudaSt
 }
 
 // One product of the tile kernel: `w` has w_rows rows (FFN_GLU: 2 J) of k.
-// A cluster of S CTAs takes a tile: a power of two up to 8, until the launch
-// has 148 CTAs or a CTA's share of K falls under four k-blocks.
+// A cluster of S CTAs, a power of two, takes a tile.  Either one CTA an SM with
+// a ring twice as deep, where S <= 4 gives most SMs one and each run of K fills
+// the ring (fewer joins, loads further ahead: 128 tokens x 4096 x 14336 78.7 us
+// so 68.6, 300 x 1032 x 2776 27.0 so 22.9, 64 x 4096 x 14336 67.4 so 63.0); or as
+// many CTAs as 148 SMs want, two of them an SM, up to S = 8 and down to four
+// k-blocks a run.  Few tokens are bound by the weights' way from memory, for which
+// every SM has to load: 64 x 2048 x 5632 takes 25.4 us with one CTA on 88 of the
+// SMs and 24.3 with two on each, 8 x 4096 x 4096 25.3 with one on 128 of them and
+// 23.4.  A whole K a CTA of the down product, in one wave, is no faster either
+// (512 x 4096 x 4096 51.4 us, in two runs 50.4).
 template <int NT, int MODE>
 int ffn_tile_launch(const void* w, int w_rows, const void* x, int k, FfnTileParams& prm,
                     cudaStream_t st) {
@@ -1154,9 +1165,18 @@ int ffn_tile_launch(const void* w, int w_rows, const void* x, int k, FfnTilePara
   const long long tiles = (long long)((prm.J + ROWS - 1) / ROWS) * prm.n_tt;
   if (!fits_i32(tiles)) return TF_ERR_TOO_LARGE;
   int S = 1;
+  if constexpr (NT >= 32) {
+    using C = TileCfg<NT, true>;
+    while (S < 4 && tiles * S * 2 <= 148 && prm.n_kblk >= 8 * S) S *= 2;
+    if ((S > 1 || MODE == FFN_GLU) && tiles * S <= 148 &&
+        tiles * S >= (NT == 128 ? 74 : 111) && prm.n_kblk / S >= C::STAGES)
+      return launch_ex(ffn_tile_kernel<NT, MODE, true>, dim3((unsigned)tiles, (unsigned)S),
+                       kTileThreads, C::SMEM_ALLOC, st, S, prm.pdl, ta, tb, prm);
+    S = 1;
+  }
   while (S < 8 && tiles * S < 148 && prm.n_kblk >= 8 * S) S *= 2;
-  return launch_ex(ffn_tile_kernel<NT, MODE>, dim3((unsigned)tiles, (unsigned)S), kTileThreads,
-                   TileCfg<NT>::SMEM_ALLOC, st, S, prm.pdl, ta, tb, prm);
+  return launch_ex(ffn_tile_kernel<NT, MODE, false>, dim3((unsigned)tiles, (unsigned)S),
+                   kTileThreads, TileCfg<NT, false>::SMEM_ALLOC, st, S, prm.pdl, ta, tb, prm);
 }
 
 template <int MODE>

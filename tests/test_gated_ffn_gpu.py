@@ -35,7 +35,9 @@ SIZES = [(1, 8, 8), (1, 64, 128), (2, 520, 1416), (3, 72, 136), (7, 4096, 512), 
          # few tiles and a long sum: of dx, of the weights' gradients, ragged
          (129, 520, 2776), (5, 8, 5000), (4100, 64, 72), (2056, 8, 8),
          # every product in 256 x 256 tiles, a long K in each
-         (1030, 3208, 2568)]
+         (1030, 3208, 2568),
+         # a deep ring in clusters of one, two and four
+         (300, 1032, 2776), (130, 2568, 1032), (50, 4096, 4096), (20, 4096, 4096)]
 
 
 @pytest.mark.parametrize("m,d,F", SIZES)
