@@ -33,9 +33,10 @@
 
 namespace tfb {
 
-constexpr int kBnThreads = 256;
-constexpr int kBnWarps = kBnThreads / 32;
 constexpr int kBnMaxCols = 8192;
+// A CTA's warps and teams, for teams of WPR warps
+__host__ __device__ constexpr int bn_warps(int wpr) { return wpr > 8 ? wpr : 8; }
+__host__ __device__ constexpr int bn_teams(int wpr) { return bn_warps(wpr) / wpr; }
 
 struct BlockNormParams {
   const __nv_bfloat16* x;
@@ -51,9 +52,9 @@ struct BlockNormParams {
 };
 
 // ---------------------------------------------------------------- teams and rings
-// A row is worked on by a team of WPR warps (the smallest of 1, 2, 4, 8 that
-// holds it at VPT 16-byte vectors a thread); a 256-thread CTA has 8 / WPR
-// teams, each with a contiguous run of rows.  The rows' tensors arrive through
+// A row is worked on by a team of WPR warps (the smallest of 1, 2, 4, 8, 16 that
+// holds it at VPT 16-byte vectors a thread); a CTA of 256 threads has 8 / WPR
+// teams, one of 512 a team of 16 warps.  The rows' tensors arrive through
 // a ring of shared-memory stages, filled by bulk copies of one or several
 // whole rows (rows are contiguous), so the loads of the next rows run under
 // the arithmetic and the two reductions of this one: with plain loads the
@@ -61,11 +62,11 @@ struct BlockNormParams {
 // by load latency (4.7 and more stalled cycles an instruction).
 constexpr int kBnStages = 3;
 constexpr int kBnRed = 4 * 24;       // team_sum: at most 4 teams of several warps
-constexpr int kBnCtas = 296;  // two CTAs on each of 148 SMs
+constexpr int kBnCtas = 296;  // two CTAs on each of 148 SMs (of 512 threads: one)
 constexpr int kBnRingBytes = 98304;  // a CTA's stages, where a row is not longer
 
 struct BlockNormTeams {
-  int wpr, vpt, rows_per_team, n_teams, n_ctas;
+  int wpr, vpt, threads, rows_per_team, n_teams, n_ctas;
   int rows_per_stage, smem;
 };
 // A pure function of the shape, so that the workspace query and the launch
@@ -73,19 +74,22 @@ struct BlockNormTeams {
 // A thread has two vectors where a row allows it (the reductions are then a
 // smaller part of its work), and one in the backward pass up to 2048 columns:
 // with two, the teams of fewer than 8 warps spill registers (16384 x 2048 with
-// dropout 121 us, with one 98 us).
+// dropout 121 us, with one 98 us).  Rows past 4096 columns take 16 warps: with 8
+// and four vectors a thread, one CTA an SM had too few warps (16384 x 8192 backward
+// 311 us, with dropout 367, so 258 and 314; forward 166, so 161).
 inline BlockNormTeams block_norm_teams(int rows, int cols, int tensors) {
   BlockNormTeams t;
   const int nvec = cols / 8;
   if (tensors == 4) {
-    t.vpt = nvec <= 256 ? 1 : nvec <= 512 ? 2 : 4;
-    t.wpr = nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 128 ? 4 : 8;
+    t.vpt = nvec <= 256 ? 1 : 2;
+    t.wpr = nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 128 ? 4 : nvec <= 512 ? 8 : 16;
   } else {
-    t.vpt = nvec <= 32 ? 1 : nvec <= 512 ? 2 : 4;
-    t.wpr = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
+    t.vpt = nvec <= 32 ? 1 : 2;
+    t.wpr = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : nvec <= 512 ? 8 : 16;
   }
-  const int teams = kBnWarps / t.wpr;
-  const int want = kBnCtas * teams;
+  t.threads = bn_warps(t.wpr) * 32;
+  const int teams = bn_teams(t.wpr);
+  const int want = (t.wpr == 16 ? kBnCtas / 2 : kBnCtas) * teams;
   t.rows_per_team = rows > 0 ? (int)(((long long)rows + want - 1) / want) : 1;
   t.n_teams = (int)(((long long)rows + t.rows_per_team - 1) / t.rows_per_team);
   t.n_ctas = (t.n_teams + teams - 1) / teams;
@@ -220,21 +224,25 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*red)[kBnRed], i
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
-    float* r = red[buf] + team * 24;  // 8 slots a value, WPR of them used
+    // 8 slots a value and team, WPR of them used (16 warps: two runs of 8 slots a value)
+    float* r = red[buf] + team * 24;
     buf ^= 1;
+    float* slot = r + (warp_in_team & 7) + (warp_in_team >> 3) * 24;
     if constexpr (NV == 3) {
-      if ((lane & 7) == 0 && lane < 24) r[lane + warp_in_team] = t;
+      if ((lane & 7) == 0 && lane < 24) slot[lane] = t;
       named_bar_sync(1 + team, WPR * 32);
       t = (lane < 24 && (lane & 7) < WPR) ? r[lane] : 0.0f;
+      if (WPR == 16 && lane < 24) t += r[24 + lane];
     } else {
-      if (lane == 0) r[warp_in_team] = t;
+      if (lane == 0) slot[0] = t;
       named_bar_sync(1 + team, WPR * 32);
       t = (lane & 7) < WPR ? r[lane & 7] : 0.0f;
+      if (WPR == 16) t += r[24 + (lane & 7)];
     }
 #pragma unroll
-    for (int o = WPR / 2; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
+    for (int o = (WPR < 8 ? WPR : 8) / 2; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) v[k] = NV == 1 && WPR == 8 ? t : __shfl_sync(ALL, t, 8 * k);
+    for (int k = 0; k < NV; ++k) v[k] = NV == 1 && WPR >= 8 ? t : __shfl_sync(ALL, t, 8 * k);
   }
 }
 
@@ -244,19 +252,19 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*red)[kBnRed], i
 // given (a block's usual case: no branches on them).  The weights stay in registers over the team's rows
 // (gate * w_post as their fp32 product, renewed where the gate's row changes).
 template <int WPR, int VPT, bool ALL>
-__global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(bn_warps(WPR) * 32, WPR <= 8 ? 2 : 1)
     block_norm_fwd_kernel(const BlockNormParams p, const BlockNormTeams tm) {
   constexpr int TT = WPR * 32;
   extern __shared__ uint4 bn_stages[];
   __shared__ float red[2][kBnRed];
   __shared__ uint4 zero_cell;
-  __shared__ uint64_t bars[kBnWarps * kBnStages];
+  __shared__ uint64_t bars[8 * kBnStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int team_in_cta = (int)threadIdx.x / TT, tid = (int)threadIdx.x % TT;
-  const int team = (int)blockIdx.x * (kBnWarps / WPR) + team_in_cta;
+  const int team = (int)blockIdx.x * bn_teams(WPR) + team_in_cta;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
+    for (int i = 0; i < 8 * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_word = 0;
     zero_cell = make_uint4(0, 0, 0, 0);
     fence_mbar_init();
@@ -408,19 +416,19 @@ struct BlockNormBwdParams {
 // gate row's rows of dv f r_f, the gate's gradient is w_post c, and c times
 // the gate's row adds to dw_post.
 template <int WPR, int VPT, bool ALL>
-__global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(bn_warps(WPR) * 32, WPR <= 8 ? 2 : 1)
     block_norm_bwd_kernel(const BlockNormBwdParams p, const BlockNormTeams tm) {
-  constexpr int TT = WPR * 32, TEAMS = kBnWarps / WPR;
+  constexpr int TT = WPR * 32, TEAMS = bn_teams(WPR);
   extern __shared__ uint4 bn_stages[];
   __shared__ float red[2][kBnRed];
   __shared__ uint4 zero_cell;
-  __shared__ uint64_t bars[kBnWarps * kBnStages];
+  __shared__ uint64_t bars[8 * kBnStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int team_in_cta = (int)threadIdx.x / TT, tid = (int)threadIdx.x % TT;
   const int team = (int)blockIdx.x * TEAMS + team_in_cta;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBnWarps * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
+    for (int i = 0; i < 8 * kBnStages; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_word = 0;
     zero_cell = make_uint4(0, 0, 0, 0);
     fence_mbar_init();
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
       }
       __syncthreads();
       float* dst = (which == 0 ? p.part_post : p.part_pre) + (long long)blockIdx.x * p.cols;
-      for (int c = threadIdx.x; c < p.cols; c += kBnThreads) {
+      for (int c = threadIdx.x; c < p.cols; c += TEAMS * TT) {
         float t = sums[c];
 #pragma unroll
         for (int w = 1; w < TEAMS; ++w) t += sums[w * p.cols + c];
@@ -680,9 +688,12 @@ __global__ void __launch_bounds__(kBnThreads, VPT <= 2 ? 2 : 1)
 
 // Sums the partials: output 0 is dw_post, 1 is dw_pre (a partial a CTA), 2 + g
 // the gate's row g where more than one team has rows of it (a partial a team).
-// 128 columns a block, four a lane; each of 16 warps takes every 16th partial,
-// and the warps' sums are joined in order.
+// 64 columns a block, four a thread; each of 32 groups of 16 threads takes every
+// 32nd partial, and the groups' sums are joined in order.  Bound by the latency of
+// a thread's loads: with 128 columns a block, and so twice as many, 4096 x 4096
+// takes 51.1 us for 49.4 and 1037 x 1000 10.4 for 9.5.
 constexpr int kBnSumThreads = 512;
+constexpr int kBnSumCols = 64;
 struct BlockNormSumParams {
   const float* part_post;
   const float* part_pre;
@@ -695,10 +706,10 @@ struct BlockNormSumParams {
 
 __global__ void __launch_bounds__(kBnSumThreads)
     block_norm_sum_kernel(const BlockNormSumParams p) {
-  constexpr int WARPS = kBnSumThreads / 32;
-  __shared__ float4 s[WARPS][32];
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int col = (int)blockIdx.x * 128 + lane * 4;
+  constexpr int LANES = kBnSumCols / 4, PARTS = kBnSumThreads / LANES;
+  __shared__ float4 s[PARTS][LANES];
+  const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
+  const int col = (int)blockIdx.x * kBnSumCols + lane * 4;
   const int outs = 2 + (p.dgate ? p.gate_rows : 0);
   pdl_wait();
   for (int o = blockIdx.y; o < outs; o += gridDim.y) {
@@ -727,7 +738,7 @@ __global__ void __launch_bounds__(kBnSumThreads)
     if (col < p.cols) {
       const float* at = src + col;
 #pragma unroll 8
-      for (int t = t0 + part; t <= t1; t += WARPS) {
+      for (int t = t0 + part; t <= t1; t += PARTS) {
         const float4 v =
             *reinterpret_cast<const float4*>(at + t * step + (t == inside ? p.cols : 0));
         acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
@@ -735,12 +746,12 @@ __global__ void __launch_bounds__(kBnSumThreads)
     }
     s[part][lane] = acc;
     __syncthreads();
-    const int c = (int)blockIdx.x * 128 + (int)threadIdx.x;
-    if (threadIdx.x < 128 && c < p.cols) {
+    const int c = (int)blockIdx.x * kBnSumCols + (int)threadIdx.x;
+    if (threadIdx.x < kBnSumCols && c < p.cols) {
       const float* f = reinterpret_cast<const float*>(s) + threadIdx.x;
       float v = f[0];
 #pragma unroll
-      for (int w = 1; w < WARPS; ++w) v += f[w * 128];
+      for (int w = 1; w < PARTS; ++w) v += f[w * kBnSumCols];
       dst[c] = __float2bfloat16_rn(v);
     }
     __syncthreads();

@@ -182,13 +182,13 @@ int ensure_device_setup() {
     TFB_BN_SET(2, 2, block_norm_fwd_kernel, bn_fwd);
     TFB_BN_SET(4, 2, block_norm_fwd_kernel, bn_fwd);
     TFB_BN_SET(8, 2, block_norm_fwd_kernel, bn_fwd);
-    TFB_BN_SET(8, 4, block_norm_fwd_kernel, bn_fwd);
+    TFB_BN_SET(16, 2, block_norm_fwd_kernel, bn_fwd);
     TFB_BN_SET(1, 1, block_norm_bwd_kernel, bn_bwd);
     TFB_BN_SET(2, 1, block_norm_bwd_kernel, bn_bwd);
     TFB_BN_SET(4, 1, block_norm_bwd_kernel, bn_bwd);
     TFB_BN_SET(8, 1, block_norm_bwd_kernel, bn_bwd);
     TFB_BN_SET(8, 2, block_norm_bwd_kernel, bn_bwd);
-    TFB_BN_SET(8, 4, block_norm_bwd_kernel, bn_bwd);
+    TFB_BN_SET(16, 2, block_norm_bwd_kernel, bn_bwd);
 #undef TFB_BN_SET
     // CTA pairs that fit at once (SMs pair up within a GPC; one CTA per SM)
     g_pair_clusters[dev] = g_num_sms[dev] / 2;
@@ -1452,7 +1452,7 @@ int block_norm_check(int rows, int cols, bool gate, int gate_rows, float eps, fl
 #define TFB_BN_FWD_DISPATCH(T, ALL, LAUNCH)            \
   do {                                                 \
     if ((T).vpt == 1) LAUNCH(1, 1, ALL);               \
-    else if ((T).vpt == 4) LAUNCH(8, 4, ALL);          \
+    else if ((T).wpr == 16) LAUNCH(16, 2, ALL);        \
     else if ((T).wpr == 1) LAUNCH(1, 2, ALL);          \
     else if ((T).wpr == 2) LAUNCH(2, 2, ALL);          \
     else if ((T).wpr == 4) LAUNCH(4, 2, ALL);          \
@@ -1460,8 +1460,8 @@ int block_norm_check(int rows, int cols, bool gate, int gate_rows, float eps, fl
   } while (0)
 #define TFB_BN_BWD_DISPATCH(T, ALL, LAUNCH)            \
   do {                                                 \
-    if ((T).vpt == 2) LAUNCH(8, 2, ALL);               \
-    else if ((T).vpt == 4) LAUNCH(8, 4, ALL);          \
+    if ((T).wpr == 16) LAUNCH(16, 2, ALL);             \
+    else if ((T).vpt == 2) LAUNCH(8, 2, ALL);          \
     else if ((T).wpr == 1) LAUNCH(1, 1, ALL);          \
     else if ((T).wpr == 2) LAUNCH(2, 1, ALL);          \
     else if ((T).wpr == 4) LAUNCH(4, 1, ALL);          \
@@ -1497,7 +1497,7 @@ extern "C" int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const v
   if (int e = ensure_device_setup()) return e;
   const BlockNormTeams t = block_norm_teams(rows, cols, 2);
 #define TFB_BN_FWD(W, V, A)                                                 \
-  block_norm_fwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem,  \
+  block_norm_fwd_kernel<W, V, A><<<(unsigned)t.n_ctas, (unsigned)t.threads, t.smem,  \
                                    static_cast<cudaStream_t>(stream)>>>(p, t)
   if (f && w_post && w_pre)
     TFB_BN_FWD_DISPATCH(t, true, TFB_BN_FWD);
@@ -1563,7 +1563,7 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   p.part_gate = p.part_pre + (size_t)t.n_ctas * cols;
   p.cyclic = !gate || p.rows_per_gate == 1 || gate_rows == 1;
 #define TFB_BN_BWD(W, V, A) \
-  block_norm_bwd_kernel<W, V, A><<<(unsigned)t.n_ctas, kBnThreads, t.smem, st>>>(p, t)
+  block_norm_bwd_kernel<W, V, A><<<(unsigned)t.n_ctas, (unsigned)t.threads, t.smem, st>>>(p, t)
   if (w_post && w_pre && dy && df)
     TFB_BN_BWD_DISPATCH(t, true, TFB_BN_BWD);
   else
@@ -1579,7 +1579,7 @@ extern "C" int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const v
   s.cols = cols, s.n_ctas = t.n_ctas, s.rows_per_team = t.rows_per_team;
   s.rows_per_gate = p.rows_per_gate, s.gate_rows = gate ? gate_rows : 0;
   const int outs = 2 + (s.dgate ? gate_rows : 0);
-  const dim3 sgrid((unsigned)((cols + 127) / 128), (unsigned)std::min(outs, 1024));
+  const dim3 sgrid((unsigned)((cols + kBnSumCols - 1) / kBnSumCols), (unsigned)std::min(outs, 1024));
   return launch_ex(block_norm_sum_kernel, sgrid, kBnSumThreads, 0, st, 0, 1, s);
 }
 
