@@ -820,10 +820,11 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
 }
 
 // What is done with four joined outputs v (FFN_GLU: and the four u beside
-// them) at row `row` of the output and column `col`.
+// them; FFN_STORE: the four of the residual in w) at row `row` of the output and
+// column `col`.
 template <int MODE>
 __device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, long long row, int col,
-                                               float (&v)[4], float (&u)[4]) {
+                                               float (&v)[4], float (&u)[4], uint2 w) {
   if constexpr (MODE == FFN_GLU) {
     if (p.z) {
       float* z = p.z + row * 2 * p.J + col;
@@ -833,7 +834,6 @@ __device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, long long
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = ffn_act_rt(p.act, v[i]) * u[i];
   } else if (p.residual) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p.residual + row * p.J + col);
     v[0] += __uint_as_float(w.x << 16);
     v[1] += __uint_as_float(w.x & 0xFFFF0000u);
     v[2] += __uint_as_float(w.y << 16);
@@ -844,8 +844,9 @@ __device__ __forceinline__ void ffn_tile_store(const FfnTileParams& p, long long
 
 // Joins this CTA's share of a tile: ROWS / S outputs of every token, four at a
 // time, summed over the S partial tiles in rank order.  A thread has 8 loads
-// of other CTAs' memory in flight: one after the other, they were half of a
-// small launch's time.
+// of other CTAs' memory in flight, and the residual's before its first store
+// (which may be to the residual itself): one after the other, they were half
+// of a small launch's time.
 template <int MODE, int S>
 __device__ __forceinline__ void ffn_join(const FfnTileParams& p, uint32_t part, int rank, int j0,
                                          int t0, int tokens) {
@@ -854,9 +855,16 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, uint32_t part, 
   const int n = R4 * tokens;
   for (int e0 = threadIdx.x; e0 < n; e0 += kTileThreads * U) {
     float4 a[U][S], b[U][S];
+    uint2 res[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int e = min(e0 + k * kTileThreads, n - 1);
+      if constexpr (MODE == FFN_STORE) {
+        const int col = j0 + (rank * R4 + e % R4) * 4;
+        if (p.residual && col < p.J)
+          res[k] = *reinterpret_cast<const uint2*>(p.residual +
+                                                   ((long long)t0 + e / R4) * p.J + col);
+      }
       const uint32_t mine = part + (uint32_t)((e / R4) * 128 + (rank * R4 + e % R4) * 4) * 4;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -879,7 +887,7 @@ __device__ __forceinline__ void ffn_join(const FfnTileParams& p, uint32_t part, 
         if constexpr (MODE == FFN_GLU)
           u[0] += b[k][s].x, u[1] += b[k][s].y, u[2] += b[k][s].z, u[3] += b[k][s].w;
       }
-      ffn_tile_store<MODE>(p, (long long)t0 + e / R4, col, v, u);
+      ffn_tile_store<MODE>(p, (long long)t0 + e / R4, col, v, u, res[k]);
     }
   }
 }
