@@ -23,9 +23,9 @@
 // backward (f, y, dy, dh, dx, df), everything else stays on the chip (16384 x
 // 4096: 86 us, 6.2 TB/s; backward 141, 5.7 TB/s, and with dropout 153, when the
 // generator's multiplies fill the issue slots).  A row belongs to a team of WPR
-// warps; all statistics and sums are fp32.  The column sums of the backward pass are accumulated in registers over a team's
-// contiguous rows, written as fp32 partials and summed in a fixed order by a
-// second kernel, so results repeat bit for bit.
+// warps; all statistics and sums are fp32.  The column sums of the backward pass
+// are accumulated in registers over a team's rows, written as fp32 partials and
+// summed in a fixed order by a second kernel, so results repeat bit for bit.
 #pragma once
 
 #include "norm_act.cuh"
@@ -249,9 +249,10 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*red)[kBnRed], i
 
 // ---------------------------------------------------------------- forward
 // VPT vectors a thread; a vector past the row's end reads zeros from `zero`, so
-// that nothing but the stores is predicated.  ALL: f, w_post and w_pre are
-// given (a block's usual case: no branches on them).  The weights stay in registers over the team's rows
-// (gate * w_post as their fp32 product, renewed where the gate's row changes).
+// that nothing but the stores is predicated.  ALL: f, w_post and w_pre are given
+// (a block's usual case: no branches on them).  The weights stay in registers over
+// the team's rows (gate * w_post as their fp32 product, renewed where the gate's
+// row changes).
 template <int WPR, int VPT, bool ALL>
 __global__ void __launch_bounds__(bn_warps(WPR) * 32, WPR <= 8 ? 2 : 1)
     block_norm_fwd_kernel(const BlockNormParams p, const BlockNormTeams tm) {
