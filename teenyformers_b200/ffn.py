@@ -10,10 +10,17 @@ scales on the branch, dropout.
     y  = residual_scale x + branch_scale dropout(gate * RMSNorm(f) * post_norm)
     hn = RMSNorm(y) * next_norm                    (what the next block reads)
 
-``post_norm``, ``gate`` and ``next_norm`` are optional.  Forward: three launches
-and a fourth for the first norm, which a caller that has h (the sublayer
-before's ``hn``) saves; any number of tokens, from one decoding token on.
-Backward: six, and a seventh where few tiles have their sums split.
+``post_norm``, ``gate`` and ``next_norm`` are optional.  Sublayers follow one another with
+``next_norm`` of one as ``norm`` of the next (one tensor, and one eps):
+
+    y1, h1, s1 = first.forward(x, train=True)
+    y2, h2, s2 = second.forward(y1, h=h1, train=True)
+    d1, g2 = second.backward(s2, dy2, dh2)     # h1's gradient is in d1, the norm's is g2["norm"]
+    dx, g1 = first.backward(s1, d1)
+
+Forward: three launches and a fourth for the first norm, which a caller that has h
+(the sublayer before's ``hn``) saves; any number of tokens, from one decoding token
+on.  Backward: six, and a seventh where few tiles have their sums split.
 """
 from __future__ import annotations
 
@@ -55,11 +62,15 @@ class FeedForwardSublayer:
 
     def backward(self, saved, dy: torch.Tensor | None, dhn: torch.Tensor | None = None,
                  rng: torch.Tensor | None = None):
-        """(dx, gradients by the weights' names) from the gradients of y and hn (dy None:
-        zero; dhn with next_norm), the forward's third result and its rng."""
+        """(dx, gradients by the weights' names) from the gradients of y and hn (None: zero,
+        but not both), the forward's third result and its rng.  dx and the norm's gradient
+        are of x alone, whoever computed h.  dhn None, where hn was not used or where the
+        sublayer that took it has its gradient in dy: no gradient of next_norm."""
         x, h, f, y, z = saved
         w = self.w
         post, gate, nxt = self._around()
+        if dhn is None:
+            nxt = None
         # (f is not needed for its own gradient without a norm or gate after the block)
         dres, df, dpost, dgate, dnext = self.norm.backward(
             f if post is not None or gate is not None else None, y, dy, dhn, post, gate, nxt,
