@@ -340,7 +340,8 @@ TF_API int tf_b200_block_norm_bwd_bf16(const void* f, const void* y, const void*
  * element i is kept iff its 16 bits are below t.  The bits are those of Philox4x32-10 (Salmon,
  * Moraes, Dror, Shaw, 2011) with key `seed` and counter (i / 8, site, offset low, offset high);
  * element i has half i % 8 of the 128 bits, low halves first.  The probability is so rounded to a
- * multiple of 2^-16, and the scale belongs to the rounded one.
+ * multiple of 2^-16, and the scale belongs to the rounded one.  p is the 32-bit number passed: a
+ * caller whose p has 64 bits computes t from that and passes 1 - t / 65536, which 32 bits hold.
  * The backward pass is the same call on the gradient.  rng: device pointer to (seed, offset), two
  * 64-bit words, read when the kernel runs, so a captured graph draws new masks when they change.
  * n <= 2^35; x, residual (or NULL) and y are 16-byte aligned and may be the same buffer.

@@ -468,6 +468,14 @@ def _rng_addr(p: float, rng: torch.Tensor | None, site: int, x: torch.Tensor):
     return rng.data_ptr()
 
 
+def _drop_p(p: float) -> float:
+    """p for the C ABI, which takes 32 bits: the multiple of 2^-16 that is drawn, rounded from
+    the caller's 64-bit p (p rounded to 32 bits first may give the next one).  It is exact in
+    32 bits, and rounds to itself there."""
+    p = float(p)
+    return 1.0 - math.floor((1.0 - p) * 65536.0 + 0.5) / 65536.0 if 0.0 <= p <= 1.0 else p
+
+
 def _workspace(n: int, ws: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
     if ws is None:
         return x.new_empty(n, dtype=torch.uint8)
@@ -493,7 +501,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0,
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
     y = torch.empty_like(x) if out is None else _buffer(out, x.shape, x.dtype, x, "out")
     _launch(x, fn, x.data_ptr(), _addr(residual), y.data_ptr(), _rng_addr(p, rng, site, x),
-            x.numel(), float(p), int(site))
+            x.numel(), _drop_p(p), int(site))
     return y
 
 
@@ -539,7 +547,7 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None, w_post: torch.Tensor | N
     h = None if w_pre is None else _buffer(norm_out, x.shape, x.dtype, x, "norm_out")
     _launch(x, "tf_b200_block_norm_fwd_bf16", x.data_ptr(), _addr(f), _addr(w_post), _addr(gate),
             _addr(w_pre), y.data_ptr(), _addr(h), _rng_addr(p, rng, site, x), rows, cols, gate_rows,
-            float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
+            float(eps), float(residual_scale), float(branch_scale), _drop_p(p), int(site))
     return y, h
 
 
@@ -576,7 +584,7 @@ def block_norm_bwd(f: torch.Tensor | None, y: torch.Tensor | None, dy: torch.Ten
     _launch(like, "tf_b200_block_norm_bwd_bf16", _addr(f), _addr(y), _addr(dy), _addr(dh),
             _addr(w_post), _addr(gate), _addr(w_pre), dx.data_ptr(), _addr(df), _addr(dw_post),
             _addr(dgate), _addr(dw_pre), _rng_addr(p, rng, site, like), ws.data_ptr(), rows, cols,
-            gate_rows, float(eps), float(residual_scale), float(branch_scale), float(p), int(site))
+            gate_rows, float(eps), float(residual_scale), float(branch_scale), _drop_p(p), int(site))
     return dx, df, dw_post, dgate, dw_pre
 
 
