@@ -409,11 +409,13 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
     x [..., d] bf16; w_gate_up [2 * d_ff, d] = [Wg; Wu] (the layer's layout); w_down
     [d, d_ff]; act TF_ACT_SILU / GELU / GELU_TANH.  ``save`` also returns z
     [..., 2 * d_ff] fp32 = x [Wg; Wu]^T for gated_ffn_bwd.  ``out``, ``act_out``
-    ([..., d_ff] scratch) and ``z_out`` are buffers to use instead of new ones."""
+    ([..., d_ff] scratch) and ``z_out`` (with ``save``) are buffers to use instead of
+    new ones."""
     m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
     lead = x.shape[:-1]
     _dense(x, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, residual)
     _need(residual is None or residual.shape == x.shape, "residual must have x's shape")
+    _need(save or z_out is None, "z_out is written with save=True only")
     y = torch.empty_like(x) if out is None else _buffer(out, x.shape, torch.bfloat16, x, "out")
     a = _buffer(act_out, lead + (d_ff,), torch.bfloat16, x, "act_out")
     z = _buffer(z_out, lead + (2 * d_ff,), torch.float32, x, "z_out") if save else None
@@ -539,10 +541,12 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None, w_post: torch.Tensor | N
     x (residual stream) and f (the block's output) [..., cols] bf16; w_post, w_pre
     [cols] or None (no norm there); gate [gate_rows, cols] or None, one row for
     every rows / gate_rows consecutive rows.  f None: only the norm before a block
-    (y is x).  Returns (y, h), h None without w_pre.  ``out`` may be x."""
+    (y is x, and ``out`` is refused).  Returns (y, h), h None without w_pre, when a
+    ``norm_out`` is left as it was.  ``out`` may be x."""
     rows, cols, gate_rows = _norm_shapes(x, w_post, gate, w_pre)
     _dense(x, torch.bfloat16, "block_norm", x, f, w_post, gate, w_pre)
     _need(f is None or f.shape == x.shape, "f must have x's shape")
+    _need(f is not None or out is None, "without f, y is x: out is not written")
     y = x if f is None else _buffer(out, x.shape, x.dtype, x, "out")
     h = None if w_pre is None else _buffer(norm_out, x.shape, x.dtype, x, "norm_out")
     _launch(x, "tf_b200_block_norm_fwd_bf16", x.data_ptr(), _addr(f), _addr(w_post), _addr(gate),
