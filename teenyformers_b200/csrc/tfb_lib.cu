@@ -1205,7 +1205,9 @@ int ffn_check(int m, int d_model, int d_ff, int act) {
   if (m < 0 || d_model < 0 || d_ff < 0) return TF_ERR_INVALID_ARG;
   if (act < TF_ACT_SILU || act > TF_ACT_GELU_TANH) return TF_ERR_INVALID_ARG;
   if (d_model % 8 != 0 || d_ff % 8 != 0) return TF_ERR_UNSUPPORTED;
-  if (!fits_i32(2LL * d_ff)) return TF_ERR_TOO_LARGE;
+  // extents are rounded up to whole tiles of 256 in 32 bits
+  for (const long long v : {(long long)m, (long long)d_model, 2LL * d_ff})
+    if (!fits_i32(v + 255)) return TF_ERR_TOO_LARGE;
   // tiles of every product (128 x 64 at the smallest, up to eight runs of K)
   const long long mt = (m + 127LL) / 128, dt = (d_model + 63LL) / 64, ft = (d_ff + 31LL) / 32;
   if (!fits_i32(mt * dt) || !fits_i32(mt * ft) || !fits_i32(dt * ft)) return TF_ERR_TOO_LARGE;
