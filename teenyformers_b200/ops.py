@@ -390,13 +390,21 @@ def _buffer(t: torch.Tensor | None, shape, dtype: torch.dtype, x: torch.Tensor,
     return t
 
 
+def _rows(x: torch.Tensor, cols: int) -> int:
+    rows = x.numel() // (cols or 1)
+    if rows >= 1 << 31 or cols >= 1 << 31:  # (a C int would take the low 32 bits)
+        raise ValueError(f"{rows} rows of {cols}: at most 2^31 - 1 each")
+    return rows
+
+
 def _ffn_shapes(x, w_gate_up, w_down):
     _need(x.is_cuda and x.dim() >= 1 and w_gate_up.dim() == 2 and w_down.dim() == 2,
           "x must be a [..., d] CUDA tensor, w_gate_up and w_down matrices")
     d_ff, d = w_down.shape[1], w_down.shape[0]
     _need(x.shape[-1] == d and tuple(w_gate_up.shape) == (2 * d_ff, d),
           "expected x [..., d], w_gate_up [2 * d_ff, d], w_down [d, d_ff]")
-    return x.numel() // max(d, 1), d, d_ff
+    _need(d_ff < 1 << 31, "d_ff must be below 2^31")
+    return _rows(x, d), d, d_ff
 
 
 def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
@@ -511,7 +519,7 @@ def _norm_shapes(x, w_post, gate, w_pre):
     if not x.is_cuda or x.dim() < 1:
         raise ValueError("block_norm tensors must be [..., cols] CUDA tensors")
     cols = x.shape[-1]
-    rows = x.numel() // (cols or 1)
+    rows = _rows(x, cols)
     if (w_post is not None and w_post.numel() != cols) or (
             w_pre is not None and w_pre.numel() != cols):
         raise ValueError("a norm's weight must have the last dim's size")
