@@ -295,7 +295,8 @@ TF_API int tf_b200_gated_ffn_fwd_bf16(const void* x, const void* w_gate_up, cons
  *   dx = [dg | du] [Wg; Wu], dw_gate_up = [dg | du]^T x, dw_down = dy^T a   (bf16, rounded once;
  *   fully written, repeatable bit for bit).
  * z: the forward's; a is computed again from it.  dx NULL skips it; dw_gate_up and dw_down are
- * given or NULL each.  workspace: tf_b200_gated_ffn_bwd_workspace_size(...) bytes, 16-byte
+ * given or NULL each.  No result may lie over x, dy or w_gate_up where another of the results
+ * needs it (x: dw_gate_up, dy: dw_down, w_gate_up: dx).  workspace: tf_b200_gated_ffn_bwd_workspace_size(...) bytes, 16-byte
  * aligned.  m == 0: the weights' gradients are zero. */
 TF_API size_t tf_b200_gated_ffn_bwd_workspace_size(int m, int d_model, int d_ff);
 TF_API int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, const void* w_down,

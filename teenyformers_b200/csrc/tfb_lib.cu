@@ -1343,6 +1343,17 @@ extern "C" int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, 
   }
   if (!x || !w_gate_up || !w_down || !z || !dy || !workspace) return TF_ERR_INVALID_ARG;
   if (!dx && !dw_gate_up && !dw_down) return TF_OK;
+  // one launch writes the three results and reads what the other two are made of
+  const size_t x_bytes = (size_t)m * d_model * 2, w_bytes = (size_t)d_ff * d_model * 2;
+  const struct { const void* p; size_t n; } writes[3] = {{dx, x_bytes}, {dw_gate_up, 2 * w_bytes},
+                                                         {dw_down, w_bytes}},
+      reads[3] = {{dx ? w_gate_up : nullptr, 2 * w_bytes}, {dw_gate_up ? x : nullptr, x_bytes},
+                  {dw_down ? dy : nullptr, x_bytes}};
+  for (const auto& w : writes)
+    for (const auto& r : reads) {
+      const uintptr_t a = (uintptr_t)w.p, b = (uintptr_t)r.p;
+      if (a && b && a < b + r.n && b < a + w.n) return TF_ERR_INVALID_ARG;
+    }
   if (int e = ensure_device_setup()) return e;
   __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(workspace);
   __nv_bfloat16* a = dz + (size_t)m * 2 * d_ff;

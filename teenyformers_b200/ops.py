@@ -443,7 +443,8 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor
                   workspace: torch.Tensor | None = None):
     """(dx, dw_gate_up, dw_down) of gated_ffn from z (gated_ffn(..., save=True)) and dy;
     a False in ``need`` skips that gradient (None in its place).  The residual's
-    gradient is dy itself.  ``grads``: three tensors to write instead of new ones."""
+    gradient is dy itself.  ``grads``: three tensors to write instead of new ones (dx over
+    x or dy only where dw_gate_up or dw_down, which read them, is skipped)."""
     m, d, d_ff = _ffn_shapes(x, w_gate_up, w_down)
     _dense(x, torch.bfloat16, "gated_ffn", x, w_gate_up, w_down, dy)
     _dense(x, torch.float32, "z", z)
