@@ -314,7 +314,8 @@ TF_API int tf_b200_gated_ffn_bwd_bf16(const void* x, const void* w_gate_up, cons
  * tf_b200_rmsnorm_bf16 (fused_add_rmsnorm.rs:53-110).  y may be x.
  * Dropout: drop_p is the probability of dropping, 0 for none; rng is a device pointer to two
  * 64-bit words (seed, offset), 8-byte aligned (NULL only when drop_p == 0); `site` tells the
- * dropouts of one step apart.  See tf_b200_dropout_bf16.
+ * dropouts of one step apart.  See tf_b200_dropout_bf16.  (A NaN in a row of f under w_post makes
+ * that whole row of y NaN, the dropped places included.)
  * cols % 8 == 0, <= 8192. */
 TF_API int tf_b200_block_norm_fwd_bf16(const void* x, const void* f, const void* w_post,
                                        const void* gate, const void* w_pre, void* y, void* h,

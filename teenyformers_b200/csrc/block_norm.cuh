@@ -6,6 +6,8 @@
 //   y = residual_scale * x + branch_scale * v        (f null: y = x, not written)
 //   h = RMSNorm(y) * w_pre             (w_pre null: no h)
 //
+// A NaN of f under w_post makes its row's inverse RMS and so the whole row of y NaN, the
+// dropped places included; without w_post what is dropped leaves nothing behind.
 // RMSNorm(v) = v * rsqrt(mean(v^2) + eps) over the row.  f is a block's output,
 // x the residual stream, h what the next block reads.  The gate has one row
 // for every rows / gate_rows consecutive rows of x (one for all, one a
@@ -21,8 +23,10 @@
 //
 // Both passes are HBM-bound: 8 bytes an element forward (x, f, y, h), 12
 // backward (f, y, dy, dh, dx, df), everything else stays on the chip (16384 x
-// 4096: 86 us, 6.2 TB/s; backward 141, 5.7 TB/s, and with dropout 153, when the
-// generator's multiplies fill the issue slots).  A row belongs to a team of WPR
+// 4096, whole calls on inputs from memory: 90 us, 5.9 TB/s, with 8 gate rows and 102
+// with one or none; backward 138-144, 5.7 TB/s, and with dropout 164-169, when the
+// generator's rounds stand between a row's loads and its stores: 58 % of the issue
+// slots are taken, it is latency).  A row belongs to a team of WPR
 // warps; all statistics and sums are fp32.  The column sums of the backward pass
 // are accumulated in registers over a team's rows, written as fp32 partials and
 // summed in a fixed order by a second kernel, so results repeat bit for bit.
@@ -77,7 +81,8 @@ struct BlockNormTeams {
 // with two, the teams of fewer than 8 warps spill registers (16384 x 2048 with
 // dropout 121 us, with one 98 us).  Rows past 4096 columns take 16 warps: with 8
 // and four vectors a thread, one CTA an SM had too few warps (16384 x 8192 backward
-// 311 us, with dropout 367, so 258 and 314; forward 166, so 161).
+// 311 us, with dropout 367, so 258 and 314; forward 166, so 161; on inputs from memory
+// the latter are 276-290, 333 and 174).
 inline BlockNormTeams block_norm_teams(int rows, int cols, int tensors) {
   BlockNormTeams t;
   const int nvec = cols / 8;

@@ -32,7 +32,7 @@ __device__ __forceinline__ void dropout_put(float* p, float v) { *p = v; }
 // through a ring of shared-memory stages filled by bulk copies, so that loads
 // run on under the generator's arithmetic.  With plain loads, 16384 x 4096
 // bf16 with a residual took 89 us (18 stalled cycles an instruction waiting
-// for loads), and 126 us with four groups' loads in flight a thread; so 72 us.
+// for loads), and 126 us with four groups' loads in flight a thread; so 71-74 us.
 constexpr int kDropStages = 4;
 constexpr int kDropChunkBytes = 8192;
 constexpr int kDropSmem = kDropStages * 2 * kDropChunkBytes;

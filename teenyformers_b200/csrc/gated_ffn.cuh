@@ -42,9 +42,9 @@ enum FfnAct : int { FFN_ACT_SILU = 0, FFN_ACT_GELU = 1, FFN_ACT_GELU_TANH = 2 };
 // the polynomial of degree 6 with the least largest relative error of t P(t) against
 // erfc(x) exp(x^2) / 2 over x = 0 .. 10 (6.0e-7; fitted by linear programming).  The error
 // is relative, so that the tail keeps its digits: with t, E and the sum in fp32 it stays
-// below 5e-6 to g = -13, where E leaves fp32 (the Handbook's 7.1.26, whose bound is on the
-// absolute error, is off by 0.25 % at g = -5.5 and 1 % at -8, more than the bf16 rounding
-// behind it).  It shares its exponential with the slope's density and has no branch.
+// below 5e-6 to g = -13, where E leaves fp32 (7.1.26 of Abramowitz and Stegun's Handbook,
+// whose bound is on the absolute error, is off by 0.25 % at g = -5.5 and 1 % at -8, more
+// than the bf16 rounding behind it).  It shares its exponential with the slope's density and has no branch.
 __device__ __forceinline__ float ffn_phi(float g, float& E) {
   const float x = fabsf(g) * 0.70710678118654752f;
   const float t = __fdividef(1.0f, fmaf(0.375f, x, 1.0f));

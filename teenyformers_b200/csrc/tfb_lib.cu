@@ -1303,7 +1303,8 @@ FfnBwdPlan ffn_bwd_plan(int m, int d, int F) {
   for (int i = 0; i < 3; ++i) {
     p.ks[i] = 1;
     // it has to be worth the launch that joins the sums: with 16 k-blocks here a
-    // step of 1111 x 520 x 1416 lost 3 us by it, with 28 777 x 1032 x 2776 gains 6
+    // step of 1111 x 520 x 1416 lost 3 us by it, with 28 777 x 1032 x 2776 gains 6 (nothing
+    // between the two was measured)
     if (kblk[i] > even + 28.0) {
       const double most = std::min({8.0, kPairs / tiles[i], kblk[i] / 8.0});
       p.ks[i] = std::max(1, (int)std::min(most, std::ceil(kblk[i] / even)));
